@@ -267,10 +267,9 @@ def _encode(x, bits16, bias, top, signed):
     size = x.abs().reshape(-1, BLOCK)
     size_or_0 = torch.where(torch.isfinite(size), size, 0.0)
     scale = ((size_or_0.amax(1).view(torch.int32) >> 23) - top).clamp(min=1)
-    t = (size * ((254 - scale) << 23).view(F32).unsqueeze(1)).reshape(-1)
-    low = torch.floor(t * 2.0 ** (bias + 2) + bits16.to(F32) * 2.0 ** -16).clamp(max=8.0).nan_to_num().to(torch.int32)
-    high = ((t.view(torch.int32) + (bits16.to(torch.int32) << 4)) >> 20) - ((127 - bias) << 3)
-    code = torch.where(t < 2.0 ** (1 - bias), low, high)
+    # below 2^-126 the exponent field is 0 and the bits are those of a fixed point: the format's own subnormals
+    t = (size * ((254 - scale) << 23).view(F32).unsqueeze(1)).reshape(-1) * 2.0 ** (bias - 127)
+    code = (t.view(torch.int32) + (bits16.to(torch.int32) << 4)) >> 20
     if not signed:
         code = torch.where((x > 0) & (code < 1), 1, code)     # what is above nothing stays above nothing
     code = torch.where(torch.isfinite(x), code, 0x7F if signed else 0xFF)
@@ -283,8 +282,7 @@ def _decode(held, bias, signed):
     code, scale = held[0].to(torch.int32), held[1].to(torch.int32)
     sign = 1.0 - 2.0 * (code >> 7).to(F32) if signed else 1.0
     code = code & 0x7F if signed else code
-    fine = ((code + ((127 - bias) << 3)) << 20).view(F32)
-    value = torch.where(code < 8, code.to(F32) * 2.0 ** (-2 - bias), fine)
+    value = (code << 20).view(F32) * 2.0 ** (127 - bias)
     value = torch.where(code == (0x7F if signed else 0xFF), torch.nan, value)
     return sign * (value.reshape(-1, BLOCK) * (scale << 23).view(F32).unsqueeze(1)).reshape(-1)
 
