@@ -177,6 +177,68 @@ int mcrn_flat_clip_adam(float* p, float* g, float* m, float* v, long long n, flo
                         float beta2, float eps, int step, float max_norm, float grad_scale,
                         float* scratch, float* total_norm_out, void* stream);
 
+/* ---- gated linear recurrence: the recurrent cell (model/MegaCRN.py:38-48) with gate and candidate that do not read the
+ *      state, so that a whole sequence is one scan ----
+ *   a = sigmoid(gate), c = phi(cand):   h_t = a_t h_{t-1} + (1 - a_t) c_t ;   a step whose mask byte is 0 keeps the state
+ *   (its gate and cand may hold anything; their gradients there are 0).
+ * gate (B,T,N,G), cand (B,T,N,H), G divides H (gate j is shared by the channels j*H/G .. (j+1)*H/G - 1), mask (B,T,N) bytes
+ * or NULL: any strides (in elements, >= 0) over B, T and N, the last dimension of gate and cand contiguous.  state (B,N,H)
+ * fp32 or NULL (zeros).  out (B,T,N,H) of the inputs' type, last (B,N,H) fp32.  Arithmetic and states are fp32.
+ * B, T, N may be 0.  T <= 2^30. */
+#define MCRN_T_F32 0
+#define MCRN_T_BF16 1
+#define MCRN_T_F16 2
+#define MCRN_ACT_NONE 0 /* phi(c) = c */
+#define MCRN_ACT_TANH 1
+typedef struct mcrn_glr {
+    int B, T, N, H, G;
+    int dtype;          /* MCRN_T_*: of gate, cand, out, dout, dgate, dcand */
+    int activation;     /* MCRN_ACT_* */
+    int reserved;       /* 0 */
+    long long gate_s[3], cand_s[3], mask_s[3], dout_s[3];   /* strides over B, T, N */
+} mcrn_glr_t;
+/* Checkpoints that a 16-bit forward leaves for its backward: floats of `ckpt` (0 for MCRN_T_F32, whose backward reads `out`). */
+size_t mcrn_glr_checkpoint_floats(const mcrn_glr_t* d);
+size_t mcrn_glr_workspace_bytes(const mcrn_glr_t* d, int backward);
+/* out, last and ckpt may be NULL (not wanted).  last may be state itself: the state is then advanced in place. */
+int mcrn_glr_forward(const mcrn_glr_t* d, const void* gate, const void* cand, const unsigned char* mask, const float* state,
+                     void* ws, size_t ws_bytes, void* out, float* last, float* ckpt, void* stream);
+/* kept: `out` (MCRN_T_F32) or `ckpt` (16-bit types) of the forward call.  dout (strides dout_s), dlast: NULL = zeros; dstate: NULL =
+ * not wanted.  dgate, dcand, dstate are overwritten, contiguous. */
+int mcrn_glr_backward(const mcrn_glr_t* d, const void* gate, const void* cand, const unsigned char* mask, const float* state,
+                      const void* kept, const void* dout, const float* dlast, void* ws, size_t ws_bytes, void* dgate,
+                      void* dcand, float* dstate, void* stream);
+
+/* ---- AdamW over many tensors, beside the flat clip + Adam above ----
+ *   g' = factor g, factor = grad_scale * min(1, max_norm / (|| grad_scale g || + 1e-6)) over ALL tensors (max_norm <= 0: grad_scale)
+ *   m = b1 m + (1 - b1) g' ; v = b2 v + (1 - b2) g' g' ; p = (1 - lr wd) p - lr / (1 - b1^s) * m / (sqrt(v) / sqrt(1 - b2^s) + eps)
+ * Tensors are contiguous, fp32, or bf16 with fp32 masters that carry the update (p = their rounding).  The moments of all
+ * tensors lie in two arenas in the tensors' order, each tensor filled up with zeros to whole blocks of 64 elements
+ * (mcrn_adamw_arena_elements): fp32, or one byte an element and one scale byte a block (value = code * 2^(scale - 127); m: sign, 4
+ * exponent bits (bias 7), 3 mantissa bits; v: 5 exponent bits (bias 15), 3 mantissa bits; 0x7f and 0xff: NaN).  8-bit moments are
+ * rounded stochastically by bits that are a function of (seed, tensor, step, element). */
+typedef struct mcrn_adamw {
+    int ntensors;
+    int dtype;              /* MCRN_T_F32 or MCRN_T_BF16: parameters and gradients */
+    int state_bits;         /* 32 or 8 */
+    unsigned seed;
+    int on_device;          /* 0: lr, weight_decay, step are host arrays.  1: device arrays, read when the kernels run and `step`
+                               counted up by the call, so that a captured call can be replayed */
+    int reserved;           /* 0 */
+    double beta1, beta2, eps, max_norm, grad_scale;
+} mcrn_adamw_t;
+long long mcrn_adamw_arena_elements(const mcrn_adamw_t* a, const long long* numel);
+/* Zero-filled once by the caller; belongs to one sequence of steps (word 0 counts arrivals and is left at 0). */
+size_t mcrn_adamw_workspace_bytes(const mcrn_adamw_t* a, const long long* numel);
+/* params, grads: host arrays of device pointers; grads[i] == NULL leaves tensor i and its moments as they are.
+ * lr, weight_decay: doubles, step: int, one of each for every tensor; step is 1-based and is that of this update (on_device: the number of
+ * updates so far).  m_scale, v_scale: 8-bit moments only; master: bf16 only.  total_norm: device float or NULL. */
+int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* const* grads, const long long* numel,
+                    const double* lr, const double* weight_decay, int* step, void* m, void* v, unsigned char* m_scale,
+                    unsigned char* v_scale, float* master, void* ws, size_t ws_bytes, float* total_norm, void* stream);
+/* The values that n codes stand for (n a multiple of 64): second = 0 for m, 1 for v. */
+int mcrn_adamw_unpack(const unsigned char* codes, const unsigned char* scale, long long n, int second, float* out, void* stream);
+
 /* ---- trainer loss, forward + backward (model/traintest_MegaCRN.py:118-125, model/utils.py:126-133) ----
  * loss = masked_mae(output*std+mean, labels*std+mean) + lamb*TripletMarginLoss(margin)(query,pos,neg)
  *        + lamb1*MSELoss(query,pos), pos/neg treated as constants (the trainer detaches them).

@@ -24,6 +24,8 @@ EXPORTS = [
     "mcrn_cell_workspace_bytes", "mcrn_cell_forward", "mcrn_cell_backward",
     "mcrn_memory_workspace_bytes", "mcrn_memory_forward", "mcrn_memory_backward",
     "mcrn_flat_clip_adam", "mcrn_loss_fwd_bwd", "mcrn_eval_metrics", "mcrn_gemm_f32", "mcrn_prof_begin", "mcrn_prof_end", "mcrn_prof_clock_mhz", "mcrn_set_gemm_cfg", "mcrn_set_debug", "mcrn_model_autotune", "mcrn_autotune_entries", "mcrn_autotune_clear", "mcrn_autotune_export", "mcrn_autotune_import", "mcrn_set_precision", "mcrn_get_precision", "mcrn_set_side_stream",
+    "mcrn_glr_checkpoint_floats", "mcrn_glr_workspace_bytes", "mcrn_glr_forward", "mcrn_glr_backward",
+    "mcrn_adamw_arena_elements", "mcrn_adamw_workspace_bytes", "mcrn_adamw_step", "mcrn_adamw_unpack",
 ]
 
 
@@ -50,6 +52,20 @@ class Params(C.Structure):
 
 class Grads(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in PARAM_FIELDS]
+
+
+class Glr(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("B", "T", "N", "H", "G", "dtype", "activation", "reserved")]
+                + [(n, C.c_longlong * 3) for n in ("gate_s", "cand_s", "mask_s", "dout_s")])
+
+
+class Adamw(C.Structure):
+    _fields_ = [("ntensors", C.c_int), ("dtype", C.c_int), ("state_bits", C.c_int), ("seed", C.c_uint), ("on_device", C.c_int),
+                ("reserved", C.c_int)] + [(n, C.c_double) for n in ("beta1", "beta2", "eps", "max_norm", "grad_scale")]
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # MCRN_T_*
+ACTIVATIONS = {"none": 0, "tanh": 1}                                    # MCRN_ACT_*
 
 
 def _load():
@@ -134,6 +150,22 @@ def _load():
                                   C.POINTER(C.c_double)]
     lib.mcrn_prof_clock_mhz.restype = i
     lib.mcrn_prof_clock_mhz.argtypes = [C.POINTER(C.c_double), C.POINTER(C.c_longlong)]
+    lib.mcrn_glr_checkpoint_floats.restype = sz
+    lib.mcrn_glr_checkpoint_floats.argtypes = [C.POINTER(Glr)]
+    lib.mcrn_glr_workspace_bytes.restype = sz
+    lib.mcrn_glr_workspace_bytes.argtypes = [C.POINTER(Glr), i]
+    lib.mcrn_glr_forward.restype = i
+    lib.mcrn_glr_forward.argtypes = [C.POINTER(Glr)] + [vp] * 4 + [vp, sz] + [vp] * 3 + [vp]
+    lib.mcrn_glr_backward.restype = i
+    lib.mcrn_glr_backward.argtypes = [C.POINTER(Glr)] + [vp] * 7 + [vp, sz] + [vp] * 3 + [vp]
+    lib.mcrn_adamw_arena_elements.restype = ll
+    lib.mcrn_adamw_arena_elements.argtypes = [C.POINTER(Adamw), C.POINTER(ll)]
+    lib.mcrn_adamw_workspace_bytes.restype = sz
+    lib.mcrn_adamw_workspace_bytes.argtypes = [C.POINTER(Adamw), C.POINTER(ll)]
+    lib.mcrn_adamw_step.restype = i
+    lib.mcrn_adamw_step.argtypes = [C.POINTER(Adamw), C.POINTER(vp), C.POINTER(vp), C.POINTER(ll)] + [vp] * 8 + [vp, sz, vp, vp]
+    lib.mcrn_adamw_unpack.restype = i
+    lib.mcrn_adamw_unpack.argtypes = [vp, vp, ll, i, vp, vp]
     return lib
 
 

@@ -25,6 +25,8 @@
 #include "gemm_bf16_api.h"
 #include "wgrad_stream_api.h"
 #include "wp_stream_api.h"
+#include "glr_scan_api.h"
+#include "adamw_multi_api.h"
 #include "ops.h"
 
 namespace mcrn {
@@ -2916,6 +2918,224 @@ int mcrn_flat_clip_adam(float* p, float* g, float* m, float* v, long long n, flo
     const float bc2s = (float)sqrt(1.0 - pow((double)beta2, (double)step));
     LAUNCH(k_clip_adam, dim3(cdiv(n, 256)), dim3(256), 0, st, p, g, m, v, n, lr, beta1, beta2, eps, bc1, bc2s, max_norm,
            grad_scale, (const float*)(scratch + 1000), total_norm_out);
+    return 0;
+}
+
+// ---- gated linear recurrence ------------------------------------------------------------------------
+static bool glr_params(const mcrn_glr_t* d, GlrP& p) {
+    if (!d || d->B < 0 || d->T < 0 || d->T > (1 << 30) || d->N < 0 || d->H < 1 || d->G < 1 || d->H % d->G || d->dtype < MCRN_T_F32 || d->dtype > MCRN_T_F16 ||
+        (d->activation != MCRN_ACT_NONE && d->activation != MCRN_ACT_TANH) || d->reserved)
+        return false;
+    for (int i = 0; i < 3; ++i)
+        if (d->gate_s[i] < 0 || d->cand_s[i] < 0 || d->mask_s[i] < 0 || d->dout_s[i] < 0) return false;
+    memset(&p, 0, sizeof p);
+    p.B = d->B; p.T = d->T; p.N = d->N; p.H = d->H; p.G = d->G; p.dtype = d->dtype; p.act = d->activation;
+    p.g_sb = d->gate_s[0]; p.g_st = d->gate_s[1]; p.g_sn = d->gate_s[2];
+    p.c_sb = d->cand_s[0]; p.c_st = d->cand_s[1]; p.c_sn = d->cand_s[2];
+    p.m_sb = d->mask_s[0]; p.m_st = d->mask_s[1]; p.m_sn = d->mask_s[2];
+    p.d_sb = d->dout_s[0]; p.d_st = d->dout_s[1]; p.d_sn = d->dout_s[2];
+    return true;
+}
+size_t mcrn_glr_checkpoint_floats(const mcrn_glr_t* d) {
+    GlrP p;
+    if (!glr_params(d, p) || p.dtype == GLR_F32 || p.T < 1) return 0;
+    return (size_t)p.B * ((p.T - 1) / GLR_K) * p.N * p.H;
+}
+size_t mcrn_glr_workspace_bytes(const mcrn_glr_t* d, int backward) {
+    GlrP p;
+    if (!glr_params(d, p) || (long long)p.B * p.N == 0) return 0;
+    size_t most = 0;
+    for (p.one = 0; p.one < 2; ++p.one)        // the alignment of the pointers decides between the two
+        if (glr_plan(p, backward != 0)) most = std::max(most, glr_ws_bytes(p, backward != 0));
+    return most;
+}
+// places the workspace behind the plan
+static bool glr_place(GlrP& p, bool backward, void* ws, size_t ws_bytes) {
+    const size_t need = glr_ws_bytes(p, backward);
+    if (!need) return true;
+    if (!ws || ws_bytes < need || ((uintptr_t)ws & 255)) return false;
+    p.agg = (float*)ws;
+    p.part = (float*)((char*)ws + (need - (backward && p.parts > 1 ? (size_t)p.B * p.T * p.N * p.G * p.parts * 4 : 0)));
+    return true;
+}
+static bool glr_aligned(const GlrP& p) {
+    const uintptr_t s = p.dtype == GLR_F32 ? 3 : 1, all = (uintptr_t)p.gate | (uintptr_t)p.cand | (uintptr_t)p.out | (uintptr_t)p.dout | (uintptr_t)p.dgate | (uintptr_t)p.dcand;
+    const uintptr_t f = (uintptr_t)p.h0 | (uintptr_t)p.last | (uintptr_t)p.ckpt | (uintptr_t)p.dlast | (uintptr_t)p.dstate;
+    return !(all & s) && !(f & 3);
+}
+int mcrn_glr_forward(const mcrn_glr_t* d, const void* gate, const void* cand, const unsigned char* mask, const float* state,
+                     void* ws, size_t ws_bytes, void* out, float* last, float* ckpt, void* stream) {
+    ENTER();
+    GlrP p;
+    if (!glr_params(d, p)) FAIL("glr_forward: bad sizes, type, activation or strides");
+    if ((long long)p.B * p.N == 0) return 0;
+    if (p.T > 0 && (!gate || !cand)) FAIL("glr_forward: gate and cand are needed");
+    p.gate = gate; p.cand = cand; p.mask = mask; p.h0 = state; p.out = out; p.last = last;
+    p.ckpt = p.dtype == GLR_F32 ? nullptr : ckpt;
+    if (!glr_aligned(p)) FAIL("glr_forward: a pointer is not aligned to its type");
+    if (!glr_plan(p, false)) FAIL("glr_forward: too many sequences");
+    if (!glr_place(p, false, ws, ws_bytes)) FAIL("glr_forward: the workspace is too small or not 256-byte aligned");
+    fam(p.S > 1 ? "glr:fwd_split" : p.CL == 256 ? "glr:fwd_stream" : "glr:fwd_tile");
+    CK(launch_glr_forward(p, (hipStream_t)stream, &g_launches));
+    return 0;
+}
+int mcrn_glr_backward(const mcrn_glr_t* d, const void* gate, const void* cand, const unsigned char* mask, const float* state,
+                      const void* kept, const void* dout, const float* dlast, void* ws, size_t ws_bytes, void* dgate,
+                      void* dcand, float* dstate, void* stream) {
+    ENTER();
+    GlrP p;
+    if (!glr_params(d, p)) FAIL("glr_backward: bad sizes, type, activation or strides");
+    if ((long long)p.B * p.N == 0) return 0;
+    if (p.T > 0 && (!gate || !cand || !dgate || !dcand)) FAIL("glr_backward: gate, cand, dgate and dcand are needed");
+    if (p.T > GLR_K && !kept) FAIL("glr_backward: the forward's out (fp32) or checkpoints (16-bit types) are needed");
+    p.gate = gate; p.cand = cand; p.mask = mask; p.h0 = state;
+    if (p.dtype == GLR_F32) p.out = const_cast<void*>(kept);
+    else p.ckpt = (float*)const_cast<void*>(kept);
+    p.dout = dout; p.dlast = dlast; p.dgate = dgate; p.dcand = dcand; p.dstate = dstate;
+    if (!glr_aligned(p)) FAIL("glr_backward: a pointer is not aligned to its type");
+    if (!glr_plan(p, true)) FAIL("glr_backward: too many sequences");
+    if (!glr_place(p, true, ws, ws_bytes)) FAIL("glr_backward: the workspace is too small or not 256-byte aligned");
+    fam(p.S > 1 ? "glr:bwd_split" : p.CL == 256 ? "glr:bwd_stream" : "glr:bwd_tile");
+    CK(launch_glr_backward(p, (hipStream_t)stream, &g_launches));
+    return 0;
+}
+
+// ---- AdamW over many tensors ------------------------------------------------------------------------
+static bool adamw_ok(const mcrn_adamw_t* a, const long long* numel) {
+    if (!a || !numel || a->ntensors < 1 || a->ntensors > (1 << 20) || (a->dtype != MCRN_T_F32 && a->dtype != MCRN_T_BF16) ||
+        (a->state_bits != 32 && a->state_bits != 8) || a->reserved)
+        return false;
+    long long sum = 0;
+    for (int i = 0; i < a->ntensors; ++i) {
+        if (numel[i] < 0 || numel[i] > (1ll << 40)) return false;
+        sum += (numel[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;
+        if (sum > (1ll << 40)) return false;
+    }
+    return true;
+}
+long long mcrn_adamw_arena_elements(const mcrn_adamw_t* a, const long long* numel) {
+    if (!adamw_ok(a, numel)) return -1;
+    long long sum = 0;
+    for (int i = 0; i < a->ntensors; ++i) sum += (numel[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;
+    return sum;
+}
+// runs of 1024 elements that a block of the norm works on: about 1024 blocks in all, one run at the least
+static int adamw_norm_runs(long long elements) { return (int)std::max<long long>(1, elements / (1024ll * 1024)); }
+static const size_t ADAMW_HEAD = 256;         // ticket, factor, norm
+size_t mcrn_adamw_workspace_bytes(const mcrn_adamw_t* a, const long long* numel) {
+    const long long n = mcrn_adamw_arena_elements(a, numel);
+    if (n < 0) return 0;
+    const long long each = 1024ll * adamw_norm_runs(n), parts = n / each + a->ntensors;
+    return ADAMW_HEAD + (size_t)parts * 8 + (size_t)a->ntensors * sizeof(AdamwDyn);
+}
+int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* const* grads, const long long* numel,
+                    const double* lr, const double* weight_decay, int* step, void* m, void* v, unsigned char* m_scale,
+                    unsigned char* v_scale, float* master, void* ws, size_t ws_bytes, float* total_norm, void* stream) {
+    ENTER();
+    if (!adamw_ok(a, numel)) FAIL("adamw_step: bad number of tensors, sizes, type or state_bits");
+    if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1 && a->eps > 0 && a->grad_scale > 0)) FAIL("adamw_step: betas in [0, 1), eps > 0 and grad_scale > 0 are needed");
+    if (!params || !grads || !lr || !weight_decay || !step || !m || !v || !ws) FAIL("adamw_step: a null pointer");
+    if (a->state_bits == 8 && (!m_scale || !v_scale)) FAIL("adamw_step: 8-bit moments need their scales");
+    if (a->dtype == MCRN_T_BF16 && !master) FAIL("adamw_step: bf16 parameters need fp32 masters");
+    if (((uintptr_t)m | (uintptr_t)v | (uintptr_t)master | (uintptr_t)ws) & 15) FAIL("adamw_step: arenas and workspace must be 16-byte aligned");
+    const size_t need = mcrn_adamw_workspace_bytes(a, numel);
+    if (ws_bytes < need) FAIL("adamw_step: the workspace needs %zu bytes", need);
+    const uintptr_t size = a->dtype == MCRN_T_F32 ? 4 : 2;
+    long long elements = 0, live = 0;
+    for (int i = 0; i < a->ntensors; ++i) {
+        elements += (numel[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;
+        if (!grads[i] || !numel[i]) continue;
+        live += numel[i];
+        if (!params[i] || ((uintptr_t)params[i] | (uintptr_t)grads[i]) % size) FAIL("adamw_step: tensor %d has no parameter, or one that is not aligned to its type", i);
+        if (!a->on_device && step[i] < 1) FAIL("adamw_step: step of tensor %d is %d, the first is 1", i, step[i]);
+    }
+    if (!live) return 0;
+    const hipStream_t st = (hipStream_t)stream;
+    unsigned* ticket = (unsigned*)ws;
+    float* factor = (float*)ws + 1;
+    float* norm = total_norm ? total_norm : (float*)ws + 2;
+    double* part = (double*)((char*)ws + ADAMW_HEAD);
+    const int runs_n = adamw_norm_runs(elements);
+    AdamwDyn* dyn = (AdamwDyn*)((char*)part + (elements / (1024ll * runs_n) + a->ntensors) * 8);
+    const bool clip = a->max_norm > 0 || total_norm;
+    // small steps spread over many blocks, large ones keep a block long enough to hide its start
+    const int runs = live < (4ll << 20) ? 1 : 4;
+
+    if (a->on_device) {
+        for (int base = 0; base < a->ntensors; base += 4096) {
+            AdamwPrepP q;
+            memset(&q, 0, sizeof q);
+            q.lr = lr; q.wd = weight_decay; q.step = step; q.dyn = dyn; q.base = base; q.seed = a->seed; q.b1 = a->beta1; q.b2 = a->beta2;
+            q.nt = std::min(4096, a->ntensors - base);
+            for (int i = 0; i < q.nt; ++i)
+                if (grads[base + i] && numel[base + i]) q.has[i >> 6] |= 1ull << (i & 63);
+            CK(launch_adamw_prep(q, st));
+            ++g_launches;
+        }
+    }
+    // tensors [i, next) of a launch with `per` runs a block; returns its blocks
+    auto fill = [&](int& i, long long& off, AdamwT* t, int& nt, int per) {
+        unsigned blocks = 0;
+        nt = 0;
+        for (; i < a->ntensors && nt < ADAMW_TENSORS; ++i) {
+            const long long n = numel[i], room = (n + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;
+            if (grads[i] && n) {
+                const long long nb = (n + 1024ll * per - 1) / (1024ll * per);
+                if (nb + blocks >= (1ll << 31)) break;
+                AdamwT& e = t[nt++];
+                e.p = params[i]; e.g = grads[i]; e.n = n; e.off = off; e.blk0 = blocks; e.id = i; e.pad = 0;
+                e.flags = (((uintptr_t)params[i] | (uintptr_t)grads[i]) % (4 * size)) == 0 ? ADAMW_VEC : 0;
+                e.key = 0; e.step_size = e.inv_bc2 = e.decay = 0.f;
+                if (!a->on_device) {
+                    const double s = step[i];
+                    e.step_size = (float)(lr[i] / (1.0 - pow(a->beta1, s)));
+                    e.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(a->beta2, s)));
+                    e.decay = (float)(1.0 - lr[i] * weight_decay[i]);
+                    e.key = adamw_key(a->seed, i, (unsigned)step[i]);
+                }
+                blocks += (unsigned)nb;
+            }
+            off += room;
+        }
+        return blocks;
+    };
+    if (clip) {
+        AdamwNormP q;
+        unsigned all = 0;
+        for (int i = 0; i < a->ntensors; ++i)
+            if (grads[i]) all += (unsigned)((numel[i] + 1024ll * runs_n - 1) / (1024ll * runs_n));
+        long long off = 0;
+        unsigned blk0 = 0;
+        for (int i = 0; i < a->ntensors;) {
+            const unsigned blocks = fill(i, off, q.t, q.nt, runs_n);
+            if (!blocks) continue;
+            q.per = runs_n; q.blk0 = blk0; q.blocks = all; q.part = part; q.ticket = ticket; q.norm = norm; q.factor = factor;
+            q.max_norm = (float)a->max_norm; q.grad_scale = (float)a->grad_scale;
+            CK(launch_adamw_norm(q, blocks, a->dtype, st));
+            ++g_launches;
+            blk0 += blocks;
+        }
+    }
+    AdamwP q;
+    long long off = 0;
+    for (int i = 0; i < a->ntensors;) {
+        const unsigned blocks = fill(i, off, q.t, q.nt, runs);
+        if (!blocks) continue;
+        q.per = runs; q.m = m; q.v = v; q.ms = m_scale; q.vs = v_scale; q.master = master;
+        q.factor = clip ? factor : nullptr; q.dyn = a->on_device ? dyn : nullptr; q.grad_scale = (float)a->grad_scale;
+        q.b1 = (float)a->beta1; q.c1 = (float)(1.0 - a->beta1); q.b2 = (float)a->beta2; q.c2 = (float)(1.0 - a->beta2); q.eps = (float)a->eps;
+        fam(a->state_bits == 8 ? "adamw:8bit" : "adamw:32bit");
+        CK(launch_adamw(q, blocks, a->dtype, a->state_bits, st));
+        ++g_launches;
+    }
+    return 0;
+}
+int mcrn_adamw_unpack(const unsigned char* codes, const unsigned char* scale, long long n, int second, float* out, void* stream) {
+    ENTER();
+    if (n < 0 || n % ADAMW_BLOCK || n > (1ll << 40) || (n && (!codes || !scale || !out)) || ((uintptr_t)codes & 3) || ((uintptr_t)out & 15)) FAIL("adamw_unpack: bad arguments");
+    if (!n) return 0;
+    CK(launch_adamw_unpack(codes, scale, out, n, second != 0, (hipStream_t)stream));
+    ++g_launches;
     return 0;
 }
 

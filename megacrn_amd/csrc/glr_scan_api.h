@@ -1,0 +1,46 @@
+// glr_scan_api.h - parameter block and host entry points of the gated linear recurrence (glr_scan.h, compiled in
+// glr_scan_unit.hip).  engine.hip includes only this file.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stddef.h>
+
+namespace mcrn {
+
+enum { GLR_F32 = 0, GLR_BF16 = 1, GLR_F16 = 2 };
+
+// h_t = a_t h_{t-1} + (1 - a_t) phi(cand_t), a_t = sigmoid(gate_t); a step whose mask byte is 0 keeps the state.
+// gate (B,T,N,G), cand (B,T,N,H), D = H / G channels share a gate; strides in elements, the last dimension is contiguous.
+struct GlrP {
+    int B, T, N, H, G, dtype, act;          // act: 0 phi(c) = c, 1 phi = tanh
+    const void *gate, *cand;
+    long long g_sb, g_st, g_sn, c_sb, c_st, c_sn;
+    const uint8_t* mask;                    // nullable
+    long long m_sb, m_st, m_sn;
+    const float* h0;                        // (B,N,H) or NULL = zeros
+    void* out;                              // (B,T,N,H) contiguous, NULL = not wanted (forward only)
+    float* last;                            // (B,N,H), may be h0 itself (forward only)
+    float* ckpt;                            // (B, ceil(T/GLR_K) - 1, N, H) states before steps GLR_K, 2 GLR_K, ..; NULL = not wanted.
+                                            // f32: never written, the backward reads the same states from `out`
+    // backward
+    const void* dout;                       // (B,T,N,H) or NULL = zeros
+    long long d_sb, d_st, d_sn;
+    const float* dlast;                     // (B,N,H) or NULL = zeros
+    void *dgate, *dcand;                    // (B,T,N,G), (B,T,N,H) contiguous
+    float* dstate;                          // (B,N,H) or NULL = not wanted
+    // plan (glr_plan)
+    int one;                                // not 0: plan for one channel a thread, whatever the alignment
+    int V, CL, S, L, parts;                 // channels a thread, channel lanes a block, chunks of the time axis,
+    int chunk, first;                       // lanes and parts of a shared gate's channels; steps a chunk, first chunk of the launch
+    long long nq, tiles;                    // channel vectors of a batch entry, blocks that cover them
+    float *agg, *part;                      // workspace: chunk aggregates, partial gate gradients
+};
+
+constexpr int GLR_K = 8;                    // steps a thread holds in registers = distance of the checkpoints
+
+bool glr_plan(GlrP& p, bool backward);      // fills the plan; false: too large
+size_t glr_ws_bytes(const GlrP& p, bool backward);
+hipError_t launch_glr_forward(const GlrP& p, hipStream_t st, int* launches);
+hipError_t launch_glr_backward(const GlrP& p, hipStream_t st, int* launches);
+
+}  // namespace mcrn

@@ -1,0 +1,109 @@
+// glr_scan_unit.hip - gated linear recurrence (glr_scan.h): plan and launches
+#include "glr_scan.h"
+
+namespace mcrn {
+
+static long long up_div(long long a, long long b) { return (a + b - 1) / b; }
+
+bool glr_plan(GlrP& p, bool backward) {
+    const size_t size = p.dtype == GLR_F32 ? 4 : 2;
+    const int D = p.H / p.G;
+    const bool shared = D > 1;
+    // Four channels a thread (16 bytes of f32, 8 of the 16-bit types) where rows and pointers allow it, else one.
+    auto fits = [&](const void* q, long long a, long long b, long long c) {
+        return !q || (((uintptr_t)q % (4 * size)) == 0 && a % 4 == 0 && b % 4 == 0 && c % 4 == 0);
+    };
+    auto fits32 = [](const void* q) { return ((uintptr_t)q & 15) == 0; };
+    p.V = D % 4 == 0 || !shared ? 4 : 1;
+    if (p.H % 4 || !fits(p.cand, p.c_sb, p.c_st, p.c_sn) || !fits(p.out, 0, 0, 0) || (!shared && !fits(p.gate, p.g_sb, p.g_st, p.g_sn)) ||
+        !fits32(p.ckpt) || !fits32(p.h0))
+        p.V = 1;
+    if (p.one) p.V = 1;
+    if (backward && (!fits(p.dout, p.d_sb, p.d_st, p.d_sn) || !fits(p.dcand, 0, 0, 0) || (!shared && !fits(p.dgate, 0, 0, 0)))) p.V = 1;
+    p.nq = (long long)p.N * (p.H / p.V);
+    auto cover = [&](int CL) {
+        p.CL = CL;
+        if (shared) {
+            const int lanes = (D + p.V - 1) / p.V, most = CL < 64 ? CL : 64;
+            p.L = 1;
+            while (p.L < lanes && p.L < most) p.L *= 2;
+            p.parts = (lanes + p.L - 1) / p.L;
+            p.tiles = up_div((long long)p.N * p.G * p.parts, CL / p.L);
+        } else {
+            p.L = p.parts = 1;
+            p.tiles = up_div(p.nq, CL);
+        }
+        return p.tiles * p.B;
+    };
+    p.S = 1;
+    p.first = 0;
+    p.chunk = p.T > 0 ? p.T : 1;
+    long long blocks = cover(256);
+    if (p.T > GLR_K && blocks < 512) blocks = cover(64);
+    if (p.T > 4 * GLR_K && blocks < 512) {
+        blocks = cover(16);
+        const int span = GLR_THREADS / 16 * GLR_K;
+        long long S = blocks < 256 ? up_div(512, blocks) : 1;
+        S = S > 64 ? 64 : S;
+        const long long most = up_div(p.T, span);
+        S = S > most ? most : S;
+        if (S > 1) {
+            p.chunk = (int)(up_div(up_div(p.T, S), span) * span);
+            p.S = (int)up_div(p.T, p.chunk);
+        }
+    }
+    return p.tiles * p.B * p.S < (1ll << 31);
+}
+
+size_t glr_ws_bytes(const GlrP& p, bool backward) {
+    const size_t agg = p.S > 1 ? (size_t)p.S * p.B * 2 * p.N * p.H * 4 : 0;
+    const size_t part = backward && p.parts > 1 ? (size_t)p.B * p.T * p.N * p.G * p.parts * 4 : 0;
+    return (agg + 255) / 256 * 256 + part;
+}
+
+template <class X, int V, int CL, bool SHARED> static hipError_t run(const GlrP& p0, bool backward, hipStream_t st, int* launches) {
+    GlrP p = p0;
+    const unsigned one = (unsigned)(p.tiles * p.B);
+    (void)hipGetLastError();
+    if (CL == 16 && p.S > 1) {                            // maps of the chunks that others start from
+        if (backward) {
+            p.first = 1;
+            hipLaunchKernelGGL((glr_bwd_kernel<X, V, 16, SHARED, true>), dim3(one * (p.S - 1)), dim3(GLR_THREADS), 0, st, p);
+            p.first = 0;
+        } else {
+            hipLaunchKernelGGL((glr_fwd_kernel<X, V, 16, SHARED, true>), dim3(one * (p.S - 1)), dim3(GLR_THREADS), 0, st, p);
+        }
+        ++*launches;
+    }
+    if (backward) {
+        hipLaunchKernelGGL((glr_bwd_kernel<X, V, CL, SHARED, false>), dim3(one * p.S), dim3(GLR_THREADS), 0, st, p);
+        if (p.parts > 1) {
+            const long long n = (long long)p.B * p.T * p.N * p.G;
+            hipLaunchKernelGGL((glr_parts_kernel<X>), dim3((unsigned)up_div(n, 256)), dim3(256), 0, st, p.part, p.parts, n, p.dgate);
+            ++*launches;
+        }
+    } else {
+        hipLaunchKernelGGL((glr_fwd_kernel<X, V, CL, SHARED, false>), dim3(one * p.S), dim3(GLR_THREADS), 0, st, p);
+    }
+    ++*launches;
+    return hipGetLastError();
+}
+
+template <class X, int V> static hipError_t run_v(const GlrP& p, bool backward, hipStream_t st, int* launches) {
+    const bool shared = p.G != p.H;
+    if (p.CL == 256) return shared ? run<X, V, 256, true>(p, backward, st, launches) : run<X, V, 256, false>(p, backward, st, launches);
+    if (p.CL == 64) return shared ? run<X, V, 64, true>(p, backward, st, launches) : run<X, V, 64, false>(p, backward, st, launches);
+    return shared ? run<X, V, 16, true>(p, backward, st, launches) : run<X, V, 16, false>(p, backward, st, launches);
+}
+template <class X> static hipError_t run_x(const GlrP& p, bool backward, hipStream_t st, int* launches) {
+    return p.V == 4 ? run_v<X, 4>(p, backward, st, launches) : run_v<X, 1>(p, backward, st, launches);
+}
+static hipError_t launch(const GlrP& p, bool backward, hipStream_t st, int* launches) {
+    if (p.dtype == GLR_F32) return run_x<GlrF32>(p, backward, st, launches);
+    if (p.dtype == GLR_BF16) return run_x<GlrBf16>(p, backward, st, launches);
+    return run_x<GlrF16>(p, backward, st, launches);
+}
+hipError_t launch_glr_forward(const GlrP& p, hipStream_t st, int* launches) { return launch(p, false, st, launches); }
+hipError_t launch_glr_backward(const GlrP& p, hipStream_t st, int* launches) { return launch(p, true, st, launches); }
+
+}  // namespace mcrn

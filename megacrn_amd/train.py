@@ -118,6 +118,9 @@ def build_parser():
     p.add_argument('--gpu', type=int, default=0)
     p.add_argument('--seed', type=int, default=None, help='the reference leaves seeding commented out (:264-266)')
     p.add_argument('--save_dir', type=str, default='../save')
+    p.add_argument('--optimizer', choices=['adam', 'adamw'], default='adam', help='adam: the reference (:104); adamw: decoupled weight decay')
+    p.add_argument('--weight_decay', type=float, default=0.01, help='of adamw')
+    p.add_argument('--state_bits', type=int, choices=[32, 8], default=32, help='bits of the moments that adamw holds')
     p.add_argument('--max_batches', type=int, default=0, help='>0: stop each epoch after this many batches (smoke runs)')
     return p
 
@@ -331,7 +334,8 @@ def main(argv=None):
 
     model = get_model()
     tr = FlatTrainer(model, lr=args.lr, eps=args.epsilon, max_grad_norm=args.max_grad_norm, lamb=args.lamb,
-                     lamb1=args.lamb1, scaler_mean=float(scaler.mean), scaler_std=float(scaler.std))
+                     lamb1=args.lamb1, scaler_mean=float(scaler.mean), scaler_std=float(scaler.std), optimizer=args.optimizer,
+                     weight_decay=args.weight_decay, state_bits=args.state_bits)
     metrics = DeviceMetrics(args, scaler, device)
     # one run directory for the whole job: rank 0 names it, everybody else is told
     stamp = [time.strftime("%Y%m%d%H%M%S")]

@@ -2,7 +2,8 @@
 
 One step = forward (C ABI) -> 3-term loss (:118-125, one fused HIP kernel group) -> backward (C ABI, gradients written
 straight into one flat fp32 bucket) -> ONE all-reduce(sum) of that bucket over RCCL when world_size > 1 ->
-clip_grad_norm_(5) + Adam(lr, eps=1e-3) as a single flat HIP kernel pair.  Parameters stay ordinary
+clip_grad_norm_(5) + Adam(lr, eps=1e-3) as a single flat HIP kernel pair (``optimizer="adamw"``: clip + AdamW with moments
+of 32 or 8 bits, ``optim.py``).  Parameters stay ordinary
 ``nn.Parameter``s of the reference shapes (views into the flat buffer), so ``state_dict`` round-trips.
 
 ``num_layers == 1`` (the reference default, ``--num_rnn_layers 1``) runs the fused model entry points.
@@ -17,12 +18,18 @@ import ctypes as C
 import torch
 
 from ._lib import lib, check, Dims, Params, Grads
+from .optim import AdamW
 from . import dp
 
 
 class FlatTrainer:
     def __init__(self, model, *, lr=0.01, eps=1e-3, betas=(0.9, 0.999), max_grad_norm=5.0, lamb=0.01,
-                 lamb1=0.01, scaler_mean=0.0, scaler_std=1.0, process_group=None, autotune=True):
+                 lamb1=0.01, scaler_mean=0.0, scaler_std=1.0, process_group=None, autotune=True, optimizer="adam",
+                 weight_decay=0.01, state_bits=32):
+        if optimizer not in ("adam", "adamw"):
+            raise ValueError(f"FlatTrainer: optimizer must be 'adam' or 'adamw'; got {optimizer!r}")
+        if optimizer == "adam" and state_bits != 32:
+            raise ValueError("FlatTrainer: 8-bit moments come with optimizer='adamw'")
         self.model = model
         self.fused = model.num_layers == 1
         self.lr, self.eps, self.betas, self.max_grad_norm = lr, eps, betas, float(max_grad_norm)
@@ -38,10 +45,16 @@ class FlatTrainer:
         self.bucket = dp.FlatBucket(params, process_group)     # flat parameter / gradient buffers + the collective
         self.n, self.flat_p, self.flat_g = self.bucket.n, self.bucket.flat_p, self.bucket.flat_g
         self._gviews = self.bucket.grad_views
-        self.m = torch.zeros(self.n, device=dev)
-        self.v = torch.zeros(self.n, device=dev)
-        self.scratch = torch.zeros(2048, device=dev)
-        self.total_norm = torch.zeros(1, device=dev)
+        self.opt = None
+        if optimizer == "adamw":               # decoupled decay, moments of 32 or 8 bits (optim.py), on the same gradient views
+            self.opt = AdamW(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=self.max_grad_norm,
+                             state_bits=state_bits)
+            self.total_norm = self.opt.total_norm
+        else:
+            self.m = torch.zeros(self.n, device=dev)
+            self.v = torch.zeros(self.n, device=dev)
+            self.scratch = torch.zeros(2048, device=dev)
+            self.total_norm = torch.zeros(1, device=dev)
         self.loss_scratch = torch.zeros(4104, device=dev)
         self.losses = torch.zeros(4, device=dev)
         self.params = params
@@ -146,10 +159,15 @@ class FlatTrainer:
                     p.grad = g
         self.bucket.allreduce()                              # the single collective of the step (no-op at world 1)
         self.step_count += 1
-        check(lib.mcrn_flat_clip_adam(self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.m.data_ptr(),
-                                      self.v.data_ptr(), self.n, self.lr, self.betas[0], self.betas[1], self.eps,
-                                      self.step_count, self.max_grad_norm, self.bucket.grad_scale,
-                                      self.scratch.data_ptr(), self.total_norm.data_ptr(), st), "mcrn_flat_clip_adam")
+        if self.opt is not None:
+            for g in self.opt.param_groups:
+                g["lr"] = self.lr
+            self.opt.step(grads=self._gviews, grad_scale=self.bucket.grad_scale)
+        else:
+            check(lib.mcrn_flat_clip_adam(self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.m.data_ptr(),
+                                          self.v.data_ptr(), self.n, self.lr, self.betas[0], self.betas[1], self.eps,
+                                          self.step_count, self.max_grad_norm, self.bucket.grad_scale,
+                                          self.scratch.data_ptr(), self.total_norm.data_ptr(), st), "mcrn_flat_clip_adam")
         self.batches_seen += 1
         # a fresh tensor for the caller (self.losses is rewritten by the next step) made by an element-wise kernel:
         # .clone() of a device scalar is a hipMemcpyAsync, ~100 us of queue idle per step on this runtime

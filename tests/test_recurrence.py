@@ -1,0 +1,411 @@
+"""Gated linear recurrence: the HIP kernels against the float64 oracle, element by element within running error bounds
+(oracle/sequence_oracle.py), and what the entry points refuse."""
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import megacrn_oracle as MO
+from oracle import sequence_oracle as O
+
+TORCH = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# without a GPU
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("act", ["tanh", "none"])
+@pytest.mark.parametrize("G", [6, 2, 1])
+def test_oracle_gradient_matches_differences(act, G):
+    """The oracle's gradients against central differences in float64: truncation h^2 and cancellation 1e-16 / h at h = 1e-5 leave
+    1e-9 of values around 1."""
+    rng = np.random.default_rng(0)
+    B, T, N, H = 2, 5, 3, 6
+    gate, cand, state = rng.normal(1, 1, (B, T, N, G)), rng.normal(0, 1, (B, T, N, H)), rng.normal(0, 1, (B, N, H))
+    mask = rng.random((B, T, N)) > 0.3
+    mask[0, :, 1] = False
+    dout, dlast = rng.normal(0, 1, (B, T, N, H)), rng.normal(0, 1, (B, N, H))
+
+    def loss(*a):
+        out, last, _, _ = O.glr_fwd(*a, mask=mask, act=act)
+        return (out * dout).sum() + (last * dlast).sum()
+
+    got = O.glr_bwd(O.glr_fwd(gate, cand, state, mask, act)[3], dout, dlast)[:3]
+    for k, x in enumerate((gate, cand, state)):
+        for _ in range(6):
+            d = rng.normal(0, 1, x.shape)
+            args = [gate, cand, state]
+            args[k] = x + 1e-5 * d
+            hi = loss(*args)
+            args[k] = x - 1e-5 * d
+            assert abs((hi - loss(*args)) / 2e-5 - (got[k] * d).sum()) < 1e-7
+    assert not got[0][0, :, 1].any() and not got[1][0, :, 1].any()
+
+
+def _cpu(**over):
+    a = {"gate": torch.zeros(2, 3, 4, 8), "cand": torch.zeros(2, 3, 4, 8), "state": torch.zeros(2, 4, 8), "mask": torch.ones(2, 3, 4, dtype=torch.bool)}
+    a.update(over)
+    return a
+
+
+@pytest.mark.parametrize("over,kind", [
+    (dict(gate=torch.zeros(2, 3, 4, 3)), ValueError),                      # 3 gates for 8 channels
+    (dict(gate=torch.zeros(2, 3, 4, 0)), ValueError),
+    (dict(gate=torch.zeros(2, 2, 4, 8)), ValueError),
+    (dict(gate=torch.zeros(2, 3, 32)), ValueError),
+    (dict(gate=torch.zeros(2, 3, 4, 8, dtype=torch.bfloat16)), ValueError),
+    (dict(gate=torch.zeros(2, 3, 4, 8, dtype=torch.float64), cand=torch.zeros(2, 3, 4, 8, dtype=torch.float64)), TypeError),
+    (dict(gate=torch.zeros(2, 3, 4, 8, dtype=torch.int32)), TypeError),
+    (dict(cand=[1.0]), TypeError),
+    (dict(state=torch.zeros(2, 4, 8, dtype=torch.bfloat16)), ValueError),
+    (dict(state=torch.zeros(1, 4, 8)), ValueError),
+    (dict(mask=torch.ones(2, 3, 4)), ValueError),                          # not bool
+    (dict(mask=torch.ones(2, 4, 4, dtype=torch.bool)), ValueError),
+    (dict(mask=torch.ones(3, dtype=torch.bool)), ValueError),
+    (dict(activation="relu"), ValueError),
+    (dict(), RuntimeError),                                                # all in order, but on the CPU
+])
+def test_refusals(over, kind):
+    import megacrn_amd
+    with pytest.raises(kind):
+        megacrn_amd.gated_linear_recurrence(**_cpu(**over))
+
+
+@pytest.mark.parametrize("over,kind", [
+    (dict(state=None), ValueError), (dict(state=torch.zeros(8, 4, 2).permute(2, 1, 0)), ValueError), (dict(), RuntimeError)])
+def test_step_refusals(over, kind):
+    import megacrn_amd
+    a = _cpu(gate=torch.zeros(2, 4, 8), cand=torch.zeros(2, 4, 8), mask=None)
+    a.update(over)
+    with pytest.raises(kind):
+        megacrn_amd.gated_linear_recurrence_step(**a)
+
+
+def test_c_sizes():
+    """Checkpoints: one state in fp32 before every 8th step but the first, 16-bit types only; a workspace for long sequences with few channels."""
+    import ctypes as C
+    from megacrn_amd._lib import lib, Glr
+
+    def d(B, T, N, H, G, dtype):
+        return C.byref(Glr(B, T, N, H, G, dtype, 1, 0))
+    assert lib.mcrn_glr_checkpoint_floats(d(2, 8, 3, 4, 4, 1)) == 0
+    assert lib.mcrn_glr_checkpoint_floats(d(2, 9, 3, 4, 4, 1)) == 24
+    assert lib.mcrn_glr_checkpoint_floats(d(2, 17, 3, 4, 4, 2)) == 48
+    assert lib.mcrn_glr_checkpoint_floats(d(2, 17, 3, 4, 4, 0)) == 0
+    assert lib.mcrn_glr_checkpoint_floats(d(2, 0, 3, 4, 4, 1)) == 0
+    assert lib.mcrn_glr_workspace_bytes(d(1, 1, 207, 64, 64, 0), 1) == 0
+    assert lib.mcrn_glr_workspace_bytes(d(1, 20000, 1, 33, 33, 0), 0) > 0
+    for bad in (d(-1, 8, 3, 4, 4, 1), d(2, 8, 3, 4, 3, 1), d(2, 8, 3, 4, 4, 3), d(2, 8, 3, 0, 1, 0)):
+        assert lib.mcrn_glr_workspace_bytes(bad, 0) == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# on the GPU
+# ---------------------------------------------------------------------------------------------------------------------
+def _inputs(B, T, N, H, G, dt, mask, seed, state=True):
+    g = torch.Generator().manual_seed(seed)
+    gate = (torch.randn(B, T, N, G, generator=g) * 1.5 + 1.5).to(TORCH[dt])
+    cand = torch.randn(B, T, N, H, generator=g).to(TORCH[dt])
+    st = torch.randn(B, N, H, generator=g) if state else None
+    keep = None
+    if mask:
+        keep = torch.rand(B, T, N, generator=g) > 0.25
+        keep[:, :, N // 2] = False                       # a row that nothing is left of
+        for bad in (float("nan"), float("inf"), torch.finfo(TORCH[dt]).min):
+            hit = (torch.rand(B, T, N, generator=g) < 0.3) & ~keep
+            gate[hit], cand[hit] = bad, -bad
+    return gate, cand, st, keep, torch.randn(B, T, N, H, generator=g).to(TORCH[dt]), torch.randn(B, N, H, generator=g)
+
+
+def _np(t):
+    return None if t is None else t.double().numpy()
+
+
+def _close(got, want, bound, what):
+    got = got.detach().cpu().double().numpy()
+    assert got.shape == want.shape, what
+    over = np.abs(got - want) - bound
+    assert not (over > 0).any() and np.isfinite(got).all(), f"{what}: {(over > 0).sum()} of {over.size} beyond the bound, worst {over.max():.3g}"
+
+
+def _against_oracle(gate, cand, st, keep, dout, dlast, act, dt, lay=lambda t: t.cuda(), want_grad=True):
+    import megacrn_amd
+    m = None if keep is None else keep.numpy()
+    out, last, eh, cache = O.glr_fwd(_np(gate), _np(cand), _np(st), m, act)
+    leaves = [lay(t).detach().requires_grad_() if t is not None else None for t in (gate, cand, st)]
+    got, glast = megacrn_amd.gated_linear_recurrence(leaves[0], leaves[1], leaves[2], None if keep is None else keep.cuda(), activation=act)
+    _close(got, out, eh + O.half_step(out, dt), "out")
+    e_last = eh[:, -1] if cand.shape[1] else 0 * last
+    _close(glast, last, e_last + O.half_step(last, "f32"), "last")
+    if not want_grad:
+        return
+    have = [t for t in leaves if t is not None]
+    grads = torch.autograd.grad((got, glast), have, (lay(dout), dlast.cuda()))
+    dg, dc, ds, eg, ec, es = O.glr_bwd(cache, _np(dout), _np(dlast))
+    _close(grads[0], dg, eg + O.half_step(dg, dt), "dgate")
+    _close(grads[1], dc, ec + O.half_step(dc, dt), "dcand")
+    if st is not None:
+        _close(grads[2], ds, es + O.half_step(ds, "f32"), "dstate")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["tanh", "none"])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,N,H,G", [
+    (1, 1, 1, 1, 1), (2, 1, 3, 8, 8), (1, 2, 5, 4, 1), (3, 7, 2, 12, 12), (1, 8, 3, 33, 33), (2, 9, 3, 64, 64), (1, 16, 29, 16, 4),
+    (2, 17, 7, 20, 5), (1, 40, 3, 48, 1), (1, 127, 5, 64, 64), (1, 128, 2, 64, 16), (2, 129, 3, 32, 32), (1, 300, 1, 7, 7),
+    (1, 257, 2, 300, 1), (1, 70, 1, 70, 1), (1, 33, 2, 70, 7), (1, 20, 1, 1100, 1),
+])
+def test_against_oracle(B, T, N, H, G, dt, act):
+    _against_oracle(*_inputs(B, T, N, H, G, dt, True, B * 1000 + T * 10 + H), act, dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,N,H,G,dt,family", [
+    (1, 2100, 1, 33, 33, "f32", "split"), (2, 2051, 3, 16, 4, "bf16", "split"), (1, 4100, 2, 8, 1, "f16", "split"), (1, 1025, 1, 260, 1, "f32", "split"),
+    (32, 20, 64, 63, 63, "f32", "stream"), (33, 20, 64, 65, 5, "bf16", "stream"), (64, 1, 17, 64, 64, "f16", "stream"),
+    (8, 12, 100, 64, 64, "f32", "tile"), (1, 500, 30, 64, 64, "f32", "split"), (8, 150, 100, 64, 1, "bf16", "tile"), (16, 200, 64, 64, 64, "f32", "tile"),
+])
+def test_every_variant(B, T, N, H, G, dt, family):
+    """The plans' variants by name: one thread walks all steps, segments of a block, chunks of several blocks."""
+    from megacrn_amd import _lib
+    _lib.launch_histogram(reset=True)
+    _against_oracle(*_inputs(B, T, N, H, G, dt, T % 2 == 1, T + H, state=T % 3 != 0), "tanh", dt)
+    seen = {k for k, v in _lib.launch_histogram().items() if k.startswith("glr:") and v}
+    assert seen == {f"glr:fwd_{family}", f"glr:bwd_{family}"}, seen
+
+
+@pytest.mark.gpu
+def test_long_memory():
+    """Gates that hardly forget (1 - a down to e^-12) over 3000 steps: 1 - a has to keep its own relative precision."""
+    gate, cand, st, keep, dout, dlast = _inputs(1, 3000, 2, 12, 12, "f32", False, 5)
+    gate = gate * 2 + 6
+    _against_oracle(gate, cand, st, None, dout, dlast, "tanh", "f32")
+
+
+@pytest.mark.gpu
+def test_extreme_gates_and_small_candidates():
+    """Gates of +-100 and +-inf hold or replace the state exactly; tanh of 1e-6 .. 1e-2 keeps its relative precision."""
+    import megacrn_amd
+    gate = torch.tensor([100.0, -100.0, float("inf"), float("-inf"), 80.0, -80.0, 0.0, -0.0]).view(1, 1, 1, 8).expand(1, 40, 1, 8).contiguous()
+    cand = torch.full((1, 40, 1, 8), 0.5)
+    st = torch.arange(1.0, 9.0).view(1, 1, 8)
+    out, last = megacrn_amd.gated_linear_recurrence(gate.cuda(), cand.cuda(), st.cuda(), activation="none")
+    want = torch.tensor([1.0, 0.5, 3.0, 0.5, 5.0, 0.5])
+    assert torch.equal(out[0, 0, 0, :6].cpu(), want) and torch.equal(last[0, 0, :6].cpu(), want)
+    small = torch.logspace(-6, -0.2, 64).view(1, 1, 1, 64)
+    out, _ = megacrn_amd.gated_linear_recurrence(torch.full_like(small, -100.0).cuda(), torch.cat([small, -small], 1).cuda()[:, :1])
+    rel = (out.cpu().double() / torch.tanh(small.double()) - 1).abs().max().item()
+    assert rel <= (O.KC + 2) * O.U, rel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_strided_inputs(dt):
+    """Gate and candidate as halves of one product, transposed batches, rows of odd stride, masks shared over nodes or time."""
+    import megacrn_amd
+    torch.manual_seed(0)
+    B, T, N, H = 3, 21, 5, 16
+    both = torch.randn(B, T, N, 2 * H).to(TORCH[dt])
+    gate, cand, st, _, dout, dlast = _inputs(B, T, N, H, H, dt, False, 3)
+    views = [lambda t: torch.cat([t, t], -1).cuda()[..., t.shape[-1]:] if t.dim() == 4 else t.cuda(),
+             lambda t: t.transpose(0, 1).contiguous().cuda().transpose(0, 1),
+             lambda t: torch.nn.functional.pad(t, (0, 3)).cuda()[..., :-3] if t.dim() == 4 else t.cuda(),
+             lambda t: torch.nn.functional.pad(t, (1, 0)).cuda()[..., 1:] if t.dim() == 4 else t.cuda(),
+             lambda t: t.transpose(2, 3).contiguous().cuda().transpose(2, 3) if t.dim() == 4 else t.cuda()]
+    for lay in views:
+        _against_oracle(gate, cand, st, None, dout, dlast, "tanh", dt, lay)
+    halves = both.cuda().chunk(2, -1)
+    a, _ = megacrn_amd.gated_linear_recurrence(*halves, st.cuda())
+    b, _ = megacrn_amd.gated_linear_recurrence(*[t.contiguous() for t in halves], st.cuda())
+    assert torch.equal(a, b)
+    rows = torch.rand(B, T) > 0.3
+    for mask in (rows, rows.unsqueeze(-1), rows[:1].unsqueeze(-1), rows[:, :1, None]):
+        full = (mask if mask.dim() == 3 else mask.unsqueeze(-1)).expand(B, T, N)
+        a, _ = megacrn_amd.gated_linear_recurrence(*halves, st.cuda(), mask.cuda())
+        b, _ = megacrn_amd.gated_linear_recurrence(*halves, st.cuda(), full.contiguous().cuda())
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_gradient_of_expanded_and_partial_outputs():
+    """dout that is expanded (a sum), missing (only `last` used) or reaches one step only; a gate broadcast by its user."""
+    import megacrn_amd
+    gate, cand, st, _, _, _ = _inputs(2, 30, 3, 8, 8, "f32", False, 9)
+    out, last, eh, cache = O.glr_fwd(_np(gate), _np(cand), _np(st))
+    one = np.zeros_like(out)
+    one[:, 11] = 1.0
+    for pick, dout, dlast in ((lambda o, l: o.sum(), np.ones_like(out), None), (lambda o, l: l.sum(), None, np.ones_like(last)),
+                              (lambda o, l: o[:, 11].sum(), one, None)):
+        leaves = [t.cuda().requires_grad_() for t in (gate, cand, st)]
+        grads = torch.autograd.grad(pick(*megacrn_amd.gated_linear_recurrence(*leaves)), leaves)
+        dg, dc, ds, eg, ec, es = O.glr_bwd(cache, dout, dlast)
+        _close(grads[0], dg, eg + O.half_step(dg, "f32"), "dgate")
+        _close(grads[1], dc, ec + O.half_step(dc, "f32"), "dcand")
+        _close(grads[2], ds, es + O.half_step(ds, "f32"), "dstate")
+    row = gate[:1, :1].cuda().requires_grad_()                             # one gate row for all batch entries and steps
+    o, _ = megacrn_amd.gated_linear_recurrence(row.expand(2, 30, 3, 8), cand.cuda())
+    (g,) = torch.autograd.grad(o.sum(), row)
+    _, _, _, cache = O.glr_fwd(np.broadcast_to(_np(gate[:1, :1]), gate.shape).copy(), _np(cand))
+    dg, _, _, eg, _, _ = O.glr_bwd(cache, np.ones_like(out), None)
+    _close(g, dg.sum((0, 1), keepdims=True), (eg + O.half_step(dg, "f32")).sum((0, 1), keepdims=True) + 60 * O.U * np.abs(dg).sum((0, 1), keepdims=True), "shared row")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 0, 3, 8), (0, 5, 3, 8), (2, 5, 0, 8)])
+def test_empty(shape):
+    import megacrn_amd
+    B, T, N, H = shape
+    st = torch.randn(B, N, H, device="cuda", requires_grad=True)
+    x = torch.zeros(shape, device="cuda", requires_grad=True)
+    out, last = megacrn_amd.gated_linear_recurrence(x, x, st)
+    assert out.shape == shape and torch.equal(last, st)
+    (g,) = torch.autograd.grad(last.sum(), st)
+    assert torch.equal(g, torch.ones_like(st))
+    assert megacrn_amd.gated_linear_recurrence_step(torch.zeros(0, 3, 8, device="cuda"), torch.zeros(0, 3, 8, device="cuda"), torch.zeros(0, 3, 8, device="cuda")).shape == (0, 3, 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("G", [24, 3, 1])
+def test_steps_are_the_sequence(dt, G):
+    """Steps taken one by one give the states of the whole sequence."""
+    import megacrn_amd
+    gate, cand, st, keep, _, _ = (None if t is None else t.cuda() for t in _inputs(4, 13, 6, 24, G, dt, True, 1))
+    out, last = megacrn_amd.gated_linear_recurrence(gate, cand, st, keep)
+    now = st.clone()
+    for t in range(13):
+        o = megacrn_amd.gated_linear_recurrence_step(gate[:, t], cand[:, t], now, keep[:, t])
+        assert o.dtype == TORCH[dt]
+        want = O.glr_fwd(_np(gate[:, :t + 1].cpu()), _np(cand[:, :t + 1].cpu()), _np(st.cpu()), keep[:, :t + 1].cpu().numpy())
+        _close(o, want[0][:, -1], want[2][:, -1] + O.half_step(want[0][:, -1], dt), f"step {t}")
+    _close(now, want[1], want[2][:, -1] + O.half_step(want[1], "f32"), "state")
+    _close(last, want[1], want[2][:, -1] + O.half_step(want[1], "f32"), "last")
+    with pytest.raises(RuntimeError):
+        megacrn_amd.gated_linear_recurrence_step(gate[:, 0].requires_grad_(), cand[:, 0], now)
+
+
+@pytest.mark.gpu
+def test_nan_stays_in_its_row():
+    """A NaN that is not masked reaches its own channel's later steps and nothing else."""
+    import megacrn_amd
+    gate, cand, st, _, _, _ = (None if t is None else t.cuda() for t in _inputs(2, 300, 3, 8, 8, "f32", False, 2))
+    want, _ = megacrn_amd.gated_linear_recurrence(gate, cand, st)
+    cand[1, 150, 2, 5] = float("nan")
+    got, last = megacrn_amd.gated_linear_recurrence(gate, cand, st)
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    hit[1, 150:, 2, 5] = True
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], want[~hit]) and torch.isnan(last).sum() == 1
+
+
+@pytest.mark.gpu
+def test_graph_replay_and_other_stream():
+    """Forward, backward and a serving step captured once and replayed on new inputs, with eager work between; then the same
+    calls on a stream of their own.  One plan and one order of sums: bit for bit."""
+    import megacrn_amd
+    shapes = [(2, 24, 5, 16), (1, 2100, 1, 12)]
+    for B, T, N, H in shapes:
+        def fresh(seed):
+            return [None if t is None else t.cuda() for t in _inputs(B, T, N, H, H, "f32", True, seed)]
+
+        def run(gate, cand, st, keep, dout, dlast):
+            leaves = [t.detach().requires_grad_() for t in (gate, cand, st)]
+            out, last = megacrn_amd.gated_linear_recurrence(*leaves, keep)
+            return (out.detach(), last.detach()) + torch.autograd.grad((out, last), leaves, (dout, dlast))
+
+        static = fresh(0)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        now = static[2].clone()
+        with torch.cuda.graph(graph):
+            held = run(*static)
+            megacrn_amd.gated_linear_recurrence_step(static[0][:, 0], static[1][:, 0], now, static[3][:, 0])
+        for seed in (1, 2, 3):
+            new = fresh(seed)
+            for s, t in zip(static, new):
+                s.copy_(t)
+            now.copy_(new[2])
+            graph.replay()
+            want = run(*new)
+            torch.cuda.synchronize()
+            for a, b in zip(held, want):
+                assert torch.equal(a, b)
+            first = new[2].clone()
+            megacrn_amd.gated_linear_recurrence_step(new[0][:, 0], new[1][:, 0], first, new[3][:, 0])
+            assert torch.equal(now, first)
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            other = run(*new)
+        torch.cuda.synchronize()
+        for a, b in zip(other, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_output_changed_before_backward_is_noticed():
+    import megacrn_amd
+    gate, cand, st, _, _, _ = (None if t is None else t.cuda() for t in _inputs(1, 20, 2, 4, 4, "f32", False, 2))
+    out, last = megacrn_amd.gated_linear_recurrence(gate.requires_grad_(), cand, st)
+    loss = out.sum()
+    with torch.no_grad():
+        out.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.gpu
+def test_many_elements():
+    """More than 2^31 elements of gate and cand (bf16): offsets past 32 bits.  Gates of -100 make every step its candidate."""
+    import megacrn_amd
+    B, T, N, H = 3, 4200, 2700, 64
+    gate = torch.full((1, 1, 1, 1), -100.0, dtype=torch.bfloat16, device="cuda").expand(B, T, N, 1)
+    cand = torch.empty(B, T, N, H, dtype=torch.bfloat16, device="cuda")
+    cand.copy_((torch.arange(T, device="cuda").view(1, T, 1, 1) % 100 + torch.arange(B, device="cuda").view(B, 1, 1, 1)).to(torch.bfloat16))
+    assert cand.numel() > 2 ** 31
+    with torch.no_grad():
+        out, last = megacrn_amd.gated_linear_recurrence(gate, cand, None, activation="none")
+    for b in range(B):
+        assert torch.equal(out[b], cand[b])
+    assert torch.equal(last, cand[:, -1].float())
+
+
+@pytest.mark.gpu
+def test_agl_cell_training_run():
+    """The module as it is used: supports -> graph convolution of all steps -> recurrence -> loss -> gradients, against float64; then
+    its steps in place against the sequence, and an AdamW update of all its parameters."""
+    import megacrn_amd
+    torch.manual_seed(3)
+    B, T, N, C, H, K = 2, 11, 9, 3, 8, 3
+    cell = megacrn_amd.AGLRCell(N, C, H, K).cuda()
+    assert set(cell.state_dict()) == {"gate_cand.weights", "gate_cand.bias"}
+    S = [torch.softmax(torch.randn(N, N), -1) for _ in range(2)]
+    x, st, mask = torch.randn(B, T, N, C), torch.randn(B, N, H), torch.rand(B, T, N) > 0.2
+    d = torch.randn(B, T, N, H)
+    sup = [s.cuda() for s in S]
+    out, last = cell(x.cuda(), st.cuda(), sup, mask.cuda())
+    (out * d.cuda()).sum().backward()
+    W, b = (p.detach().cpu().double().numpy() for p in (cell.gate_cand.weights, cell.gate_cand.bias))
+    y, cache = MO.agcn_fwd(_np(x).reshape(B * T, N, C), [_np(s) for s in S], W, b, K)
+    y = y.reshape(B, T, N, 2 * H)
+    want, wlast, _, gc = O.glr_fwd(y[..., :H].copy(), y[..., H:].copy(), _np(st), mask.numpy())
+    dg, dc, _, _, _, _ = O.glr_bwd(gc, _np(d), None)
+    back = MO.agcn_bwd(np.concatenate([dg, dc], -1).reshape(B * T, N, 2 * H), cache)
+    grads = [g for g in back if isinstance(g, np.ndarray) and g.shape in (W.shape, b.shape)]
+    # the convolution's own contract is 1e-4 of a tensor's scale; the recurrence's step is no steeper than 1 in gate and candidate
+    for got, ref in ((out, want), (last, wlast), (cell.gate_cand.weights.grad, grads[0]), (cell.gate_cand.bias.grad, grads[1])):
+        assert np.abs(got.detach().cpu().double().numpy() - ref).max() <= 2e-4 * np.abs(ref).max()
+    now = st.cuda().clone()
+    for t in range(T):
+        o = cell.step(x[:, t].cuda(), now, sup, mask[:, t].cuda())
+        assert np.abs(o.cpu().double().numpy() - want[:, t]).max() <= 2e-4 * np.abs(want).max()
+    opt = megacrn_amd.AdamW(cell.parameters(), lr=1e-2, max_grad_norm=1.0, state_bits=8)
+    before = [p.detach().clone() for p in cell.parameters()]
+    opt.step()
+    for p, q in zip(cell.parameters(), before):
+        assert torch.isfinite(p).all() and 0 < (p - q).abs().max() <= 1.1e-2 * (1 + q.abs().max())
