@@ -236,8 +236,9 @@ size_t mcrn_adamw_workspace_bytes(const mcrn_adamw_t* a, const long long* numel)
 int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* const* grads, const long long* numel,
                     const double* lr, const double* weight_decay, int* step, void* m, void* v, unsigned char* m_scale,
                     unsigned char* v_scale, float* master, void* ws, size_t ws_bytes, float* total_norm, void* stream);
-/* The values that n codes stand for (n a multiple of 64): second = 0 for m, 1 for v. */
-int mcrn_adamw_unpack(const unsigned char* codes, const unsigned char* scale, long long n, int second, float* out, void* stream);
+/* The values that the n codes of each arena stand for (n a multiple of 64), fp32. */
+int mcrn_adamw_unpack(const unsigned char* m, const unsigned char* m_scale, const unsigned char* v, const unsigned char* v_scale,
+                      long long n, float* out_m, float* out_v, void* stream);
 
 /* ---- trainer loss, forward + backward (model/traintest_MegaCRN.py:118-125, model/utils.py:126-133) ----
  * loss = masked_mae(output*std+mean, labels*std+mean) + lamb*TripletMarginLoss(margin)(query,pos,neg)

@@ -54,18 +54,12 @@ class Grads(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in PARAM_FIELDS]
 
 
-class Glr(C.Structure):
-    _fields_ = ([(n, C.c_int) for n in ("B", "T", "N", "H", "G", "dtype", "activation", "reserved")]
-                + [(n, C.c_longlong * 3) for n in ("gate_s", "cand_s", "mask_s", "dout_s")])
-
-
 class Adamw(C.Structure):
     _fields_ = [("ntensors", C.c_int), ("dtype", C.c_int), ("state_bits", C.c_int), ("seed", C.c_uint), ("on_device", C.c_int),
                 ("reserved", C.c_int)] + [(n, C.c_double) for n in ("beta1", "beta2", "eps", "max_norm", "grad_scale")]
 
 
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # MCRN_T_*
-ACTIVATIONS = {"none": 0, "tanh": 1}                                    # MCRN_ACT_*
+T_F32, T_BF16, T_F16 = 0, 1, 2                                          # MCRN_T_*
 
 
 def _load():
@@ -150,26 +144,29 @@ def _load():
                                   C.POINTER(C.c_double)]
     lib.mcrn_prof_clock_mhz.restype = i
     lib.mcrn_prof_clock_mhz.argtypes = [C.POINTER(C.c_double), C.POINTER(C.c_longlong)]
-    lib.mcrn_glr_checkpoint_floats.restype = sz
-    lib.mcrn_glr_checkpoint_floats.argtypes = [C.POINTER(Glr)]
-    lib.mcrn_glr_workspace_bytes.restype = sz
-    lib.mcrn_glr_workspace_bytes.argtypes = [C.POINTER(Glr), i]
-    lib.mcrn_glr_forward.restype = i
-    lib.mcrn_glr_forward.argtypes = [C.POINTER(Glr)] + [vp] * 4 + [vp, sz] + [vp] * 3 + [vp]
-    lib.mcrn_glr_backward.restype = i
-    lib.mcrn_glr_backward.argtypes = [C.POINTER(Glr)] + [vp] * 7 + [vp, sz] + [vp] * 3 + [vp]
     lib.mcrn_adamw_arena_elements.restype = ll
     lib.mcrn_adamw_arena_elements.argtypes = [C.POINTER(Adamw), C.POINTER(ll)]
     lib.mcrn_adamw_workspace_bytes.restype = sz
     lib.mcrn_adamw_workspace_bytes.argtypes = [C.POINTER(Adamw), C.POINTER(ll)]
-    lib.mcrn_adamw_step.restype = i
-    lib.mcrn_adamw_step.argtypes = [C.POINTER(Adamw), C.POINTER(vp), C.POINTER(vp), C.POINTER(ll)] + [vp] * 8 + [vp, sz, vp, vp]
-    lib.mcrn_adamw_unpack.restype = i
-    lib.mcrn_adamw_unpack.argtypes = [vp, vp, ll, i, vp, vp]
     return lib
 
 
 lib = _load()
+
+
+def _load_host():
+    """The C++ host nodes (csrc/host_nodes.cpp) call the library that is loaded here, through the addresses they get."""
+    try:
+        from . import _host
+    except ImportError as e:
+        raise ImportError(f"megacrn_amd/_host.so is missing or does not load ({e}): build it with `make -C megacrn_amd/csrc host`") from e
+    _host.bind({s: C.cast(getattr(lib, s), C.c_void_p).value
+                for s in ("mcrn_last_error", "mcrn_glr_checkpoint_floats", "mcrn_glr_workspace_bytes", "mcrn_glr_forward",
+                          "mcrn_glr_backward", "mcrn_adamw_step", "mcrn_adamw_unpack")})
+    return _host
+
+
+host = _load_host()
 
 F32, BF16X3, BF16 = 0, 1, 2
 PRECISIONS = {"f32": F32, "bf16x3": BF16X3, "bf16": BF16}

@@ -250,18 +250,18 @@ __global__ void adamw_prep_kernel(AdamwPrepP p) {
     p.dyn[k] = d;
 }
 
-// The values that codes stand for, four a thread.
-template <bool SECOND>
-__global__ __launch_bounds__(256) void adamw_unpack_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scale,
-                                                           float* __restrict__ out, long long n4) {
+// The values that codes stand for, four a thread: m (blockIdx.y 0) and v.
+__global__ __launch_bounds__(256) void adamw_unpack_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ ms, const uint8_t* __restrict__ v,
+                                                           const uint8_t* __restrict__ vs, float* __restrict__ om, float* __restrict__ ov, long long n4) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= n4) return;
-    const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[i];
-    const int s = scale[i * 4 / ADAMW_BLOCK];
-    float v[4];
+    const bool second = blockIdx.y != 0;
+    const uint32_t c = reinterpret_cast<const uint32_t*>(second ? v : m)[i];
+    const int s = (second ? vs : ms)[i * 4 / ADAMW_BLOCK];
+    float x[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = adamw_decode<SECOND>((c >> (8 * k)) & 0xffu, s);
-    AdamwF32::store4(out, i * 4, v);
+    for (int k = 0; k < 4; ++k) x[k] = second ? adamw_decode<true>((c >> (8 * k)) & 0xffu, s) : adamw_decode<false>((c >> (8 * k)) & 0xffu, s);
+    AdamwF32::store4(second ? ov : om, i * 4, x);
 }
 
 }  // namespace mcrn

@@ -60,6 +60,6 @@ unsigned adamw_key(unsigned seed, int id, unsigned step);
 hipError_t launch_adamw(const AdamwP& p, unsigned blocks, int dtype, int bits, hipStream_t st);
 hipError_t launch_adamw_norm(const AdamwNormP& p, unsigned blocks, int dtype, hipStream_t st);
 hipError_t launch_adamw_prep(const AdamwPrepP& p, hipStream_t st);
-hipError_t launch_adamw_unpack(const uint8_t* codes, const uint8_t* scale, float* out, long long n, bool second, hipStream_t st);
+hipError_t launch_adamw_unpack(const uint8_t* m, const uint8_t* ms, const uint8_t* v, const uint8_t* vs, long long n, float* om, float* ov, hipStream_t st);
 
 }  // namespace mcrn

@@ -25,12 +25,10 @@ hipError_t launch_adamw_prep(const AdamwPrepP& p, hipStream_t st) {
     hipLaunchKernelGGL(adamw_prep_kernel, dim3((unsigned)((p.nt + 63) / 64)), dim3(64), 0, st, p);
     return hipGetLastError();
 }
-hipError_t launch_adamw_unpack(const uint8_t* codes, const uint8_t* scale, float* out, long long n, bool second, hipStream_t st) {
+hipError_t launch_adamw_unpack(const uint8_t* m, const uint8_t* ms, const uint8_t* v, const uint8_t* vs, long long n, float* om, float* ov, hipStream_t st) {
     (void)hipGetLastError();
     const long long n4 = n / 4;
-    const dim3 grid((unsigned)((n4 + 255) / 256));
-    if (second) hipLaunchKernelGGL((adamw_unpack_kernel<true>), grid, dim3(256), 0, st, codes, scale, out, n4);
-    else hipLaunchKernelGGL((adamw_unpack_kernel<false>), grid, dim3(256), 0, st, codes, scale, out, n4);
+    hipLaunchKernelGGL(adamw_unpack_kernel, dim3((unsigned)((n4 + 255) / 256), 2), dim3(256), 0, st, m, ms, v, vs, om, ov, n4);
     return hipGetLastError();
 }
 

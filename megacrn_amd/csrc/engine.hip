@@ -3130,11 +3130,14 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     }
     return 0;
 }
-int mcrn_adamw_unpack(const unsigned char* codes, const unsigned char* scale, long long n, int second, float* out, void* stream) {
+int mcrn_adamw_unpack(const unsigned char* m, const unsigned char* m_scale, const unsigned char* v, const unsigned char* v_scale,
+                      long long n, float* out_m, float* out_v, void* stream) {
     ENTER();
-    if (n < 0 || n % ADAMW_BLOCK || n > (1ll << 40) || (n && (!codes || !scale || !out)) || ((uintptr_t)codes & 3) || ((uintptr_t)out & 15)) FAIL("adamw_unpack: bad arguments");
+    if (n < 0 || n % ADAMW_BLOCK || n > (1ll << 40) || (n && (!m || !m_scale || !v || !v_scale || !out_m || !out_v)) ||
+        (((uintptr_t)m | (uintptr_t)v) & 3) || (((uintptr_t)out_m | (uintptr_t)out_v) & 15))
+        FAIL("adamw_unpack: bad arguments");
     if (!n) return 0;
-    CK(launch_adamw_unpack(codes, scale, out, n, second != 0, (hipStream_t)stream));
+    CK(launch_adamw_unpack(m, m_scale, v, v_scale, n, out_m, out_v, (hipStream_t)stream));
     ++g_launches;
     return 0;
 }

@@ -10,8 +10,8 @@ import ctypes as C
 
 import torch
 
-from ._lib import lib, check, Adamw, DTYPES
-from .modules import _need_gpu, _stream
+from ._lib import lib, host, Adamw, T_F32, T_BF16
+from .modules import _need_gpu
 
 BLOCK = 64          # elements that share a scale of the 8-bit moments
 
@@ -60,7 +60,7 @@ class AdamW:
         self.state_bits, self.seed, self.capturable = state_bits, int(seed), bool(capturable)
         k = len(self.params)
         self._numel = (C.c_longlong * k)(*[p.numel() for p in self.params])
-        self._cfg = Adamw(k, DTYPES[self.dtype], state_bits, self.seed & 0xFFFFFFFF, int(self.capturable), 0, self.betas[0],
+        self._cfg = Adamw(k, T_F32 if self.dtype == torch.float32 else T_BF16, state_bits, self.seed & 0xFFFFFFFF, int(self.capturable), 0, self.betas[0],
                           self.betas[1], self.eps, self.max_grad_norm, 1.0)
         n = lib.mcrn_adamw_arena_elements(C.byref(self._cfg), self._numel)
         dev = self.device
@@ -80,20 +80,23 @@ class AdamW:
             for p, o in zip(self.params, self.offsets):
                 self.master[o:o + p.numel()].copy_(p.detach().reshape(-1))
         nb = lib.mcrn_adamw_workspace_bytes(C.byref(self._cfg), self._numel)
-        self._ws, self._nb = torch.zeros(nb, dtype=torch.uint8, device=dev), nb
+        self._ws = torch.zeros(nb, dtype=torch.uint8, device=dev)
         self.total_norm = torch.zeros((), device=dev)
-        self._ptrs = (C.c_void_p * k)()
-        self._grads = (C.c_void_p * k)()
         self._lr, self._wd, self._steps = (C.c_double * k)(), (C.c_double * k)(), (C.c_int * k)()
-        self._dev = None
+        self._dev = self._seen = None
         if self.capturable:
             self._dev = (torch.zeros(k, dtype=torch.float64, device=dev), torch.zeros(k, dtype=torch.float64, device=dev),
                          torch.zeros(k, dtype=torch.int32, device=dev))
             self.sync_lr()
+        self._numel_at = C.addressof(self._numel)
+        self._hyper = tuple(C.addressof(a) for a in (self._lr, self._wd, self._steps)) if self._dev is None else tuple(t.data_ptr() for t in self._dev)
 
     # -- learning rates
     def _read_groups(self):
-        i = 0
+        now = [(g["lr"], g["weight_decay"]) for g in self.param_groups]
+        if now == self._seen:
+            return
+        self._seen, i = now, 0
         for g in self.param_groups:
             lr, wd = g["lr"], g["weight_decay"]
             for _ in g["params"]:
@@ -115,44 +118,14 @@ class AdamW:
         params = self.params
         if grads is None:
             grads = [p.grad for p in params]
-        elif len(grads) != len(params):
-            raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(params)} parameters")
-        capturing = torch.cuda.is_current_stream_capturing()
-        if capturing and not self.capturable:
-            raise RuntimeError("AdamW.step inside a graph capture needs capturable=True: its step counts would be replayed unchanged")
-        held = []                                        # contiguous copies live until the kernels are queued
-        for i, (p, g) in enumerate(zip(params, grads)):
-            if g is None:
-                self._grads[i] = None
-                continue
-            if g.dtype != self.dtype or g.device != self.device or g.shape != p.shape:
-                raise ValueError(f"AdamW.step: gradient {i} must be a {self.dtype} tensor of shape {tuple(p.shape)} on {self.device}")
-            if p.dtype != self.dtype or p.device != self.device or not p.is_contiguous() or p.numel() != self._numel[i]:
-                raise ValueError(f"AdamW.step: parameter {i} is no longer the contiguous {self.dtype} tensor that the optimizer was made for")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                held.append(g)
-            self._ptrs[i], self._grads[i] = p.data_ptr(), g.data_ptr()
         if not self.capturable:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW.step inside a graph capture needs capturable=True: its step counts would be replayed unchanged")
             self._read_groups()
-            for i, g in enumerate(grads):
-                self._steps[i] += g is not None
-        lr, wd, steps = (self._lr, self._wd, self._steps) if self._dev is None else (t.data_ptr() for t in self._dev)
         cfg = self._cfg
         cfg.max_norm, cfg.grad_scale = self.max_grad_norm, float(grad_scale)
-        norm = self.total_norm.data_ptr() if self.max_grad_norm > 0 else None
-        with torch.cuda.device(self.device):
-            try:
-                check(lib.mcrn_adamw_step(C.byref(cfg), self._ptrs, self._grads, self._numel, lr, wd, steps, self._m.data_ptr(),
-                                          self._v.data_ptr(), None if self._ms is None else self._ms.data_ptr(),
-                                          None if self._vs is None else self._vs.data_ptr(),
-                                          None if self.master is None else self.master.data_ptr(), self._ws.data_ptr(), self._nb,
-                                          norm, _stream()), "mcrn_adamw_step")
-            except RuntimeError:
-                if not self.capturable:                  # nothing was updated
-                    for i, g in enumerate(grads):
-                        self._steps[i] -= g is not None
-                raise
+        host.adamw_step(C.addressof(cfg), params, grads, self._numel_at, *self._hyper, self._m, self._v, self._ms, self._vs,
+                        self.master, self._ws, self.total_norm if self.max_grad_norm > 0 else None)
 
     def zero_grad(self, set_to_none=True):
         for p in self.params:
@@ -168,14 +141,7 @@ class AdamW:
         32 bits: the optimizer's own; 8 bits: what the codes stand for."""
         if self.state_bits == 32:
             return self._m, self._v
-        out = []
-        with torch.cuda.device(self.device):
-            for codes, scale, second in ((self._m, self._ms, 0), (self._v, self._vs, 1)):
-                t = torch.empty(codes.numel(), device=self.device)
-                check(lib.mcrn_adamw_unpack(codes.data_ptr(), scale.data_ptr(), codes.numel(), second, t.data_ptr(), _stream()),
-                      "mcrn_adamw_unpack")
-                out.append(t)
-        return tuple(out)
+        return host.adamw_unpack(self._m, self._ms, self._v, self._vs)
 
     def steps(self):
         """Updates of each tensor so far."""

@@ -85,19 +85,29 @@ def test_step_refusals(over, kind):
 def test_c_sizes():
     """Checkpoints: one state in fp32 before every 8th step but the first, 16-bit types only; a workspace for long sequences with few channels."""
     import ctypes as C
-    from megacrn_amd._lib import lib, Glr
+    from megacrn_amd._lib import lib
 
-    def d(B, T, N, H, G, dtype):
-        return C.byref(Glr(B, T, N, H, G, dtype, 1, 0))
-    assert lib.mcrn_glr_checkpoint_floats(d(2, 8, 3, 4, 4, 1)) == 0
-    assert lib.mcrn_glr_checkpoint_floats(d(2, 9, 3, 4, 4, 1)) == 24
-    assert lib.mcrn_glr_checkpoint_floats(d(2, 17, 3, 4, 4, 2)) == 48
-    assert lib.mcrn_glr_checkpoint_floats(d(2, 17, 3, 4, 4, 0)) == 0
-    assert lib.mcrn_glr_checkpoint_floats(d(2, 0, 3, 4, 4, 1)) == 0
-    assert lib.mcrn_glr_workspace_bytes(d(1, 1, 207, 64, 64, 0), 1) == 0
-    assert lib.mcrn_glr_workspace_bytes(d(1, 20000, 1, 33, 33, 0), 0) > 0
-    for bad in (d(-1, 8, 3, 4, 4, 1), d(2, 8, 3, 4, 3, 1), d(2, 8, 3, 4, 4, 3), d(2, 8, 3, 0, 1, 0)):
-        assert lib.mcrn_glr_workspace_bytes(bad, 0) == 0
+    class Glr(C.Structure):                                # mcrn_glr_t
+        _fields_ = [("i", C.c_int * 8), ("s", C.c_longlong * 12)]
+
+    def ck(*a):
+        f = lib.mcrn_glr_checkpoint_floats
+        f.restype, f.argtypes = C.c_size_t, [C.POINTER(Glr)]
+        return f(C.byref(Glr((C.c_int * 8)(*a, 1, 0))))
+
+    def ws(*a, backward=0):
+        f = lib.mcrn_glr_workspace_bytes
+        f.restype, f.argtypes = C.c_size_t, [C.POINTER(Glr), C.c_int]
+        return f(C.byref(Glr((C.c_int * 8)(*a, 1, 0))), backward)
+    assert ck(2, 8, 3, 4, 4, 1) == 0
+    assert ck(2, 9, 3, 4, 4, 1) == 24
+    assert ck(2, 17, 3, 4, 4, 2) == 48
+    assert ck(2, 17, 3, 4, 4, 0) == 0
+    assert ck(2, 0, 3, 4, 4, 1) == 0
+    assert ws(1, 1, 207, 64, 64, 0, backward=1) == 0
+    assert ws(1, 20000, 1, 33, 33, 0) > 0
+    for bad in ((-1, 8, 3, 4, 4, 1), (2, 8, 3, 4, 3, 1), (2, 8, 3, 4, 4, 3), (2, 8, 3, 0, 1, 0)):
+        assert ws(*bad) == 0
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -345,6 +355,15 @@ def test_graph_replay_and_other_stream():
         torch.cuda.synchronize()
         for a, b in zip(other, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_second_derivative_is_refused():
+    import megacrn_amd
+    gate, cand, st, _, _, _ = (None if t is None else t.cuda() for t in _inputs(1, 20, 2, 4, 4, "f32", False, 2))
+    out, _ = megacrn_amd.gated_linear_recurrence(gate.requires_grad_(), cand, st)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out.sum(), gate, create_graph=True)
 
 
 @pytest.mark.gpu
