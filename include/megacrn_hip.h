@@ -228,11 +228,11 @@ typedef struct mcrn_adamw {
     double beta1, beta2, eps, max_norm, grad_scale;
 } mcrn_adamw_t;
 long long mcrn_adamw_arena_elements(const mcrn_adamw_t* a, const long long* numel);
-/* Zero-filled once by the caller; belongs to one sequence of steps (word 0 counts arrivals and is left at 0). */
 size_t mcrn_adamw_workspace_bytes(const mcrn_adamw_t* a, const long long* numel);
 /* params, grads: host arrays of device pointers; grads[i] == NULL leaves tensor i and its moments as they are.
  * lr, weight_decay: doubles, step: int, one of each for every tensor; step is 1-based and is that of this update (on_device: the number of
- * updates so far).  m_scale, v_scale: 8-bit moments only; master: bf16 only.  total_norm: device float or NULL. */
+ * updates so far).  m_scale, v_scale: 8-bit moments only; master: bf16 only.  total_norm: device float that receives the norm when max_norm > 0, or
+ * NULL. */
 int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* const* grads, const long long* numel,
                     const double* lr, const double* weight_decay, int* step, void* m, void* v, unsigned char* m_scale,
                     unsigned char* v_scale, float* master, void* ws, size_t ws_bytes, float* total_norm, void* stream);

@@ -103,6 +103,26 @@ template <bool SECOND> __device__ __forceinline__ unsigned adamw_encode(float x,
     return SECOND ? code : code | ((__float_as_uint(x) >> 24) & 0x80u);
 }
 
+__device__ __forceinline__ double adamw_block_sum(double s, double* sh) {      // in every thread; sh: one double a wave
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+
+// What the gradients are multiplied by: grad_scale, and max_norm / norm where the norm over all tensors is larger.  Every block adds the
+// partial sums (a few hundred, from L2) in the same order: no further launch, no counter, the same number everywhere.
+__device__ __forceinline__ float adamw_factor(const AdamwP& p, double* sh) {
+    double s = 0.0;
+    for (int j = threadIdx.x; j < p.parts; j += 256) s += p.part[j];
+    s = adamw_block_sum(s, sh);
+    const float norm = (float)(sqrt(s) * (double)p.grad_scale);
+    if (p.norm && blockIdx.x == 0 && threadIdx.x == 0) p.norm[0] = norm;
+    const float c = p.max_norm / (norm + 1e-6f);
+    return p.grad_scale * (c > 1.f ? 1.f : c);                // a NaN norm makes every gradient NaN
+}
+
 // One block: `per` runs of 1024 elements of one tensor, four neighbours a thread.
 template <class X, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamwP p) {
@@ -112,7 +132,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwP p) {
     float step_size = t.step_size, inv_bc2 = t.inv_bc2, decay = t.decay;
     unsigned key = t.key;
     if (p.dyn) { const AdamwDyn d = p.dyn[t.id]; step_size = d.step_size; inv_bc2 = d.inv_bc2; decay = d.decay; key = d.key; }
-    const float factor = p.factor ? p.factor[0] : p.grad_scale;
+    __shared__ double sh[4];
+    const float factor = p.parts ? adamw_factor(p, sh) : p.grad_scale;
     const long long first = (long long)(blockIdx.x - t.blk0) * p.per * 1024;
     for (int r = 0; r < p.per; ++r) {
         const long long i = first + r * 1024 + threadIdx.x * 4;
@@ -189,51 +210,38 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwP p) {
     }
 }
 
-// Sum of squares in 64 bits (the squares of floats are exact there): a block's sum to part[], and the block that arrives last
-// adds all of them in their order - the same result whichever block that is - and leaves norm and factor.
+// Sums of squares in 64 bits (the squares of floats are exact there), one a block; adamw_kernel adds them in their order.
 template <class X>
 __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwNormP p) {
     const int ti = adamw_tensor(p);
     double s = 0.0;
     if (ti >= 0) {
         const AdamwT t = p.t[ti];
-        const long long first = (long long)(blockIdx.x - t.blk0) * p.per * 1024;
-        for (int r = 0; r < p.per; ++r) {
-            const long long i = first + r * 1024 + threadIdx.x * 4;
-            if (i >= t.n) break;
+        const long long first = (long long)(blockIdx.x - t.blk0) * p.per * 1024, end = min(t.n, first + p.per * 1024ll);
+        long long i = first + threadIdx.x * 4;
+        constexpr int U = 8;                                  // loads in flight
+        if (t.flags & ADAMW_VEC) {
+            for (; first + (i - first) / 1024 * 1024 + U * 1024 <= end; i += U * 1024) {
+                float g[U][4];
+#pragma unroll
+                for (int u = 0; u < U; ++u) X::load4(t.g, i + u * 1024, g[u]);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s = fma((double)g[u][k], (double)g[u][k], s);
+            }
+        }
+        for (; i < end; i += 1024) {
             float g[4] = {0.f, 0.f, 0.f, 0.f};
-            if (i + 4 <= t.n && (t.flags & ADAMW_VEC)) X::load4(t.g, i, g);
-            else for (int k = 0; k < 4; ++k) if (i + k < t.n) g[k] = X::load1(t.g, i + k);
+            if (i + 4 <= end && (t.flags & ADAMW_VEC)) X::load4(t.g, i, g);
+            else for (int k = 0; k < 4; ++k) if (i + k < end) g[k] = X::load1(t.g, i + k);
 #pragma unroll
             for (int k = 0; k < 4; ++k) s = fma((double)g[k], (double)g[k], s);
         }
     }
     __shared__ double sh[4];
-    __shared__ bool last;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __hip_atomic_store(p.part + p.blk0 + blockIdx.x, (sh[0] + sh[1]) + (sh[2] + sh[3]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __threadfence();
-        last = atomicInc(p.ticket, p.blocks - 1) == p.blocks - 1;      // wraps to 0 for the next call
-    }
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    s = 0.0;
-    for (unsigned j = threadIdx.x; j < p.blocks; j += 256) s += __hip_atomic_load(p.part + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const float norm = (float)(sqrt((sh[0] + sh[1]) + (sh[2] + sh[3])) * (double)fabsf(p.grad_scale));
-        const float c = p.max_norm / (norm + 1e-6f);
-        p.norm[0] = norm;
-        p.factor[0] = p.max_norm > 0.f ? p.grad_scale * (c > 1.f ? 1.f : c) : p.grad_scale;     // a NaN norm makes every gradient NaN
-    }
+    s = adamw_block_sum(s, sh);
+    if (threadIdx.x == 0) p.part[p.blk0 + blockIdx.x] = s;
 }
 
 // Steps counted on the device (a captured step is replayed with its own numbers): one thread a tensor.

@@ -33,18 +33,18 @@ struct AdamwP {
     void *m, *v;                          // arenas: float, or codes
     uint8_t *ms, *vs;                     // scale bytes, one for each 64 elements
     float* master;                        // arena of fp32 parameters (16-bit ones only)
-    const float* factor;                  // what the gradients are multiplied by (clipping), NULL: grad_scale
+    const double* part;                   // sums of squares of the gradients and their number (0: no clipping)
+    int parts;
+    float max_norm;
+    float* norm;                          // receives the norm, or NULL
     const AdamwDyn* dyn;                  // NULL: the tensors' own values
     float grad_scale, b1, c1, b2, c2, eps;   // c = 1 - b
 };
 struct AdamwNormP {
     AdamwT t[ADAMW_TENSORS];
     int nt, per;
-    unsigned blk0, blocks;                // first partial sum of this launch, partial sums of all launches
+    unsigned blk0;                        // first partial sum of this launch
     double* part;
-    unsigned* ticket;                     // 0 before the first launch; left at 0
-    float *norm, *factor;
-    float max_norm, grad_scale;
 };
 struct AdamwPrepP {
     const double *lr, *wd;                // device, one for each tensor

@@ -2939,7 +2939,7 @@ static bool glr_params(const mcrn_glr_t* d, GlrP& p) {
 size_t mcrn_glr_checkpoint_floats(const mcrn_glr_t* d) {
     GlrP p;
     if (!glr_params(d, p) || p.dtype == GLR_F32 || p.T < 1) return 0;
-    return (size_t)p.B * ((p.T - 1) / GLR_K) * p.N * p.H;
+    return (size_t)p.B * ((p.T - 1) / glr_steps(p.T)) * p.N * p.H;
 }
 size_t mcrn_glr_workspace_bytes(const mcrn_glr_t* d, int backward) {
     GlrP p;
@@ -2949,14 +2949,19 @@ size_t mcrn_glr_workspace_bytes(const mcrn_glr_t* d, int backward) {
         if (glr_plan(p, backward != 0)) most = std::max(most, glr_ws_bytes(p, backward != 0));
     return most;
 }
-// places the workspace behind the plan
-static bool glr_place(GlrP& p, bool backward, void* ws, size_t ws_bytes) {
+static bool glr_workspace(GlrP& p, bool backward, void* ws, size_t ws_bytes) {
     const size_t need = glr_ws_bytes(p, backward);
-    if (!need) return true;
-    if (!ws || ws_bytes < need || ((uintptr_t)ws & 255)) return false;
-    p.agg = (float*)ws;
-    p.part = (float*)((char*)ws + (need - (backward && p.parts > 1 ? (size_t)p.B * p.T * p.N * p.G * p.parts * 4 : 0)));
+    if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 255))) return false;
+    glr_place(p, ws);
     return true;
+}
+// A lane addresses its rows with 32 bits behind a base of its block: rows of a tile (128 at most, in time) and the nodes of a row
+static bool glr_near(const GlrP& p) {
+    const long long es = p.dtype == GLR_F32 ? 4 : 2, rows = GLR_TILE < p.T ? GLR_TILE : p.T, most = 1ll << 32;
+    auto fits = [&](bool used, long long st, long long sn, long long w, long long size) { return !used || (rows * st + p.N * sn + w) * size < most; };
+    const long long NH = (long long)p.N * p.H;
+    return fits(true, p.g_st, p.g_sn, p.G, es) && fits(true, p.c_st, p.c_sn, p.H, es) && fits(p.mask, p.m_st, p.m_sn, 1, 1) && fits(p.dout, p.d_st, p.d_sn, p.H, es) &&
+           fits(true, NH, 0, NH, 4);
 }
 static bool glr_aligned(const GlrP& p) {
     const uintptr_t s = p.dtype == GLR_F32 ? 3 : 1, all = (uintptr_t)p.gate | (uintptr_t)p.cand | (uintptr_t)p.out | (uintptr_t)p.dout | (uintptr_t)p.dgate | (uintptr_t)p.dcand;
@@ -2974,8 +2979,9 @@ int mcrn_glr_forward(const mcrn_glr_t* d, const void* gate, const void* cand, co
     p.ckpt = p.dtype == GLR_F32 ? nullptr : ckpt;
     if (!glr_aligned(p)) FAIL("glr_forward: a pointer is not aligned to its type");
     if (!glr_plan(p, false)) FAIL("glr_forward: too many sequences");
-    if (!glr_place(p, false, ws, ws_bytes)) FAIL("glr_forward: the workspace is too small or not 256-byte aligned");
-    fam(p.S > 1 ? "glr:fwd_split" : p.CL == 256 ? "glr:fwd_stream" : "glr:fwd_tile");
+    if (!glr_near(p)) FAIL("glr_forward: strides over time or nodes reach over 4 GB within %d steps", GLR_TILE);
+    if (!glr_workspace(p, false, ws, ws_bytes)) FAIL("glr_forward: the workspace is too small or not 256-byte aligned");
+    fam(p.chain ? "glr:fwd_chain" : p.S > 1 ? "glr:fwd_split" : p.CL == 256 ? "glr:fwd_stream" : "glr:fwd_tile");
     CK(launch_glr_forward(p, (hipStream_t)stream, &g_launches));
     return 0;
 }
@@ -2987,15 +2993,16 @@ int mcrn_glr_backward(const mcrn_glr_t* d, const void* gate, const void* cand, c
     if (!glr_params(d, p)) FAIL("glr_backward: bad sizes, type, activation or strides");
     if ((long long)p.B * p.N == 0) return 0;
     if (p.T > 0 && (!gate || !cand || !dgate || !dcand)) FAIL("glr_backward: gate, cand, dgate and dcand are needed");
-    if (p.T > GLR_K && !kept) FAIL("glr_backward: the forward's out (fp32) or checkpoints (16-bit types) are needed");
+    if (p.T > glr_steps(p.T) && !kept) FAIL("glr_backward: the forward's out (fp32) or checkpoints (16-bit types) are needed");
     p.gate = gate; p.cand = cand; p.mask = mask; p.h0 = state;
     if (p.dtype == GLR_F32) p.out = const_cast<void*>(kept);
     else p.ckpt = (float*)const_cast<void*>(kept);
     p.dout = dout; p.dlast = dlast; p.dgate = dgate; p.dcand = dcand; p.dstate = dstate;
     if (!glr_aligned(p)) FAIL("glr_backward: a pointer is not aligned to its type");
     if (!glr_plan(p, true)) FAIL("glr_backward: too many sequences");
-    if (!glr_place(p, true, ws, ws_bytes)) FAIL("glr_backward: the workspace is too small or not 256-byte aligned");
-    fam(p.S > 1 ? "glr:bwd_split" : p.CL == 256 ? "glr:bwd_stream" : "glr:bwd_tile");
+    if (!glr_near(p)) FAIL("glr_backward: strides over time or nodes reach over 4 GB within %d steps", GLR_TILE);
+    if (!glr_workspace(p, true, ws, ws_bytes)) FAIL("glr_backward: the workspace is too small or not 256-byte aligned");
+    fam(p.chain ? "glr:bwd_chain" : p.S > 1 ? "glr:bwd_split" : p.CL == 256 ? "glr:bwd_stream" : "glr:bwd_tile");
     CK(launch_glr_backward(p, (hipStream_t)stream, &g_launches));
     return 0;
 }
@@ -3019,14 +3026,13 @@ long long mcrn_adamw_arena_elements(const mcrn_adamw_t* a, const long long* nume
     for (int i = 0; i < a->ntensors; ++i) sum += (numel[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;
     return sum;
 }
-// runs of 1024 elements that a block of the norm works on: about 1024 blocks in all, one run at the least
-static int adamw_norm_runs(long long elements) { return (int)std::max<long long>(1, elements / (1024ll * 1024)); }
-static const size_t ADAMW_HEAD = 256;         // ticket, factor, norm
+// runs of 1024 elements that a block of the norm works on: about 512 blocks in all
+static int adamw_norm_runs(long long elements) { return (int)std::max<long long>(1, elements / (512ll * 1024)); }
 size_t mcrn_adamw_workspace_bytes(const mcrn_adamw_t* a, const long long* numel) {
     const long long n = mcrn_adamw_arena_elements(a, numel);
     if (n < 0) return 0;
     const long long each = 1024ll * adamw_norm_runs(n), parts = n / each + a->ntensors;
-    return ADAMW_HEAD + (size_t)parts * 8 + (size_t)a->ntensors * sizeof(AdamwDyn);
+    return (size_t)parts * 8 + (size_t)a->ntensors * sizeof(AdamwDyn);
 }
 int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* const* grads, const long long* numel,
                     const double* lr, const double* weight_decay, int* step, void* m, void* v, unsigned char* m_scale,
@@ -3051,13 +3057,11 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     }
     if (!live) return 0;
     const hipStream_t st = (hipStream_t)stream;
-    unsigned* ticket = (unsigned*)ws;
-    float* factor = (float*)ws + 1;
-    float* norm = total_norm ? total_norm : (float*)ws + 2;
-    double* part = (double*)((char*)ws + ADAMW_HEAD);
+    double* part = (double*)ws;
     const int runs_n = adamw_norm_runs(elements);
     AdamwDyn* dyn = (AdamwDyn*)((char*)part + (elements / (1024ll * runs_n) + a->ntensors) * 8);
-    const bool clip = a->max_norm > 0 || total_norm;
+    const bool clip = a->max_norm > 0;
+    unsigned parts = 0;
     // small steps spread over many blocks, large ones keep a block long enough to hide its start
     const int runs = live < (4ll << 20) ? 1 : 4;
 
@@ -3101,19 +3105,14 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     };
     if (clip) {
         AdamwNormP q;
-        unsigned all = 0;
-        for (int i = 0; i < a->ntensors; ++i)
-            if (grads[i]) all += (unsigned)((numel[i] + 1024ll * runs_n - 1) / (1024ll * runs_n));
         long long off = 0;
-        unsigned blk0 = 0;
         for (int i = 0; i < a->ntensors;) {
             const unsigned blocks = fill(i, off, q.t, q.nt, runs_n);
             if (!blocks) continue;
-            q.per = runs_n; q.blk0 = blk0; q.blocks = all; q.part = part; q.ticket = ticket; q.norm = norm; q.factor = factor;
-            q.max_norm = (float)a->max_norm; q.grad_scale = (float)a->grad_scale;
+            q.per = runs_n; q.blk0 = parts; q.part = part;
             CK(launch_adamw_norm(q, blocks, a->dtype, st));
             ++g_launches;
-            blk0 += blocks;
+            parts += blocks;
         }
     }
     AdamwP q;
@@ -3122,7 +3121,7 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
         const unsigned blocks = fill(i, off, q.t, q.nt, runs);
         if (!blocks) continue;
         q.per = runs; q.m = m; q.v = v; q.ms = m_scale; q.vs = v_scale; q.master = master;
-        q.factor = clip ? factor : nullptr; q.dyn = a->on_device ? dyn : nullptr; q.grad_scale = (float)a->grad_scale;
+        q.part = part; q.parts = (int)parts; q.max_norm = (float)a->max_norm; q.norm = clip ? total_norm : nullptr; q.dyn = a->on_device ? dyn : nullptr; q.grad_scale = (float)a->grad_scale;
         q.b1 = (float)a->beta1; q.c1 = (float)(1.0 - a->beta1); q.b2 = (float)a->beta2; q.c2 = (float)(1.0 - a->beta2); q.eps = (float)a->eps;
         fam(a->state_bits == 8 ? "adamw:8bit" : "adamw:32bit");
         CK(launch_adamw(q, blocks, a->dtype, a->state_bits, st));

@@ -5,10 +5,9 @@
 //     dcand = lam (1 - a) phi'(c)      dgate = sum over the gate's channels of lam a (1 - a)(h_{t-1} - c)      dstate = a_0 lam_0
 //
 // Both directions are first-order recurrences y' = A y + X whose maps compose: (A1, X1) then (A2, X2) = (A1 A2, A2 X1 + X2).
-// A block of 256 threads covers CL channel lanes (V channels each) x SEG = 256 / CL time segments of GLR_K steps.  A thread loads
-// its GLR_K steps into registers, reduces them to one map, the block composes the SEG maps through LDS, and the thread runs its steps
-// again from the state that enters its segment: every input is read from HBM once, whatever SEG is.  The block walks the time axis
-// tile by tile (SEG * GLR_K steps), the loads of the next tile in flight while the current one is computed.
+// A block of 256 threads covers CL channel lanes (V channels each) x SEG = 256 / CL time segments of K steps.  A thread loads its K
+// steps into registers, reduces them to one map, the block composes the SEG maps (lanes of a wave by row swaps, waves through LDS),
+// and the thread runs its steps from the state that enters its segment: every input is read from HBM once, whatever SEG is.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -17,63 +16,101 @@
 namespace mcrn {
 
 constexpr int GLR_THREADS = 256;
+// the scheduler does not move work across: a phase's temporaries die before the next one's live (else occupancy falls by a wave)
+#define GLR_PHASE() __builtin_amdgcn_sched_barrier(0)
+// a value is computed here and not where it is used: moved behind the wait, it would keep all its operands in registers
+#define GLR_HERE(x) asm volatile("" : "+v"(x))
+enum { GLR_WALK = 0, GLR_AGG = 1, GLR_CHAIN = 2 };
 
 // ---- storage types --------------------------------------------------------------------------------------------------
+// FINE: the step's functions keep all of fp32 (16-bit types: what their own rounding leaves of it, and fewer instructions)
 struct GlrF32 {
     typedef float S;
+    static constexpr bool FINE = true;
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
+    static __device__ __forceinline__ float inf() { return __builtin_inff(); }
 };
 struct GlrBf16 {
-    typedef uint16_t S;
-    static __device__ __forceinline__ float up(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
-    static __device__ __forceinline__ uint16_t down(float f) {          // round to nearest even; NaN stays NaN
-        uint32_t u = __float_as_uint(f);
-        if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-        return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-    }
+    typedef __bf16 S;
+    static constexpr bool FINE = false;
+    static __device__ __forceinline__ float up(__bf16 v) { return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, v) << 16); }
+    static __device__ __forceinline__ __bf16 down(float f) { return (__bf16)f; }     // to the nearest, ties to even, by the hardware
+    static __device__ __forceinline__ __bf16 inf() { return (__bf16)__builtin_inff(); }
 };
 struct GlrF16 {
     typedef _Float16 S;
+    static constexpr bool FINE = false;
     static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
     static __device__ __forceinline__ _Float16 down(float f) { return (_Float16)f; }
+    static __device__ __forceinline__ _Float16 inf() { return (_Float16)__builtin_inff(); }
 };
 
 template <class X, int V> struct alignas(sizeof(typename X::S) * V) GlrVec { typename X::S e[V]; };
 
-template <class X, int V> __device__ __forceinline__ GlrVec<X, V> glr_load(const void* p, long long at) {
-    return *reinterpret_cast<const GlrVec<X, V>*>(static_cast<const typename X::S*>(p) + at);
+// element i; a pair of bf16 is taken apart in its 32-bit word
+template <class X, int V> __device__ __forceinline__ float glr_up(const GlrVec<X, V>& r, int i) { return X::up(r.e[i]); }
+template <> __device__ __forceinline__ float glr_up<GlrBf16, 4>(const GlrVec<GlrBf16, 4>& r, int i) {
+    const uint2 w = __builtin_bit_cast(uint2, r);
+    const uint32_t u = i < 2 ? w.x : w.y;
+    return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
 }
-template <class X, int V> __device__ __forceinline__ void glr_store(void* p, long long at, const float* v) {
+// Addresses: a base that is the same for the whole block (scalar registers, advanced by scalar adds) + 32 bits of a lane's own bytes
+template <class X, int V> __device__ __forceinline__ GlrVec<X, V> glr_load(const char* base, uint32_t off) {
+    return *reinterpret_cast<const GlrVec<X, V>*>(base + off);
+}
+template <class X, int V> __device__ __forceinline__ void glr_store(char* base, uint32_t off, const float* v) {
     GlrVec<X, V> r;
 #pragma unroll
     for (int i = 0; i < V; ++i) r.e[i] = X::down(v[i]);
-    *reinterpret_cast<GlrVec<X, V>*>(static_cast<typename X::S*>(p) + at) = r;
+    *reinterpret_cast<GlrVec<X, V>*>(base + off) = r;
 }
+// K rows of a thread, from row seg * K of the tile on.  What lies behind the tile's last row `end` reads that one instead: with
+// `most` = the lane's bytes to its last row (all ones in a whole tile) that is one minimum a row, and no second path for the loads.
+template <class X, int V, int K>
+__device__ __forceinline__ void glr_rows(GlrVec<X, V>* r, const char* base, uint32_t lane, uint32_t st, int seg, bool full, int end) {
+    uint32_t off = lane + (uint32_t)(seg * K) * st, most = 0xffffffffu;
+    if (!full) {
+        const int at = min(seg * K, end);
+        off = lane + (uint32_t)at * st;
+        most = (uint32_t)(end - at) * st;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const uint32_t o = (uint32_t)k * st;
+        r[k] = glr_load<X, V>(base, off + (o < most ? o : most));
+    }
+}
+struct GlrByte {
+    typedef uint8_t S;
+};
 
 // ---- the functions of a step -----------------------------------------------------------------------------------------
-__device__ __forceinline__ float glr_exp(float x) {       // e^x, x <= 0, ~1 ulp: the product x log2(e) carries its rounding error along
+// 2^(x log2 e).  The product's rounding is an error of |x| u in the exponent; FINE carries it along (the guard keeps infinities).
+template <bool FINE> __device__ __forceinline__ float glr_exp(float x) {
     const float L2E = 1.44269502162933349609f, L2E_LO = 1.92596299112661746887e-8f;    // log2(e) = L2E + L2E_LO
     const float t = x * L2E;
-    const float lo = fmaf(x, L2E_LO, fmaf(x, L2E, -t));
     const float e = __builtin_amdgcn_exp2f(t);
-    return t < -126.f ? 0.f : fmaf(e, lo * 0.693147182464599609375f, e);
+    if (!FINE) return e;
+    const float lo = fmaf(x, L2E_LO, fmaf(x, L2E, -t)) * 0.693147182464599609375f;
+    return fabsf(t) < 128.f ? fmaf(e, lo, e) : e;
 }
-// sigmoid(-|g|) with the sign of g: z.  1 - a = z > 0 ? z : 1 + z, a (1 - a) = |z| - z^2; neither form cancels.
-__device__ __forceinline__ float glr_z(float g) {
-    const float e = glr_exp(-fabsf(g));
-    return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
+// 1 - sigmoid(g): its relative error stays that of the exponential, however little is forgotten
+template <bool FINE> __device__ __forceinline__ float glr_w(float g) { return __builtin_amdgcn_rcpf(1.f + glr_exp<FINE>(g)); }
+// the same and p = sigmoid(g)(1 - sigmoid(g)), from the exponential that cannot overflow
+template <bool FINE> __device__ __forceinline__ void glr_wp(float g, float& w, float& p) {
+    const float e = glr_exp<FINE>(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
+    w = g >= 0.f ? s : r;
+    p = s * r;
 }
-__device__ __forceinline__ float glr_w(float z) { return (int)__float_as_uint(z) >= 0 ? z : 1.f + z; }
-__device__ __forceinline__ float glr_tanh(float u) {
-    const float e = glr_exp(-2.f * fabsf(u));
-    const float far = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), u);
-    const float q = u * u;                                // near 0 the quotient cancels: Taylor's series to u^11, off by < 2^-25 below 0.35
-    float s = fmaf(q, -1382.f / 155925.f, 62.f / 2835.f);
-    s = fmaf(q, s, -17.f / 315.f);
+// 1 - 2 / (1 + e^2u), off by 2 u absolutely; below a quarter, where that shows, Taylor's series (next term below u / 4 of the value)
+template <bool FINE> __device__ __forceinline__ float glr_tanh(float u) {
+    const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + glr_exp<false>(2.f * u)), 1.f);
+    const float q = u * u;
+    float s = FINE ? fmaf(q, 62.f / 2835.f, -17.f / 315.f) : -17.f / 315.f;
     s = fmaf(q, s, 2.f / 15.f);
     s = fmaf(q, s, -1.f / 3.f);
-    return fabsf(u) < 0.35f ? fmaf(u * q, s, u) : far;
+    return fabsf(u) < 0.25f ? fmaf(u * q, s, u) : far;
 }
 
 // ---- where a thread works ----------------------------------------------------------------------------------------------
@@ -83,32 +120,41 @@ struct GlrAt {
     int gi, gl, part;          // its gate's index in (.., G), its lane among the gate's lanes, its part
     bool active;
 };
-template <int V, int CL, bool SHARED> __device__ __forceinline__ GlrAt glr_where(const GlrP& p) {
+// CHAIN: the chunk is the next one of the block's channels that no block has taken yet, so that the block which has to hand over the
+// state has started before; REV: from the last chunk on
+template <int V, int CL, bool SHARED, bool CHAIN, bool REV> __device__ __forceinline__ GlrAt glr_where(const GlrP& p) {
     GlrAt w;
     unsigned blk = blockIdx.x;
     const unsigned tile = blk % (unsigned)p.tiles;
     blk /= (unsigned)p.tiles;
     w.b = (int)(blk % (unsigned)p.B);
-    w.chunk = (int)(blk / (unsigned)p.B) + p.first;
+    if (CHAIN) {
+        __shared__ int taken;
+        if (threadIdx.x == 0) taken = (int)atomicAdd(p.ticket + (tile + (unsigned)w.b * (unsigned)p.tiles), 1u);
+        __syncthreads();
+        w.chunk = __builtin_amdgcn_readfirstlane(taken);
+        if (REV) w.chunk = p.S - 1 - w.chunk;
+    } else {
+        w.chunk = (int)(blk / (unsigned)p.B) + p.first;
+    }
     w.cl = (int)threadIdx.x % CL;
     w.seg = (int)threadIdx.x / CL;
     w.t0 = w.chunk * p.chunk;
     w.t1 = min(p.T, w.t0 + p.chunk);
     if (SHARED) {              // L lanes a (gate, part): channels behind the gate's last stay idle
-        const long long unit = (long long)tile * (CL / p.L) + w.cl / p.L;
+        const unsigned unit = tile * (unsigned)(CL / p.L) + w.cl / p.L;
         const int D = p.H / p.G;
         w.gl = w.cl % p.L;
-        w.part = (int)(unit % p.parts);
-        const long long ng = unit / p.parts;
+        w.part = (int)(unit % (unsigned)p.parts);
+        const unsigned ng = unit / (unsigned)p.parts;
         const int d = (w.part * p.L + w.gl) * V;
-        w.active = ng < (long long)p.N * p.G && d < D;
-        w.n = w.active ? (int)(ng / p.G) : 0;
-        w.gi = w.active ? (int)(ng % p.G) : 0;
+        w.active = ng < (unsigned)p.N * (unsigned)p.G && d < D;
+        w.n = w.active ? (int)(ng / (unsigned)p.G) : 0;
+        w.gi = w.active ? (int)(ng % (unsigned)p.G) : 0;
         w.ch = w.active ? w.gi * D + d : 0;
     } else {
-        const long long q = (long long)tile * CL + w.cl;
-        const int hv = p.H / V;
-        w.active = q < p.nq;
+        const unsigned q = tile * CL + w.cl, hv = p.H / V;
+        w.active = q < (unsigned)p.nq;
         w.n = w.active ? (int)(q / hv) : 0;
         w.ch = w.active ? (int)(q % hv) * V : 0;
         w.gi = w.ch;
@@ -118,137 +164,238 @@ template <int V, int CL, bool SHARED> __device__ __forceinline__ GlrAt glr_where
     return w;
 }
 
-// The maps of the block's SEG segments, composed: `enter` = what reaches the thread's segment when `carry` reaches the tile's first one
-// (its last, REV), and carry = what leaves the tile.  A[], X[] = the thread's own map.  lds: SEG x CL x V pairs, its own in every other call.
+// ---- composing the maps of a block's segments ---------------------------------------------------------------------------
+__device__ __forceinline__ float glr_f(unsigned u) { return __uint_as_float(u); }
+__device__ __forceinline__ unsigned glr_u(float f) { return __float_as_uint(f); }
+
+// First part: the thread's own map A[], X[] -> EA[], EX[], the wave's segments before the thread's (behind it, REV), and the waves' maps in
+// lds (GLR_THREADS / 64 x CL x V pairs, its own in every other call).
 template <int V, int CL, bool REV>
-__device__ __forceinline__ void glr_block_scan(float2* lds, int cl, int seg, const float* A, const float* X, float* carry, float* enter) {
-    constexpr int SEG = GLR_THREADS / CL;
+__device__ __forceinline__ void glr_scan_maps(float2* lds, int cl, const float* A, const float* X, float* EA, float* EX) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const bool odd = threadIdx.x & 16, upper = threadIdx.x & 32;
 #pragma unroll
-    for (int i = 0; i < V; ++i) lds[(seg * V + i) * CL + cl] = make_float2(A[i], X[i]);
+    for (int i = 0; i < V; ++i) {
+        float TA = A[i], TX = X[i];
+        EA[i] = 1.f; EX[i] = 0.f;
+        if (CL == 16) {                                    // four segments a wave, one in each row of 16 lanes
+            const auto sa = __builtin_amdgcn_permlane16_swap(glr_u(TA), glr_u(TA), false, false);      // even rows' values, odd rows' values
+            const auto sx = __builtin_amdgcn_permlane16_swap(glr_u(TX), glr_u(TX), false, false);
+            const float a0 = glr_f(sa[0]), a1 = glr_f(sa[1]), x0 = glr_f(sx[0]), x1 = glr_f(sx[1]);
+            const bool second = REV ? !odd : odd;
+            const float ea = second ? (REV ? a1 : a0) : 1.f, ex = second ? (REV ? x1 : x0) : 0.f;
+            const float pa = a0 * a1, px = REV ? fmaf(a0, x1, x0) : fmaf(a1, x0, x1);
+            const auto qa = __builtin_amdgcn_permlane32_swap(glr_u(pa), glr_u(pa), false, false);
+            const auto qx = __builtin_amdgcn_permlane32_swap(glr_u(px), glr_u(px), false, false);
+            const float b0 = glr_f(qa[0]), b1 = glr_f(qa[1]), y0 = glr_f(qx[0]), y1 = glr_f(qx[1]);
+            const bool later = REV ? !upper : upper;
+            EX[i] = later ? fmaf(ea, REV ? y1 : y0, ex) : ex;
+            EA[i] = later ? ea * (REV ? b1 : b0) : ea;
+            TA = b0 * b1;
+            TX = REV ? fmaf(b0, y1, y0) : fmaf(b1, y0, y1);
+        }
+        if (CL == 64 || (threadIdx.x & 63) < CL) lds[(wave * V + i) * CL + cl] = make_float2(TA, TX);
+        GLR_PHASE();
+    }
     __syncthreads();
+}
+// Second part: `enter` = what reaches the thread's segment when `carry` reaches the tile's first one (its last, REV); carry = what leaves the
+// tile; prod *= the product of all A (AGG).
+template <int V, int CL, bool REV, bool AGG>
+__device__ __forceinline__ void glr_scan_carry(const float2* lds, int cl, const float* EA, const float* EX, float* carry, float* prod, float* enter) {
+    constexpr int W = GLR_THREADS / 64;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         float h = carry[i], e = h;
 #pragma unroll
-        for (int j = 0; j < SEG; ++j) {
-            const int s = REV ? SEG - 1 - j : j;
+        for (int j = 0; j < W; ++j) {
+            const int s = REV ? W - 1 - j : j;
             const float2 m = lds[(s * V + i) * CL + cl];
-            e = s == seg ? h : e;
+            if (s == wave) e = h;
             h = fmaf(m.x, h, m.y);
+            if (AGG) prod[i] *= m.x;
         }
-        enter[i] = e;
+        enter[i] = CL == 16 ? fmaf(EA[i], e, EX[i]) : e;
         carry[i] = h;
+        GLR_PHASE();
     }
 }
 
+// Splits (WALK with more than one chunk): carry = what the maps of `n` chunks, one behind the other in the order of the walk, make of it.
+// The segments' threads take a run of chunks each, then the runs are composed as segments are.  at: the first one's A, X at at[NH];
+// step: from one to the next.
+template <int V, int CL>
+__device__ __forceinline__ void glr_chunks_before(float2* lds, const GlrAt& w, const float* at, long long step, long long NH, int n, float* carry) {
+    constexpr int SEG = GLR_THREADS / CL;
+    const int per = (n + SEG - 1) / SEG, j0 = w.seg * per, j1 = min(n, j0 + per);
+    float A[V], X[V], EA[V], EX[V], none[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { A[i] = 1.f; X[i] = 0.f; }
+#pragma unroll 4
+    for (int j = j0; j < j1; ++j) {
+        const float* g = at + j * step;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float a = g[i], x = g[NH + i];
+            X[i] = fmaf(a, X[i], x);
+            A[i] *= a;
+        }
+    }
+    glr_scan_maps<V, CL, false>(lds, w.cl, A, X, EA, EX);
+    glr_scan_carry<V, CL, false, false>(lds, w.cl, EA, EX, carry, none, none);
+}
+
+// ---- handing the state from block to block (CHAIN) ------------------------------------------------------------------------
+// A word of all ones says that the state is not there yet (a state of that NaN pattern is sent as the usual NaN).  Each word is valid by
+// itself: no fence, no flag.  The wait ends: see glr_where; the bound only turns a broken workspace into NaN instead of a hang.
+template <int V> __device__ __forceinline__ void glr_send(unsigned* at, const float* v) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const unsigned u = glr_u(v[i]);
+        __hip_atomic_store(at + i, u == 0xffffffffu ? 0x7fc00000u : u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+template <int V> __device__ __forceinline__ void glr_receive(const unsigned* at, float* v) {
+    for (int tries = 0; tries < (1 << 22); ++tries) {
+        bool there = true;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const unsigned u = __hip_atomic_load(at + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            v[i] = glr_f(u);
+            there = there && u != 0xffffffffu;
+        }
+        if (there) return;
+        __builtin_amdgcn_s_sleep(2);
+    }
+}
+__global__ void glr_clear_kernel(unsigned* __restrict__ words, long long tickets, long long n) {
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) words[i] = i < tickets ? 0u : 0xffffffffu;
+}
+
 // ---- forward -----------------------------------------------------------------------------------------------------------
-// AGG: only the chunk's map is wanted (agg[chunk][b][A | X][N*H]); otherwise the chunk starts from the state that the maps of the chunks before it give.
-template <class X, int V, int CL, bool SHARED, bool AGG>
-__global__ __launch_bounds__(GLR_THREADS) void glr_fwd_kernel(GlrP p) {
-    constexpr int K = GLR_K, SEG = GLR_THREADS / CL, VG = SHARED ? 1 : V;
-    __shared__ float2 lds[SEG > 1 ? 2 : 1][SEG > 1 ? SEG * CL * V : 1];
-    const GlrAt w = glr_where<V, CL, SHARED>(p);
+// WALK: the block walks its chunk tile by tile, from the state that the maps of the chunks before it give (one chunk: from h0).
+// AGG: only the chunk's map is wanted (agg[chunk][b][A | X][N*H]).  CHAIN: the chunk is one tile, its state comes from the block before.
+template <class X, int V, int K, int CL, bool SHARED, int MODE>
+__global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) void glr_fwd_kernel(GlrP p) {
+    constexpr bool AGG = MODE == GLR_AGG, CHAIN = MODE == GLR_CHAIN, REV = false;
+    constexpr int SEG = GLR_THREADS / CL, VG = SHARED ? 1 : V, W = GLR_THREADS / 64, span = SEG * K;
+    typedef typename X::S S;
+    __shared__ float2 lds[SEG > 1 ? 2 : 1][SEG > 1 ? W * CL * V : 1];
+    const GlrAt w = glr_where<V, CL, SHARED, CHAIN, REV>(p);
     const long long NH = (long long)p.N * p.H, hoff = (long long)w.n * p.H + w.ch;
-    const long long g_at = w.b * p.g_sb + w.n * p.g_sn + w.gi, c_at = w.b * p.c_sb + w.n * p.c_sn + w.ch, m_at = w.b * p.m_sb + w.n * p.m_sn;
+    const long long es = sizeof(S), rb = NH * es;          // bytes of an element, of a row of out
+    const char* pg = static_cast<const char*>(p.gate) + (w.b * p.g_sb + w.t0 * p.g_st) * es;
+    const char* pc = static_cast<const char*>(p.cand) + (w.b * p.c_sb + w.t0 * p.c_st) * es;
+    const char* pm = reinterpret_cast<const char*>(p.mask) + (w.b * p.m_sb + w.t0 * p.m_st);
+    char* po = static_cast<char*>(p.out) + ((long long)w.b * p.T + w.t0) * rb;
+    const uint32_t lg = (uint32_t)((w.n * p.g_sn + w.gi) * es), lc = (uint32_t)((w.n * p.c_sn + w.ch) * es), lm = (uint32_t)(w.n * p.m_sn);
+    const uint32_t lo = (uint32_t)(hoff * es) + (uint32_t)(w.seg * K) * (uint32_t)rb;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     int par = 0;
 
     float carry[V], prod[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) { carry[i] = 0.f; prod[i] = 1.f; }
     if (!AGG) {
-        if (p.h0 && w.active) {
+        if (p.h0 && w.active && (!CHAIN || w.chunk == 0)) {
 #pragma unroll
             for (int i = 0; i < V; ++i) carry[i] = p.h0[w.b * NH + hoff + i];
         }
-        for (int j = 0; j < w.chunk; ++j) {               // the chunks before this one
-            const float* g = p.agg + ((long long)j * p.B + w.b) * 2 * NH + hoff;
-#pragma unroll
-            for (int i = 0; i < V; ++i) carry[i] = fmaf(g[i], carry[i], g[NH + i]);
+        if (!CHAIN && CL == 16 && w.chunk > 0) {           // the chunks before this one
+            const long long step = (long long)p.B * 2 * NH;
+            glr_chunks_before<V, CL>(lds[1], w, p.agg + (long long)w.b * 2 * NH + hoff, step, NH, w.chunk, carry);
         }
     }
 
-    GlrVec<X, VG> rg[K];
-    GlrVec<X, V> rc[K];
-    uint8_t rm[K];
-    auto fetch = [&](int tb) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int t = min(tb + w.seg * K + k, w.t1 - 1);
-            rg[k] = glr_load<X, VG>(p.gate, g_at + t * p.g_st);
-            rc[k] = glr_load<X, V>(p.cand, c_at + t * p.c_st);
-            rm[k] = p.mask ? p.mask[m_at + t * p.m_st] : (uint8_t)1;
-        }
-    };
-    if (w.t0 < w.t1) fetch(w.t0);
-    for (int tb = w.t0; tb < w.t1; tb += SEG * K) {
+    for (int tb = w.t0; tb < w.t1; tb += span) {
         const int ts = tb + w.seg * K;
-        float ww[K][V], cc[K][V];                         // 1 - a and phi(cand); a masked step is w = 0, c = 0
+        const bool full = tb + span <= w.t1;
+        const bool live = SEG == 1 || tb + wave * (64 / CL) * K < w.t1;       // a wave behind the last step only takes part in the scan
+        float ww[K][V], cc[K][V];                          // 1 - a and phi(cand); a masked step is w = 0, c = 0
+        if (live) {
+            GlrVec<X, VG> rg[K];
+            GlrVec<X, V> rc[K];
+            GlrVec<GlrByte, 1> rm[K];
+            const int end = w.t1 - 1 - tb;
+            glr_rows<X, VG, K>(rg, pg, lg, (uint32_t)(p.g_st * es), w.seg, full, end);
+            glr_rows<X, V, K>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
+            if (p.mask) glr_rows<GlrByte, 1, K>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
+            if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give w = 0, c = 0
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const bool on = rm[k] != 0 && ts + k < w.t1;
+                for (int k = 0; k < K; ++k) {
+                    const bool on = ts + k < w.t1 && (!p.mask || rm[k].e[0] != 0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float wi = (SHARED && i) ? ww[k][0] : glr_w(glr_z(X::up(rg[k].e[SHARED ? 0 : i])));
-                ww[k][i] = on ? wi : 0.f;
-                cc[k][i] = on ? X::up(rc[k].e[i]) : 0.f;
+                    for (int i = 0; i < VG; ++i) rg[k].e[i] = on ? rg[k].e[i] : X::inf();
+#pragma unroll
+                    for (int i = 0; i < V; ++i) rc[k].e[i] = on ? rc[k].e[i] : (S)0.f;
+                }
             }
-        }
-        if (tb + SEG * K < w.t1) fetch(tb + SEG * K);
-        if (p.act) {
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < V; ++i) cc[k][i] = glr_tanh(cc[k][i]);
+                for (int i = 0; i < V; ++i) {
+                    ww[k][i] = (SHARED && i) ? ww[k][0] : glr_w<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
+                    cc[k][i] = glr_up<X, V>(rc[k], i);
+                }
+            if (p.act) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) cc[k][i] = glr_tanh<X::FINE>(cc[k][i]);
+            }
         }
+        GLR_PHASE();
+        pg += span * p.g_st * es;
+        pc += span * p.c_st * es;
+        pm += span * p.m_st;
         float h[V];
         if (SEG > 1 || AGG) {
             float A[V], Xl[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 A[i] = 1.f; Xl[i] = 0.f;
+            }
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     A[i] = fmaf(-ww[k][i], A[i], A[i]);
                     Xl[i] = fmaf(ww[k][i], cc[k][i] - Xl[i], Xl[i]);
                 }
             }
-            if (AGG) {
-                if (SEG == 1) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) { carry[i] = fmaf(A[i], carry[i], Xl[i]); prod[i] *= A[i]; }
-                } else {
-                    // the product of the tile's A: the same composition from carry 1 with X = 0
-                    float none[V], dummy[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) none[i] = 0.f;
-                    glr_block_scan<V, CL, false>(lds[par], w.cl, w.seg, A, Xl, carry, dummy);
-                    par ^= 1;
-                    glr_block_scan<V, CL, false>(lds[par], w.cl, w.seg, A, none, prod, dummy);
-                    par ^= 1;
-                }
-                continue;
-            }
-            glr_block_scan<V, CL, false>(lds[par], w.cl, w.seg, A, Xl, carry, h);
+            float EA[V], EX[V];
+            glr_scan_maps<V, CL, REV>(lds[par], w.cl, A, Xl, EA, EX);
+            if (CHAIN && w.chunk > 0 && w.active) glr_receive<V>(p.carry + ((long long)(w.chunk - 1) * p.B + w.b) * NH + hoff, carry);
+            glr_scan_carry<V, CL, REV, AGG>(lds[par], w.cl, EA, EX, carry, prod, h);
+            if (CHAIN && w.chunk < p.S - 1 && w.active && w.seg == 0) glr_send<V>(p.carry + ((long long)w.chunk * p.B + w.b) * NH + hoff, carry);
             par ^= 1;
+            if (AGG) continue;
+            GLR_PHASE();
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) h[i] = carry[i];
         }
+        if (live) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int i = 0; i < V; ++i) h[i] = fmaf(ww[k][i], cc[k][i] - h[i], h[i]);
-            const int t = ts + k;
-            if (w.active && t < w.t1 && p.out) glr_store<X, V>(p.out, ((long long)w.b * p.T + t) * NH + hoff, h);
+            if (w.active && p.out && (full || ts + k < w.t1)) glr_store<X, V>(po + k * rb, lo, h);
         }
-        if (p.ckpt && w.active && ts + K < p.T) {         // the state before step ts + K
+        }
+        po += span * rb;
+        if (p.ckpt && w.active && ts + K < p.T) {          // the state before step ts + K
             const long long nck = (p.T - 1) / K;
-            glr_store<GlrF32, V>(p.ckpt, ((long long)w.b * nck + ts / K) * NH + hoff, h);
+            glr_store<GlrF32, V>(reinterpret_cast<char*>(p.ckpt + ((long long)w.b * nck + tb / K) * NH), (uint32_t)((w.seg * NH + hoff) * 4), h);
         }
         if (SEG == 1) {
 #pragma unroll
             for (int i = 0; i < V; ++i) carry[i] = h[i];
         }
+        if (CHAIN) break;
     }
     if (!w.active || w.seg != 0) return;
     if (AGG) {
@@ -262,102 +409,151 @@ __global__ __launch_bounds__(GLR_THREADS) void glr_fwd_kernel(GlrP p) {
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------
+// sum over the L lanes of a gate, in every one of them
+template <int CTRL> __device__ __forceinline__ float glr_add_dpp(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float glr_lane_sum(float s, int L) {
+    if (L > 1) s = glr_add_dpp<0xB1>(s);                   // neighbours
+    if (L > 2) s = glr_add_dpp<0x4E>(s);                   // pairs
+    if (L > 4) s = glr_add_dpp<0x141>(s);                  // halves of 8 lanes, mirrored
+    if (L > 8) s = glr_add_dpp<0x140>(s);                  // halves of 16 lanes, mirrored
+    if (L > 16) s += __shfl_xor(s, 16, 64);
+    if (L > 32) s += __shfl_xor(s, 32, 64);
+    return s;
+}
+
 // Walks the time axis from its end; `carry` is mu_{t+1} = a_{t+1} lam_{t+1}, what reaches step t from the steps behind it.
-template <class X, int V, int CL, bool SHARED, bool AGG>
-__global__ __launch_bounds__(GLR_THREADS) void glr_bwd_kernel(GlrP p) {
-    constexpr int K = GLR_K, SEG = GLR_THREADS / CL, VG = SHARED ? 1 : V;
-    __shared__ float2 lds[SEG > 1 ? 2 : 1][SEG > 1 ? SEG * CL * V : 1];
-    const GlrAt w = glr_where<V, CL, SHARED>(p);
-    const long long NH = (long long)p.N * p.H, hoff = (long long)w.n * p.H + w.ch;
-    const long long g_at = w.b * p.g_sb + w.n * p.g_sn + w.gi, c_at = w.b * p.c_sb + w.n * p.c_sn + w.ch, m_at = w.b * p.m_sb + w.n * p.m_sn;
-    const long long d_at = w.b * p.d_sb + w.n * p.d_sn + w.ch, nck = (p.T - 1) / K;
+template <class X, int V, int K, int CL, bool SHARED, int MODE>
+__global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
+    constexpr bool AGG = MODE == GLR_AGG, CHAIN = MODE == GLR_CHAIN, REV = true;
+    constexpr int SEG = GLR_THREADS / CL, VG = SHARED ? 1 : V, W = GLR_THREADS / 64, span = SEG * K;
+    typedef typename X::S S;
+    __shared__ float2 lds[SEG > 1 ? 2 : 1][SEG > 1 ? W * CL * V : 1];
+    const GlrAt w = glr_where<V, CL, SHARED, CHAIN, REV>(p);
+    const long long NH = (long long)p.N * p.H, NG = (long long)p.N * p.G, hoff = (long long)w.n * p.H + w.ch, nck = (p.T - 1) / K;
+    const long long es = sizeof(S), rb = NH * es, gb = NG * es;
+    const int ntile = (w.t1 - w.t0 + span - 1) / span, tl = w.t0 + (ntile - 1) * span;      // tiles, first step of the last one
+    const char* pg = static_cast<const char*>(p.gate) + (w.b * p.g_sb + tl * p.g_st) * es;
+    const char* pc = static_cast<const char*>(p.cand) + (w.b * p.c_sb + tl * p.c_st) * es;
+    const char* pd = static_cast<const char*>(p.dout) + (w.b * p.d_sb + tl * p.d_st) * es;
+    const char* pm = reinterpret_cast<const char*>(p.mask) + (w.b * p.m_sb + tl * p.m_st);
+    char* pdc = static_cast<char*>(p.dcand) + ((long long)w.b * p.T + tl) * rb;
+    char* pdg = static_cast<char*>(p.dgate) + ((long long)w.b * p.T + tl) * gb;
+    const uint32_t lg = (uint32_t)((w.n * p.g_sn + w.gi) * es), lc = (uint32_t)((w.n * p.c_sn + w.ch) * es), lm = (uint32_t)(w.n * p.m_sn);
+    const uint32_t ld = (uint32_t)((w.n * p.d_sn + w.ch) * es), ldc = (uint32_t)(hoff * es) + (uint32_t)(w.seg * K) * (uint32_t)rb;
+    const uint32_t ldg = (uint32_t)(((long long)w.n * p.G + w.gi) * es) + (uint32_t)(w.seg * K) * (uint32_t)gb;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     int par = 0;
 
     float carry[V], prod[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) { carry[i] = 0.f; prod[i] = 1.f; }
     if (!AGG) {
-        if (p.dlast && w.active) {
+        if (p.dlast && w.active && (!CHAIN || w.chunk == p.S - 1)) {
 #pragma unroll
             for (int i = 0; i < V; ++i) carry[i] = p.dlast[w.b * NH + hoff + i];
         }
-        for (int j = p.S - 1; j > w.chunk; --j) {         // the chunks behind this one
-            const float* g = p.agg + ((long long)j * p.B + w.b) * 2 * NH + hoff;
-#pragma unroll
-            for (int i = 0; i < V; ++i) carry[i] = fmaf(g[i], carry[i], g[NH + i]);
+        if (!CHAIN && CL == 16 && w.chunk < p.S - 1) {     // the chunks behind this one
+            const long long step = (long long)p.B * 2 * NH;
+            glr_chunks_before<V, CL>(lds[1], w, p.agg + ((long long)(p.S - 1) * p.B + w.b) * 2 * NH + hoff, -step, NH, p.S - 1 - w.chunk, carry);
         }
     }
 
-    GlrVec<X, VG> rg[K];
-    GlrVec<X, V> rc[K], rd[K];
-    GlrVec<GlrF32, V> rs;                                 // the state before the segment's first step
-    uint8_t rm[K];
-    auto fetch = [&](int tb) {
-        const int ts = tb + w.seg * K;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int t = min(ts + k, w.t1 - 1);
-            rg[k] = glr_load<X, VG>(p.gate, g_at + t * p.g_st);
-            if (!AGG) rc[k] = glr_load<X, V>(p.cand, c_at + t * p.c_st);
-            if (p.dout) rd[k] = glr_load<X, V>(p.dout, d_at + t * p.d_st);
-            rm[k] = p.mask ? p.mask[m_at + t * p.m_st] : (uint8_t)1;
-        }
-        if (!AGG) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) rs.e[i] = 0.f;
-            if (ts == 0) {
-                if (p.h0) rs = glr_load<GlrF32, V>(p.h0, w.b * NH + hoff);
-            } else if (ts < w.t1) {                       // f32: out_{ts-1} is that state
-                rs = p.dtype == GLR_F32 ? glr_load<GlrF32, V>(p.out, ((long long)w.b * p.T + ts - 1) * NH + hoff)
-                                        : glr_load<GlrF32, V>(p.ckpt, ((long long)w.b * nck + ts / K - 1) * NH + hoff);
-            }
-        }
-    };
-    const int span = SEG * K, ntile = (w.t1 - w.t0 + span - 1) / span;
-    if (ntile > 0) fetch(w.t0 + (ntile - 1) * span);
     for (int it = ntile - 1; it >= 0; --it) {
         const int tb = w.t0 + it * span, ts = tb + w.seg * K;
-        float ww[K][V], wc[K][V], q[K][V], dd[K][V];      // 1 - a, its product with phi', a (1 - a)(h_{t-1} - c), dout
-        float h[V];
+        const bool full = tb + span <= w.t1;
+        const bool live = SEG == 1 || tb + wave * (64 / CL) * K < w.t1;       // a wave behind the last step only takes part in the scan
+        float ww[K][V], wc[K][V], q[K][V], dd[K][V];       // 1 - a, its product with phi', a (1 - a)(h_{t-1} - c), dout
+        if (live) {
+            GlrVec<X, VG> rg[K];
+            GlrVec<X, V> rc[K], rd[K];
+            GlrVec<GlrF32, V> rs;                          // the state before the segment's first step
+            GlrVec<GlrByte, 1> rm[K];
+            const int end = w.t1 - 1 - tb;
+            glr_rows<X, VG, K>(rg, pg, lg, (uint32_t)(p.g_st * es), w.seg, full, end);
+            if (!AGG) glr_rows<X, V, K>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
+            if (p.dout) {
+                glr_rows<X, V, K>(rd, pd, ld, (uint32_t)(p.d_st * es), w.seg, full, end);
+            } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = AGG ? 0.f : rs.e[i];
+                for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const bool in = ts + k < w.t1, on = rm[k] != 0 && in;
-            float z = 0.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if (!SHARED || i == 0) z = on ? glr_z(X::up(rg[k].e[SHARED ? 0 : i])) : 0.f;
-                ww[k][i] = glr_w(z);
-                q[k][i] = fmaf(-z, z, fabsf(z));
-                dd[k][i] = in && p.dout ? X::up(rd[k].e[i]) : 0.f;
-                wc[k][i] = !AGG && on ? X::up(rc[k].e[i]) : 0.f;
+                    for (int i = 0; i < V; ++i) rd[k].e[i] = (S)0.f;
             }
-        }
-        if (it > 0) fetch(tb - span);
-        if (!AGG && p.act) {
+            if (p.mask) glr_rows<GlrByte, 1, K>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
+            if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give w = p = 0, c = 0
 #pragma unroll
-            for (int k = 0; k < K; ++k)
+                for (int k = 0; k < K; ++k) {
+                    const bool in = ts + k < w.t1, on = in && (!p.mask || rm[k].e[0] != 0);
 #pragma unroll
-                for (int i = 0; i < V; ++i) wc[k][i] = glr_tanh(wc[k][i]);
-        }
-        if (!AGG) {
+                    for (int i = 0; i < VG; ++i) rg[k].e[i] = on ? rg[k].e[i] : X::inf();
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        if (!AGG) rc[k].e[i] = on ? rc[k].e[i] : (S)0.f;
+                        rd[k].e[i] = in ? rd[k].e[i] : (S)0.f;
+                    }
+                }
+            }
+            if (!AGG) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) rs.e[i] = 0.f;
+                if (ts == 0) {
+                    if (p.h0) rs = glr_load<GlrF32, V>(reinterpret_cast<const char*>(p.h0 + w.b * NH), (uint32_t)(hoff * 4));
+                } else if (ts < w.t1) {                    // f32: out_{ts-1} is that state
+                    const float* at = p.dtype == GLR_F32 ? static_cast<const float*>(p.out) + ((long long)w.b * p.T + tb - 1) * NH : p.ckpt + ((long long)w.b * nck + tb / K - 1) * NH;
+                    rs = glr_load<GlrF32, V>(reinterpret_cast<const char*>(at), (uint32_t)(hoff * 4) + (uint32_t)(p.dtype == GLR_F32 ? w.seg * K : w.seg) * (uint32_t)(NH * 4));
+                }
+            }
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float c = wc[k][i], diff = c - h[i];
-                    q[k][i] *= -diff;
-                    h[i] = fmaf(ww[k][i], diff, h[i]);
-                    wc[k][i] = p.act ? ww[k][i] * fmaf(-c, c, 1.f) : ww[k][i];
+                    if (SHARED && i) { ww[k][i] = ww[k][0]; q[k][i] = q[k][0]; }
+                    else if (AGG) ww[k][i] = glr_w<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
+                    else glr_wp<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i), ww[k][i], q[k][i]);
+                    dd[k][i] = glr_up<X, V>(rd[k], i);
+                    if (!AGG) wc[k][i] = glr_up<X, V>(rc[k], i);
                 }
+            if (!AGG && p.act) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) wc[k][i] = glr_tanh<X::FINE>(wc[k][i]);
+            }
+            GLR_PHASE();
+            if (!AGG) {
+                float h[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) h[i] = rs.e[i];
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float c = wc[k][i], diff = c - h[i];
+                        q[k][i] *= -diff;
+                        h[i] = fmaf(ww[k][i], diff, h[i]);
+                        wc[k][i] = p.act ? ww[k][i] * fmaf(-c, c, 1.f) : ww[k][i];
+                        GLR_HERE(q[k][i]);
+                        GLR_HERE(wc[k][i]);
+                    }
+            }
         }
+        GLR_PHASE();
+        pg -= span * p.g_st * es;
+        pc -= span * p.c_st * es;
+        pd -= span * p.d_st * es;
+        pm -= span * p.m_st;
         float mu[V];
         if (SEG > 1 || AGG) {
             float A[V], Xl[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 A[i] = 1.f; Xl[i] = 0.f;
+            }
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
 #pragma unroll
                 for (int k = K - 1; k >= 0; --k) {
                     A[i] = fmaf(-ww[k][i], A[i], A[i]);
@@ -365,30 +561,22 @@ __global__ __launch_bounds__(GLR_THREADS) void glr_bwd_kernel(GlrP p) {
                     Xl[i] = fmaf(-ww[k][i], lam, lam);
                 }
             }
-            if (AGG) {
-                if (SEG == 1) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) { carry[i] = fmaf(A[i], carry[i], Xl[i]); prod[i] *= A[i]; }
-                } else {
-                    float none[V], dummy[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) none[i] = 0.f;
-                    glr_block_scan<V, CL, true>(lds[par], w.cl, w.seg, A, Xl, carry, dummy);
-                    par ^= 1;
-                    glr_block_scan<V, CL, true>(lds[par], w.cl, w.seg, A, none, prod, dummy);
-                    par ^= 1;
-                }
-                continue;
-            }
-            glr_block_scan<V, CL, true>(lds[par], w.cl, w.seg, A, Xl, carry, mu);
+            float EA[V], EX[V];
+            glr_scan_maps<V, CL, REV>(lds[par], w.cl, A, Xl, EA, EX);
+            if (CHAIN && w.chunk < p.S - 1 && w.active) glr_receive<V>(p.carry + ((long long)(w.chunk + 1) * p.B + w.b) * NH + hoff, carry);
+            glr_scan_carry<V, CL, REV, AGG>(lds[par], w.cl, EA, EX, carry, prod, mu);
+            if (CHAIN && w.chunk > 0 && w.active && w.seg == 0) glr_send<V>(p.carry + ((long long)w.chunk * p.B + w.b) * NH + hoff, carry);
             par ^= 1;
+            if (AGG) continue;
+            GLR_PHASE();
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) mu[i] = carry[i];
         }
+        if (live) {
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) {
-            const int t = ts + k;
+            const bool in = w.active && (full || ts + k < w.t1);
             float dc[V], dg[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -397,25 +585,28 @@ __global__ __launch_bounds__(GLR_THREADS) void glr_bwd_kernel(GlrP p) {
                 dg[i] = lam * q[k][i];
                 mu[i] = fmaf(-ww[k][i], lam, lam);
             }
-            const long long row = ((long long)w.b * p.T + t) * p.N + w.n;
-            if (w.active && t < w.t1) glr_store<X, V>(p.dcand, row * p.H + w.ch, dc);
+            if (in) glr_store<X, V>(pdc + k * rb, ldc, dc);
             if (!SHARED) {
-                if (w.active && t < w.t1) glr_store<X, VG>(p.dgate, row * p.G + w.gi, dg);
+                if (in) glr_store<X, VG>(pdg + k * gb, ldg, dg);
             } else {
                 float s = 0.f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) s += w.active ? dg[i] : 0.f;
-                for (int o = p.L >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-                if (w.active && w.gl == 0 && t < w.t1) {
-                    if (p.parts == 1) glr_store<X, 1>(p.dgate, row * p.G + w.gi, &s);
-                    else p.part[(row * p.G + w.gi) * p.parts + w.part] = s;
+                s = glr_lane_sum(s, p.L);
+                if (in && w.gl == 0) {
+                    if (p.parts == 1) glr_store<X, 1>(pdg + k * gb, ldg, &s);
+                    else p.part[((((long long)w.b * p.T + ts + k) * p.N + w.n) * p.G + w.gi) * p.parts + w.part] = s;
                 }
             }
         }
+        }
+        pdc -= span * rb;
+        pdg -= span * gb;
         if (SEG == 1) {
 #pragma unroll
             for (int i = 0; i < V; ++i) carry[i] = mu[i];
         }
+        if (CHAIN) break;
     }
     if (!w.active || w.seg != 0) return;
     if (AGG) {
@@ -435,7 +626,7 @@ __global__ void glr_parts_kernel(const float* __restrict__ part, int parts, long
     if (i >= n) return;
     float s = 0.f;
     for (int j = 0; j < parts; ++j) s += part[i * parts + j];
-    glr_store<X, 1>(dgate, i, &s);
+    glr_store<X, 1>(static_cast<char*>(dgate) + i * sizeof(typename X::S), 0, &s);
 }
 
 }  // namespace mcrn

@@ -20,7 +20,7 @@ struct GlrP {
     const float* h0;                        // (B,N,H) or NULL = zeros
     void* out;                              // (B,T,N,H) contiguous, NULL = not wanted (forward only)
     float* last;                            // (B,N,H), may be h0 itself (forward only)
-    float* ckpt;                            // (B, ceil(T/GLR_K) - 1, N, H) states before steps GLR_K, 2 GLR_K, ..; NULL = not wanted.
+    float* ckpt;                            // (B, ceil(T/K) - 1, N, H) states before steps K, 2 K, .. (K = glr_steps(T)); NULL = not wanted.
                                             // f32: never written, the backward reads the same states from `out`
     // backward
     const void* dout;                       // (B,T,N,H) or NULL = zeros
@@ -30,16 +30,21 @@ struct GlrP {
     float* dstate;                          // (B,N,H) or NULL = not wanted
     // plan (glr_plan)
     int one;                                // not 0: plan for one channel a thread, whatever the alignment
-    int V, CL, S, L, parts;                 // channels a thread, channel lanes a block, chunks of the time axis,
+    int V, K, CL, S, L, parts;              // channels and steps a thread, channel lanes a block, chunks of the time axis,
     int chunk, first;                       // lanes and parts of a shared gate's channels; steps a chunk, first chunk of the launch
     long long nq, tiles;                    // channel vectors of a batch entry, blocks that cover them
-    float *agg, *part;                      // workspace: chunk aggregates, partial gate gradients
+    bool chain;                             // a chunk is one tile and takes its state from the block before it
+    float *agg, *part;                      // workspace: chunk aggregates, partial gate gradients,
+    unsigned *ticket, *carry;               // chunks taken of each tile, states behind the chunks (chain)
 };
 
-constexpr int GLR_K = 8;                    // steps a thread holds in registers = distance of the checkpoints
+constexpr int GLR_K = 8;                    // steps a thread holds in registers, at most = distance of the checkpoints
+constexpr int GLR_TILE = 128;               // steps of a block's tile, at most
+int glr_steps(int T);
 
 bool glr_plan(GlrP& p, bool backward);      // fills the plan; false: too large
 size_t glr_ws_bytes(const GlrP& p, bool backward);
+void glr_place(GlrP& p, void* ws);          // the plan's parts of the workspace
 hipError_t launch_glr_forward(const GlrP& p, hipStream_t st, int* launches);
 hipError_t launch_glr_backward(const GlrP& p, hipStream_t st, int* launches);
 

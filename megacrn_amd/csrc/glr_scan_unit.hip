@@ -5,6 +5,9 @@ namespace mcrn {
 
 static long long up_div(long long a, long long b) { return (a + b - 1) / b; }
 
+// Steps a thread holds.  T alone decides, so that a backward finds the checkpoints of its forward.
+int glr_steps(int T) { return T <= 1 ? 1 : T <= 4 || (T > 8 && T <= 12) ? 4 : GLR_K; }
+
 bool glr_plan(GlrP& p, bool backward) {
     const size_t size = p.dtype == GLR_F32 ? 4 : 2;
     const int D = p.H / p.G;
@@ -37,66 +40,87 @@ bool glr_plan(GlrP& p, bool backward) {
     };
     p.S = 1;
     p.first = 0;
+    p.chain = false;
     p.chunk = p.T > 0 ? p.T : 1;
+    p.K = glr_steps(p.T);
     long long blocks = cover(256);
-    if (p.T > GLR_K && blocks < 512) blocks = cover(64);
-    if (p.T > 4 * GLR_K && blocks < 512) {
-        blocks = cover(16);
+    if (p.T > GLR_K && p.K == GLR_K && blocks < 512) {
         const int span = GLR_THREADS / 16 * GLR_K;
-        long long S = blocks < 256 ? up_div(512, blocks) : 1;
-        S = S > 64 ? 64 : S;
-        const long long most = up_div(p.T, span);
-        S = S > most ? most : S;
-        if (S > 1) {
+        if (p.T <= GLR_THREADS / 64 * GLR_K) {
+            cover(64);                                    // one tile
+        } else if ((blocks = cover(16)) >= 256 && p.T > span) {
+            p.chain = true;
+            p.chunk = span;
+            p.S = (int)up_div(p.T, span);
+        } else if (p.T > span) {
+            long long S = up_div(1024, blocks);
+            S = S > 256 ? 256 : S;
+            const long long most = up_div(p.T, span);
+            S = S > most ? most : S;
             p.chunk = (int)(up_div(up_div(p.T, S), span) * span);
             p.S = (int)up_div(p.T, p.chunk);
         }
     }
-    return p.tiles * p.B * p.S < (1ll << 31);
+    return p.tiles * p.CL < (1ll << 31) && (long long)p.N * p.G * p.parts < (1ll << 31) && p.tiles * p.B * p.S < (1ll << 31);
 }
 
+// [tickets | states] or [chunk aggregates], then the partial gate gradients; each part 256-byte aligned
+static size_t chain_words(const GlrP& p) { return (size_t)(p.tiles * p.B) + (size_t)p.S * p.B * p.N * p.H; }
+static size_t head_bytes(const GlrP& p) {
+    const size_t n = p.chain ? chain_words(p) * 4 : p.S > 1 ? (size_t)p.S * p.B * 2 * p.N * p.H * 4 : 0;
+    return (n + 255) / 256 * 256;
+}
 size_t glr_ws_bytes(const GlrP& p, bool backward) {
-    const size_t agg = p.S > 1 ? (size_t)p.S * p.B * 2 * p.N * p.H * 4 : 0;
-    const size_t part = backward && p.parts > 1 ? (size_t)p.B * p.T * p.N * p.G * p.parts * 4 : 0;
-    return (agg + 255) / 256 * 256 + part;
+    return head_bytes(p) + (backward && p.parts > 1 ? (size_t)p.B * p.T * p.N * p.G * p.parts * 4 : 0);
+}
+void glr_place(GlrP& p, void* ws) {
+    p.agg = (float*)ws;
+    p.ticket = (unsigned*)ws;
+    p.carry = p.ticket + p.tiles * p.B;
+    p.part = (float*)((char*)ws + head_bytes(p));
 }
 
-template <class X, int V, int CL, bool SHARED> static hipError_t run(const GlrP& p0, bool backward, hipStream_t st, int* launches) {
+template <class X, int V, int K, int CL, bool SHARED> static hipError_t run(const GlrP& p0, bool backward, hipStream_t st, int* launches) {
     GlrP p = p0;
     const unsigned one = (unsigned)(p.tiles * p.B);
+    const dim3 block(GLR_THREADS);
     (void)hipGetLastError();
-    if (CL == 16 && p.S > 1) {                            // maps of the chunks that others start from
-        if (backward) {
-            p.first = 1;
-            hipLaunchKernelGGL((glr_bwd_kernel<X, V, 16, SHARED, true>), dim3(one * (p.S - 1)), dim3(GLR_THREADS), 0, st, p);
-            p.first = 0;
-        } else {
-            hipLaunchKernelGGL((glr_fwd_kernel<X, V, 16, SHARED, true>), dim3(one * (p.S - 1)), dim3(GLR_THREADS), 0, st, p);
-        }
+    if (CL == 16 && p.chain) {
+        const long long words = (long long)chain_words(p);
+        hipLaunchKernelGGL(glr_clear_kernel, dim3((unsigned)up_div(words, 256)), dim3(256), 0, st, p.ticket, p.tiles * p.B, words);
+        if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, GLR_K, 16, SHARED, GLR_CHAIN>), dim3(one * p.S), block, 0, st, p);
+        else hipLaunchKernelGGL((glr_fwd_kernel<X, V, GLR_K, 16, SHARED, GLR_CHAIN>), dim3(one * p.S), block, 0, st, p);
         ++*launches;
-    }
-    if (backward) {
-        hipLaunchKernelGGL((glr_bwd_kernel<X, V, CL, SHARED, false>), dim3(one * p.S), dim3(GLR_THREADS), 0, st, p);
-        if (p.parts > 1) {
-            const long long n = (long long)p.B * p.T * p.N * p.G;
-            hipLaunchKernelGGL((glr_parts_kernel<X>), dim3((unsigned)up_div(n, 256)), dim3(256), 0, st, p.part, p.parts, n, p.dgate);
+    } else {
+        if (CL == 16 && p.S > 1) {                        // maps of the chunks that others start from
+            p.first = backward ? 1 : 0;
+            if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, GLR_K, 16, SHARED, GLR_AGG>), dim3(one * (p.S - 1)), block, 0, st, p);
+            else hipLaunchKernelGGL((glr_fwd_kernel<X, V, GLR_K, 16, SHARED, GLR_AGG>), dim3(one * (p.S - 1)), block, 0, st, p);
+            p.first = 0;
             ++*launches;
         }
-    } else {
-        hipLaunchKernelGGL((glr_fwd_kernel<X, V, CL, SHARED, false>), dim3(one * p.S), dim3(GLR_THREADS), 0, st, p);
+        if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, K, CL, SHARED, GLR_WALK>), dim3(one * p.S), block, 0, st, p);
+        else hipLaunchKernelGGL((glr_fwd_kernel<X, V, K, CL, SHARED, GLR_WALK>), dim3(one * p.S), block, 0, st, p);
     }
     ++*launches;
+    if (backward && p.parts > 1) {
+        const long long n = (long long)p.B * p.T * p.N * p.G;
+        hipLaunchKernelGGL((glr_parts_kernel<X>), dim3((unsigned)up_div(n, 256)), dim3(256), 0, st, p.part, p.parts, n, p.dgate);
+        ++*launches;
+    }
     return hipGetLastError();
 }
 
-template <class X, int V> static hipError_t run_v(const GlrP& p, bool backward, hipStream_t st, int* launches) {
-    const bool shared = p.G != p.H;
-    if (p.CL == 256) return shared ? run<X, V, 256, true>(p, backward, st, launches) : run<X, V, 256, false>(p, backward, st, launches);
-    if (p.CL == 64) return shared ? run<X, V, 64, true>(p, backward, st, launches) : run<X, V, 64, false>(p, backward, st, launches);
-    return shared ? run<X, V, 16, true>(p, backward, st, launches) : run<X, V, 16, false>(p, backward, st, launches);
+template <class X, int V, bool SHARED> static hipError_t run_v(const GlrP& p, bool backward, hipStream_t st, int* launches) {
+    if (p.K == 1) return run<X, V, 1, 256, SHARED>(p, backward, st, launches);
+    if (p.K == 4) return run<X, V, 4, 256, SHARED>(p, backward, st, launches);
+    if (p.CL == 256) return run<X, V, GLR_K, 256, SHARED>(p, backward, st, launches);
+    if (p.CL == 64) return run<X, V, GLR_K, 64, SHARED>(p, backward, st, launches);
+    return run<X, V, GLR_K, 16, SHARED>(p, backward, st, launches);
 }
 template <class X> static hipError_t run_x(const GlrP& p, bool backward, hipStream_t st, int* launches) {
-    return p.V == 4 ? run_v<X, 4>(p, backward, st, launches) : run_v<X, 1>(p, backward, st, launches);
+    if (p.G != p.H) return p.V == 4 ? run_v<X, 4, true>(p, backward, st, launches) : run_v<X, 1, true>(p, backward, st, launches);
+    return p.V == 4 ? run_v<X, 4, false>(p, backward, st, launches) : run_v<X, 1, false>(p, backward, st, launches);
 }
 static hipError_t launch(const GlrP& p, bool backward, hipStream_t st, int* launches) {
     if (p.dtype == GLR_F32) return run_x<GlrF32>(p, backward, st, launches);

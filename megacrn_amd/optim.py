@@ -80,7 +80,7 @@ class AdamW:
             for p, o in zip(self.params, self.offsets):
                 self.master[o:o + p.numel()].copy_(p.detach().reshape(-1))
         nb = lib.mcrn_adamw_workspace_bytes(C.byref(self._cfg), self._numel)
-        self._ws = torch.zeros(nb, dtype=torch.uint8, device=dev)
+        self._ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         self.total_norm = torch.zeros((), device=dev)
         self._lr, self._wd, self._steps = (C.c_double * k)(), (C.c_double * k)(), (C.c_int * k)()
         self._dev = self._seen = None
