@@ -65,20 +65,26 @@ template <class X, int V> __device__ __forceinline__ void glr_store(char* base, 
     for (int i = 0; i < V; ++i) r.e[i] = X::down(v[i]);
     *reinterpret_cast<GlrVec<X, V>*>(base + off) = r;
 }
-// K rows of a thread, from row seg * K of the tile on.  What lies behind the tile's last row `end` reads that one instead: with
-// `most` = the lane's bytes to its last row (all ones in a whole tile) that is one minimum a row, and no second path for the loads.
-template <class X, int V, int K>
+// K rows of a thread, from row seg * K of the tile on.  What lies behind the tile's last row `end` reads that one instead: one minimum a
+// row.  ONCE (no loop around it): whole tiles go without, by scalar bases (in a loop the second path costs registers, and spills).
+template <class X, int V, int K, bool ONCE>
 __device__ __forceinline__ void glr_rows(GlrVec<X, V>* r, const char* base, uint32_t lane, uint32_t st, int seg, bool full, int end) {
-    uint32_t off = lane + (uint32_t)(seg * K) * st, most = 0xffffffffu;
-    if (!full) {
-        const int at = min(seg * K, end);
-        off = lane + (uint32_t)at * st;
-        most = (uint32_t)(end - at) * st;
-    }
+    if (ONCE && full) {
+        const uint32_t off = lane + (uint32_t)(seg * K) * st;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const uint32_t o = (uint32_t)k * st;
-        r[k] = glr_load<X, V>(base, off + (o < most ? o : most));
+        for (int k = 0; k < K; ++k) r[k] = glr_load<X, V>(base + (uint64_t)k * st, off);
+    } else {
+        uint32_t off = lane + (uint32_t)(seg * K) * st, most = 0xffffffffu;
+        if (!full) {
+            const int at = min(seg * K, end);
+            off = lane + (uint32_t)at * st;
+            most = (uint32_t)(end - at) * st;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const uint32_t o = (uint32_t)k * st;
+            r[k] = glr_load<X, V>(base, off + (o < most ? o : most));
+        }
     }
 }
 struct GlrByte {
@@ -103,11 +109,14 @@ template <bool FINE> __device__ __forceinline__ void glr_wp(float g, float& w, f
     w = g >= 0.f ? s : r;
     p = s * r;
 }
-// 1 - 2 / (1 + e^2u), off by 2 u absolutely; below a quarter, where that shows, Taylor's series (next term below u / 4 of the value)
+// 1 - 2 / (1 + e^2u): off by 3 units of 2^-24 whatever u is, which shows relatively near 0.  FINE: Taylor's series below 1/4 (its next term is
+// 2^-26 of the value).  16-bit types: u itself below 2^-8 (off by u^2 / 3 < 2^-17 of the value, the quotient by 2^-14 above: their own steps
+// are 2^-12 and 2^-9) - 5 instructions of 39 fewer in a forward that they bound.
 template <bool FINE> __device__ __forceinline__ float glr_tanh(float u) {
     const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + glr_exp<false>(2.f * u)), 1.f);
+    if (!FINE) return fabsf(u) < 0.00390625f ? u : far;
     const float q = u * u;
-    float s = FINE ? fmaf(q, 62.f / 2835.f, -17.f / 315.f) : -17.f / 315.f;
+    float s = fmaf(q, 62.f / 2835.f, -17.f / 315.f);
     s = fmaf(q, s, 2.f / 15.f);
     s = fmaf(q, s, -1.f / 3.f);
     return fabsf(u) < 0.25f ? fmaf(u * q, s, u) : far;
@@ -128,19 +137,11 @@ template <int V, int CL, bool SHARED, bool CHAIN, bool REV> __device__ __forcein
     const unsigned tile = blk % (unsigned)p.tiles;
     blk /= (unsigned)p.tiles;
     w.b = (int)(blk % (unsigned)p.B);
-    if (CHAIN) {
-        __shared__ int taken;
-        if (threadIdx.x == 0) taken = (int)atomicAdd(p.ticket + (tile + (unsigned)w.b * (unsigned)p.tiles), 1u);
-        __syncthreads();
-        w.chunk = __builtin_amdgcn_readfirstlane(taken);
-        if (REV) w.chunk = p.S - 1 - w.chunk;
-    } else {
-        w.chunk = (int)(blk / (unsigned)p.B) + p.first;
-    }
+    __shared__ int taken;
+    int mine = 0;
+    if (CHAIN && threadIdx.x == 0) mine = (int)atomicAdd(p.ticket + (tile + (unsigned)w.b * (unsigned)p.tiles), 1u);
     w.cl = (int)threadIdx.x % CL;
     w.seg = (int)threadIdx.x / CL;
-    w.t0 = w.chunk * p.chunk;
-    w.t1 = min(p.T, w.t0 + p.chunk);
     if (SHARED) {              // L lanes a (gate, part): channels behind the gate's last stay idle
         const unsigned unit = tile * (unsigned)(CL / p.L) + w.cl / p.L;
         const int D = p.H / p.G;
@@ -161,6 +162,16 @@ template <int V, int CL, bool SHARED, bool CHAIN, bool REV> __device__ __forcein
         w.gl = 0;
         w.part = 0;
     }
+    if (CHAIN) {
+        if (threadIdx.x == 0) taken = mine;
+        __syncthreads();
+        w.chunk = __builtin_amdgcn_readfirstlane(taken);
+        if (REV) w.chunk = p.S - 1 - w.chunk;
+    } else {
+        w.chunk = (int)(blk / (unsigned)p.B) + p.first;
+    }
+    w.t0 = w.chunk * p.chunk;
+    w.t1 = min(p.T, w.t0 + p.chunk);
     return w;
 }
 
@@ -319,9 +330,9 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
             GlrVec<X, V> rc[K];
             GlrVec<GlrByte, 1> rm[K];
             const int end = w.t1 - 1 - tb;
-            glr_rows<X, VG, K>(rg, pg, lg, (uint32_t)(p.g_st * es), w.seg, full, end);
-            glr_rows<X, V, K>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
-            if (p.mask) glr_rows<GlrByte, 1, K>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
+            glr_rows<X, VG, K, CHAIN>(rg, pg, lg, (uint32_t)(p.g_st * es), w.seg, full, end);
+            glr_rows<X, V, K, CHAIN>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
+            if (p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
             if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give w = 0, c = 0
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
@@ -361,9 +372,11 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
 #pragma unroll
                 for (int i = 0; i < V; ++i)
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
+                for (int k = 0; k < K; ++k) {              // from here on ww, cc hold the maps up to each step
                     A[i] = fmaf(-ww[k][i], A[i], A[i]);
                     Xl[i] = fmaf(ww[k][i], cc[k][i] - Xl[i], Xl[i]);
+                    ww[k][i] = A[i];
+                    cc[k][i] = Xl[i];
                 }
             }
             float EA[V], EX[V];
@@ -378,18 +391,22 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
 #pragma unroll
             for (int i = 0; i < V; ++i) h[i] = carry[i];
         }
+        float o[V];
         if (live) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) h[i] = fmaf(ww[k][i], cc[k][i] - h[i], h[i]);
-            if (w.active && p.out && (full || ts + k < w.t1)) glr_store<X, V>(po + k * rb, lo, h);
+            for (int i = 0; i < V; ++i) {
+                if (SEG > 1) o[i] = fmaf(ww[k][i], h[i], cc[k][i]);
+                else o[i] = h[i] = fmaf(ww[k][i], cc[k][i] - h[i], h[i]);
+            }
+            if (w.active && p.out && (full || ts + k < w.t1)) glr_store<X, V>(po + k * rb, lo, o);
         }
         }
         po += span * rb;
         if (p.ckpt && w.active && ts + K < p.T) {          // the state before step ts + K
             const long long nck = (p.T - 1) / K;
-            glr_store<GlrF32, V>(reinterpret_cast<char*>(p.ckpt + ((long long)w.b * nck + tb / K) * NH), (uint32_t)((w.seg * NH + hoff) * 4), h);
+            glr_store<GlrF32, V>(reinterpret_cast<char*>(p.ckpt + ((long long)w.b * nck + tb / K) * NH), (uint32_t)((w.seg * NH + hoff) * 4), o);
         }
         if (SEG == 1) {
 #pragma unroll
@@ -471,17 +488,17 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
             GlrVec<GlrF32, V> rs;                          // the state before the segment's first step
             GlrVec<GlrByte, 1> rm[K];
             const int end = w.t1 - 1 - tb;
-            glr_rows<X, VG, K>(rg, pg, lg, (uint32_t)(p.g_st * es), w.seg, full, end);
-            if (!AGG) glr_rows<X, V, K>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
+            glr_rows<X, VG, K, CHAIN>(rg, pg, lg, (uint32_t)(p.g_st * es), w.seg, full, end);
+            if (!AGG) glr_rows<X, V, K, CHAIN>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
             if (p.dout) {
-                glr_rows<X, V, K>(rd, pd, ld, (uint32_t)(p.d_st * es), w.seg, full, end);
+                glr_rows<X, V, K, CHAIN>(rd, pd, ld, (uint32_t)(p.d_st * es), w.seg, full, end);
             } else {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
 #pragma unroll
                     for (int i = 0; i < V; ++i) rd[k].e[i] = (S)0.f;
             }
-            if (p.mask) glr_rows<GlrByte, 1, K>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
+            if (p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
             if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give w = p = 0, c = 0
 #pragma unroll
                 for (int k = 0; k < K; ++k) {

@@ -46,9 +46,11 @@ bool glr_plan(GlrP& p, bool backward) {
     long long blocks = cover(256);
     if (p.T > GLR_K && p.K == GLR_K && blocks < 512) {
         const int span = GLR_THREADS / 16 * GLR_K;
-        if (p.T <= GLR_THREADS / 64 * GLR_K) {
-            cover(64);                                    // one tile
-        } else if ((blocks = cover(16)) >= 256 && p.T > span) {
+        const int quarter = GLR_THREADS / 64 * GLR_K;     // steps of a wave of the 16-lane form, of a tile of the 64-lane form
+        const bool loose = up_div(p.T, quarter) < 3 * up_div(p.T, span);      // over a quarter of the 16-lane form's waves would idle
+        if (p.T <= quarter || (loose && cover(64) >= 256)) {
+            cover(64);
+        } else if ((blocks = cover(16)) >= 64 && p.T > span) {
             p.chain = true;
             p.chunk = span;
             p.S = (int)up_div(p.T, span);

@@ -83,7 +83,8 @@ def test_step_refusals(over, kind):
 
 
 def test_c_sizes():
-    """Checkpoints: one state in fp32 before every 8th step but the first, 16-bit types only; a workspace for long sequences with few channels."""
+    """Checkpoints: one state in fp32 before every 8th step (every 4th of up to 4 and of 9 to 12 steps) but the first, 16-bit types only; a
+    workspace for long sequences with few channels."""
     import ctypes as C
     from megacrn_amd._lib import lib
 
@@ -100,7 +101,8 @@ def test_c_sizes():
         f.restype, f.argtypes = C.c_size_t, [C.POINTER(Glr), C.c_int]
         return f(C.byref(Glr((C.c_int * 8)(*a, 1, 0))), backward)
     assert ck(2, 8, 3, 4, 4, 1) == 0
-    assert ck(2, 9, 3, 4, 4, 1) == 24
+    assert ck(2, 9, 3, 4, 4, 1) == 48
+    assert ck(2, 13, 3, 4, 4, 1) == 24
     assert ck(2, 17, 3, 4, 4, 2) == 48
     assert ck(2, 17, 3, 4, 4, 0) == 0
     assert ck(2, 0, 3, 4, 4, 1) == 0
@@ -142,7 +144,7 @@ def _close(got, want, bound, what):
 def _against_oracle(gate, cand, st, keep, dout, dlast, act, dt, lay=lambda t: t.cuda(), want_grad=True):
     import megacrn_amd
     m = None if keep is None else keep.numpy()
-    out, last, eh, cache = O.glr_fwd(_np(gate), _np(cand), _np(st), m, act)
+    out, last, eh, cache = O.glr_fwd(_np(gate), _np(cand), _np(st), m, act, dt)
     leaves = [lay(t).detach().requires_grad_() if t is not None else None for t in (gate, cand, st)]
     got, glast = megacrn_amd.gated_linear_recurrence(leaves[0], leaves[1], leaves[2], None if keep is None else keep.cuda(), activation=act)
     _close(got, out, eh + O.half_step(out, dt), "out")
@@ -289,7 +291,7 @@ def test_steps_are_the_sequence(dt, G):
     for t in range(13):
         o = megacrn_amd.gated_linear_recurrence_step(gate[:, t], cand[:, t], now, keep[:, t])
         assert o.dtype == TORCH[dt]
-        want = O.glr_fwd(_np(gate[:, :t + 1].cpu()), _np(cand[:, :t + 1].cpu()), _np(st.cpu()), keep[:, :t + 1].cpu().numpy())
+        want = O.glr_fwd(_np(gate[:, :t + 1].cpu()), _np(cand[:, :t + 1].cpu()), _np(st.cpu()), keep[:, :t + 1].cpu().numpy(), dt=dt)
         _close(o, want[0][:, -1], want[2][:, -1] + O.half_step(want[0][:, -1], dt), f"step {t}")
     _close(now, want[1], want[2][:, -1] + O.half_step(want[1], "f32"), "state")
     _close(last, want[1], want[2][:, -1] + O.half_step(want[1], "f32"), "last")
