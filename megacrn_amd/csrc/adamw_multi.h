@@ -30,38 +30,44 @@ __host__ __device__ __forceinline__ unsigned adamw_key_of(unsigned seed, int id,
     return adamw_mix(seed + 0x9E3779B9u * (unsigned)(id + 1) + adamw_mix(step));
 }
 
+typedef float AdamwV4 __attribute__((ext_vector_type(4)));
+typedef __bf16 AdamwH4 __attribute__((ext_vector_type(4)));
+// NT: what is streamed once through a step that is larger than the caches (launch_adamw) leaves them alone
+template <bool NT, class V> __device__ __forceinline__ V adamw_ld(const void* p) {
+    return NT ? __builtin_nontemporal_load(static_cast<const V*>(p)) : *static_cast<const V*>(p);
+}
+template <bool NT, class V> __device__ __forceinline__ void adamw_st(void* p, V v) {
+    if (NT) __builtin_nontemporal_store(v, static_cast<V*>(p));
+    else *static_cast<V*>(p) = v;
+}
 struct AdamwF32 {
+    typedef float S;
     static constexpr bool WIDE = true;
-    static __device__ __forceinline__ void load4(const void* p, long long i, float* v) {
-        const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    template <bool NT> static __device__ __forceinline__ void load4(const void* p, long long i, float* v) {
+        const AdamwV4 r = adamw_ld<NT, AdamwV4>(static_cast<const float*>(p) + i);
         v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
     }
-    static __device__ __forceinline__ float load1(const void* p, long long i) { return static_cast<const float*>(p)[i]; }
-    static __device__ __forceinline__ void store4(void* p, long long i, const float* v) {
-        *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    template <bool NT> static __device__ __forceinline__ void store4(void* p, long long i, const float* v) {
+        const AdamwV4 r = {v[0], v[1], v[2], v[3]};
+        adamw_st<NT>(static_cast<float*>(p) + i, r);
     }
-    static __device__ __forceinline__ void store1(void* p, long long i, float v) { static_cast<float*>(p)[i] = v; }
 };
 struct AdamwBf16 {
+    typedef __bf16 S;
     static constexpr bool WIDE = false;
-    static __device__ __forceinline__ uint32_t down(float f) {            // to the nearest, ties to even; NaN stays NaN
-        const uint32_t u = __float_as_uint(f);
-        if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
-        return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-    }
-    static __device__ __forceinline__ void load4(const void* p, long long i, float* v) {
-        const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    template <bool NT> static __device__ __forceinline__ void load4(const void* p, long long i, float* v) {
+        typedef uint32_t U2 __attribute__((ext_vector_type(2)));
+        const U2 r = adamw_ld<NT, U2>(static_cast<const uint16_t*>(p) + i);
         v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
         v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
     }
-    static __device__ __forceinline__ float load1(const void* p, long long i) {
-        return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+    template <bool NT> static __device__ __forceinline__ void store4(void* p, long long i, const float* v) {
+        const AdamwH4 r = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};       // to the nearest, ties to even, by the hardware
+        adamw_st<NT>(static_cast<__bf16*>(p) + i, r);
     }
-    static __device__ __forceinline__ void store4(void* p, long long i, const float* v) {
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(down(v[0]) | (down(v[1]) << 16), down(v[2]) | (down(v[3]) << 16));
-    }
-    static __device__ __forceinline__ void store1(void* p, long long i, float v) { static_cast<uint16_t*>(p)[i] = (uint16_t)down(v); }
 };
+template <class X> __device__ __forceinline__ float adamw_load1(const void* p, long long i) { return (float)static_cast<const typename X::S*>(p)[i]; }
+template <class X> __device__ __forceinline__ void adamw_store1(void* p, long long i, float v) { static_cast<typename X::S*>(p)[i] = (typename X::S)v; }
 
 // the tensor that this block works on: the last one whose first block is not behind it (one compare a lane)
 template <class P> __device__ __forceinline__ int adamw_tensor(const P& p) {
@@ -85,22 +91,40 @@ __device__ __forceinline__ unsigned adamw_finite_bits(float x) {
     const unsigned u = __float_as_uint(x) & 0x7fffffffu;
     return u < 0x7f800000u ? u : 0u;
 }
-template <bool SECOND> __device__ __forceinline__ float adamw_decode(unsigned code, int scale) {
-    // the code's exponent and mantissa in a float's places, then the difference of the biases and the scale as one power of two
-    if (SECOND) {
-        const float v = __builtin_amdgcn_ldexpf(__uint_as_float(code << 20), scale - 15);
-        return code == 0xffu ? __uint_as_float(0x7fc00000u) : v;
-    }
-    const float v = __builtin_amdgcn_ldexpf(__uint_as_float(((code & 0x7fu) << 20) | ((code & 0x80u) << 24)), scale - 7);
-    return (code & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : v;
+// four codes -> values.  m: the hardware's own format (e4m3), times the scale.  v: the code's exponent and mantissa in a float's places, then
+// the difference of the biases and the scale as one power of two (what is below the format's normal numbers is so below the float's).
+__device__ __forceinline__ void adamw_decode_m(unsigned codes, int scale, float* m) {
+    const float s = __uint_as_float((unsigned)scale << 23);
+    m[0] = __builtin_amdgcn_cvt_f32_fp8(codes, 0) * s;
+    m[1] = __builtin_amdgcn_cvt_f32_fp8(codes, 1) * s;
+    m[2] = __builtin_amdgcn_cvt_f32_fp8(codes, 2) * s;
+    m[3] = __builtin_amdgcn_cvt_f32_fp8(codes, 3) * s;
 }
-template <bool SECOND> __device__ __forceinline__ unsigned adamw_encode(float x, int scale, unsigned bits16) {
-    const float t = __builtin_amdgcn_ldexpf(fabsf(x), (SECOND ? 15 : 7) - scale);
-    unsigned code = (__float_as_uint(t) + (bits16 << 4)) >> 20;
-    if (SECOND) code = x > 0.f && code == 0u ? 1u : code;
-    const bool finite = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
-    code = finite ? code : (SECOND ? 0xffu : 0x7fu);
-    return SECOND ? code : code | ((__float_as_uint(x) >> 24) & 0x80u);
+__device__ __forceinline__ void adamw_decode_v(unsigned codes, int scale, float* v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const unsigned c = (codes >> (8 * k)) & 0xffu;
+        v[k] = c == 0xffu ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(__uint_as_float(c << 20), scale - 15);
+    }
+}
+// value -> code.  FINITE: the caller has seen that every value of the wave is
+template <bool FINITE> __device__ __forceinline__ unsigned adamw_encode_m(float x, int scale, unsigned bits) {
+    const float t = __builtin_amdgcn_ldexpf(fabsf(x), 7 - scale);
+    unsigned code = (__float_as_uint(t) + ((bits & 0xffffu) << 4)) >> 20;
+    if (!FINITE) code = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u ? code : 0x7fu;
+    return code | ((__float_as_uint(x) >> 24) & 0x80u);
+}
+template <bool FINITE> __device__ __forceinline__ unsigned adamw_encode_v(float x, int scale, unsigned bits) {
+    const float t = __builtin_amdgcn_ldexpf(x, 15 - scale);
+    const unsigned least = __float_as_uint(x) < 1u ? __float_as_uint(x) : 1u;      // what is above 0 stays above 0
+    unsigned code = (__float_as_uint(t) + ((bits >> 12) & 0xffff0u)) >> 20;
+    code = code > least ? code : least;
+    if (!FINITE) code = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u ? code : 0xffu;
+    return code;
+}
+__device__ __forceinline__ unsigned adamw_max4(unsigned a, unsigned b, unsigned c, unsigned d) {
+    const unsigned x = a > b ? a : b, y = c > d ? c : d;
+    return x > y ? x : y;
 }
 
 __device__ __forceinline__ double adamw_block_sum(double s, double* sh) {      // in every thread; sh: one double a wave
@@ -111,107 +135,149 @@ __device__ __forceinline__ double adamw_block_sum(double s, double* sh) {      /
     return (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-// What the gradients are multiplied by: grad_scale, and max_norm / norm where the norm over all tensors is larger.  Every block adds the
-// partial sums (a few hundred, from L2) in the same order: no further launch, no counter, the same number everywhere.
-__device__ __forceinline__ float adamw_factor(const AdamwP& p, double* sh) {
+// What the gradients are multiplied by: grad_scale, and max_norm / norm where the norm over all tensors is larger, from the partial sums in
+// their order (the same number whoever adds them).
+__device__ __forceinline__ float adamw_factor(const double* part, int parts, float grad_scale, float max_norm, float* norm_out, double* sh) {
     double s = 0.0;
-    for (int j = threadIdx.x; j < p.parts; j += 256) s += p.part[j];
+    for (int j = threadIdx.x; j < parts; j += 256) s += part[j];
     s = adamw_block_sum(s, sh);
-    const float norm = (float)(sqrt(s) * (double)p.grad_scale);
-    if (p.norm && blockIdx.x == 0 && threadIdx.x == 0) p.norm[0] = norm;
-    const float c = p.max_norm / (norm + 1e-6f);
-    return p.grad_scale * (c > 1.f ? 1.f : c);                // a NaN norm makes every gradient NaN
+    const float norm = (float)(sqrt(s) * (double)grad_scale);
+    if (norm_out && threadIdx.x == 0) norm_out[0] = norm;
+    const float c = max_norm / (norm + 1e-6f);
+    return grad_scale * (c > 1.f ? 1.f : c);                  // a NaN norm makes every gradient NaN
+}
+// One block, for steps of many blocks: 473 us with 129 K blocks that each add 523 sums (132 M parameters in bf16, 8-bit moments), 406 so.
+// Small steps let every block add them, which saves the launch (9 us of work in all).
+__global__ __launch_bounds__(256) void adamw_factor_kernel(const double* part, int parts, float grad_scale, float max_norm, float* norm, float* factor) {
+    __shared__ double sh[4];
+    const float f = adamw_factor(part, parts, grad_scale, max_norm, norm, sh);
+    if (threadIdx.x == 0) factor[0] = f;
 }
 
-// One block: `per` runs of 1024 elements of one tensor, four neighbours a thread.
-template <class X, int BITS>
-__global__ __launch_bounds__(256) void adamw_kernel(AdamwP p) {
-    const int ti = adamw_tensor(p);
-    if (ti < 0) return;
-    const AdamwT t = p.t[ti];
-    float step_size = t.step_size, inv_bc2 = t.inv_bc2, decay = t.decay;
-    unsigned key = t.key;
-    if (p.dyn) { const AdamwDyn d = p.dyn[t.id]; step_size = d.step_size; inv_bc2 = d.inv_bc2; decay = d.decay; key = d.key; }
-    __shared__ double sh[4];
-    const float factor = p.parts ? adamw_factor(p, sh) : p.grad_scale;
-    const long long first = (long long)(blockIdx.x - t.blk0) * p.per * 1024;
-    for (int r = 0; r < p.per; ++r) {
-        const long long i = first + r * 1024 + threadIdx.x * 4;
-        if (first + r * 1024 >= t.n) return;
-        const bool whole = i + 4 <= t.n, some = i < t.n;
-        const bool vec = whole && (t.flags & ADAMW_VEC);
-        const long long a = t.off + i;
-        float g[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (some) {                       // the arenas reach to the end of the block of 64: four of their elements at a time
-            if (vec) X::load4(t.g, i, g);
-            else for (int k = 0; k < 4; ++k) if (i + k < t.n) g[k] = X::load1(t.g, i + k);
-            if (!X::WIDE) AdamwF32::load4(p.master, a, w);
-            else if (vec) X::load4(t.p, i, w);
-            else for (int k = 0; k < 4; ++k) if (i + k < t.n) w[k] = X::load1(t.p, i + k);
-            if (BITS == 32) {
-                AdamwF32::load4(p.m, a, m);
-                AdamwF32::load4(p.v, a, v);
-            } else {
-                const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.m) + a);
-                const uint32_t cv = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.v) + a);
-                const int sm = p.ms[a / ADAMW_BLOCK], sv = p.vs[a / ADAMW_BLOCK];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    m[k] = adamw_decode<false>((cm >> (8 * k)) & 0xffu, sm);
-                    v[k] = adamw_decode<true>((cv >> (8 * k)) & 0xffu, sv);
-                }
-            }
-        }
+// What a thread reads for its four neighbours of a run.
+template <int BITS> struct AdamwRaw {
+    float g[4], w[4], m[4], v[4];
+    unsigned cm, cv;
+    int sm, sv;
+};
+// i: first of the four, a: its place in the arenas (which reach to the end of the block of 64: always four elements there).  WHOLE: the
+// run lies inside the tensor and can be read four elements at a time.
+template <class X, int BITS, bool NT, bool WHOLE>
+__device__ __forceinline__ void adamw_read(const AdamwP& p, const AdamwT& t, long long i, AdamwRaw<BITS>& r) {
+    const long long a = t.off + i;
+    const bool some = WHOLE || i < t.n;
+    if (WHOLE) {
+        X::template load4<NT>(t.g, i, r.g);
+        if (X::WIDE) X::template load4<NT>(t.p, i, r.w);
+    } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float gk = g[k] * factor;
-            m[k] = p.b1 * m[k] + p.c1 * gk;
-            v[k] = p.b2 * v[k] + (p.c2 * gk) * gk;
-            w[k] = w[k] * decay - step_size * (m[k] / (sqrtf(v[k]) * inv_bc2 + p.eps));
+            r.g[k] = i + k < t.n ? adamw_load1<X>(t.g, i + k) : 0.f;
+            r.w[k] = X::WIDE && i + k < t.n ? adamw_load1<X>(t.p, i + k) : 0.f;
+            r.m[k] = r.v[k] = 0.f;
         }
-        if (i + 4 > t.n) {                // what lies behind the tensor's end stays 0 (a factor that is not finite would make it NaN)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) if (i + k >= t.n) m[k] = v[k] = w[k] = 0.f;
-        }
-        if (some) {
-            if (vec) X::store4(t.p, i, w);
-            else for (int k = 0; k < 4; ++k) if (i + k < t.n) X::store1(t.p, i + k, w[k]);
-            if (!X::WIDE) AdamwF32::store4(p.master, a, w);
-        }
+    }
+    if (some) {
+        if (!X::WIDE) AdamwF32::load4<NT>(p.master, a, r.w);
         if (BITS == 32) {
-            if (some) { AdamwF32::store4(p.m, a, m); AdamwF32::store4(p.v, a, v); }
-        } else {
-            unsigned tm = 0, tv = 0;
+            AdamwF32::load4<NT>(p.m, a, r.m);
+            AdamwF32::load4<NT>(p.v, a, r.v);
+        }
+    }
+    if (BITS == 8) {
+        r.cm = some ? adamw_ld<NT, unsigned>(static_cast<const uint8_t*>(p.m) + a) : 0u;
+        r.cv = some ? adamw_ld<NT, unsigned>(static_cast<const uint8_t*>(p.v) + a) : 0u;
+        r.sm = some ? p.ms[a / ADAMW_BLOCK] : 1;
+        r.sv = some ? p.vs[a / ADAMW_BLOCK] : 1;
+    }
+}
+template <class X, int BITS, bool NT, bool WHOLE>
+__device__ __forceinline__ void adamw_update(const AdamwP& p, const AdamwT& t, const AdamwDyn& h, float factor, long long i, AdamwRaw<BITS>& r) {
+    const long long a = t.off + i;
+    if (BITS == 8) {
+        adamw_decode_m(r.cm, r.sm, r.m);
+        adamw_decode_v(r.cv, r.sv, r.v);
+    }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const unsigned um = adamw_finite_bits(m[k]), uv = adamw_finite_bits(v[k]);
-                tm = tm > um ? tm : um;
-                tv = tv > uv ? tv : uv;
-            }
-            const int em = (int)(adamw_row_max(tm) >> 23), ev = (int)(adamw_row_max(tv) >> 23);
-            const int sm = em > 8 ? em - 7 : 1, sv = ev > 16 ? ev - 15 : 1;
-            unsigned cm = 0, cv = 0;
+    for (int k = 0; k < 4; ++k) {
+        const float g = r.g[k] * factor;
+        r.m[k] = p.b1 * r.m[k] + p.c1 * g;
+        r.v[k] = p.b2 * r.v[k] + (p.c2 * g) * g;
+        // root and reciprocal by the hardware, each off by one unit of the last place: below the rounding of the update itself
+        const float q = r.m[k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(r.v[k]) * h.inv_bc2 + p.eps);
+        r.w[k] = __builtin_fmaf(-h.step_size, q, r.w[k] * h.decay);
+    }
+    const bool some = WHOLE || i < t.n;
+    if (!WHOLE) {                         // what lies behind the tensor's end stays 0 (a factor that is not finite would make it NaN)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const unsigned long long e = (unsigned long long)(i + k);
-                const unsigned bits = adamw_mix((unsigned)e * 0x9E3779B9u + (unsigned)(e >> 32) * 0x85157AF5u + key);
-                cm |= adamw_encode<false>(m[k], sm, bits & 0xffffu) << (8 * k);
-                cv |= adamw_encode<true>(v[k], sv, bits >> 16) << (8 * k);
-            }
-            if (some) {
-                *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.m) + a) = cm;
-                *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.v) + a) = cv;
-                if ((threadIdx.x & 15) == 0) {
-                    p.ms[a / ADAMW_BLOCK] = (uint8_t)sm;
-                    p.vs[a / ADAMW_BLOCK] = (uint8_t)sv;
-                }
-            }
+        for (int k = 0; k < 4; ++k) if (i + k >= t.n) r.m[k] = r.v[k] = r.w[k] = 0.f;
+    }
+    if (WHOLE) X::template store4<NT>(t.p, i, r.w);
+    else for (int k = 0; k < 4; ++k) if (i + k < t.n) adamw_store1<X>(t.p, i + k, r.w[k]);
+    if (some && !X::WIDE) AdamwF32::store4<NT>(p.master, a, r.w);
+    if (BITS == 32) {
+        if (some) { AdamwF32::store4<NT>(p.m, a, r.m); AdamwF32::store4<NT>(p.v, a, r.v); }
+        return;
+    }
+    unsigned um[4], uv[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { um[k] = __float_as_uint(r.m[k]) & 0x7fffffffu; uv[k] = __float_as_uint(r.v[k]); }
+    unsigned tm = adamw_max4(um[0], um[1], um[2], um[3]), tv = adamw_max4(uv[0], uv[1], uv[2], uv[3]);
+    const bool finite = !__any(tm >= 0x7f800000u || tv >= 0x7f800000u);
+    if (!finite) {                        // the scale comes from the values that are
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { um[k] = adamw_finite_bits(r.m[k]); uv[k] = adamw_finite_bits(r.v[k]); }
+        tm = adamw_max4(um[0], um[1], um[2], um[3]);
+        tv = adamw_max4(uv[0], uv[1], uv[2], uv[3]);
+    }
+    const int em = (int)(adamw_row_max(tm) >> 23), ev = (int)(adamw_row_max(tv) >> 23);
+    const int sm = em > 8 ? em - 7 : 1, sv = ev > 16 ? ev - 15 : 1;
+    const unsigned e0 = (unsigned)i * 0x9E3779B9u + (unsigned)((unsigned long long)i >> 32) * 0x85157AF5u + h.key;
+    unsigned cm = 0, cv = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {         // i is a multiple of 4: i + k has the same upper 32 bits
+        const unsigned bits = adamw_mix(e0 + (unsigned)k * 0x9E3779B9u);
+        cm |= (finite ? adamw_encode_m<true>(r.m[k], sm, bits) : adamw_encode_m<false>(r.m[k], sm, bits)) << (8 * k);
+        cv |= (finite ? adamw_encode_v<true>(r.v[k], sv, bits) : adamw_encode_v<false>(r.v[k], sv, bits)) << (8 * k);
+    }
+    if (some) {
+        adamw_st<NT>(static_cast<uint8_t*>(p.m) + a, cm);
+        adamw_st<NT>(static_cast<uint8_t*>(p.v) + a, cv);
+        if ((threadIdx.x & 15) == 0) {
+            p.ms[a / ADAMW_BLOCK] = (uint8_t)sm;
+            p.vs[a / ADAMW_BLOCK] = (uint8_t)sv;
         }
     }
 }
 
+// One block: `per` runs of 1024 elements of one tensor, four neighbours a thread; a run is read while the one before it is computed.
+template <class X, int BITS, bool NT>
+__global__ __launch_bounds__(256) void adamw_kernel(AdamwP p) {
+    const int ti = adamw_tensor(p);
+    if (ti < 0) return;
+    const AdamwT t = p.t[ti];
+    AdamwDyn d = {t.step_size, t.inv_bc2, t.decay, t.key};
+    if (p.dyn) d = p.dyn[t.id];
+    const long long first = (long long)(blockIdx.x - t.blk0) * p.per * 1024;
+    const int runs = (int)min((long long)p.per, (t.n - first + 1023) / 1024), whole = (t.flags & ADAMW_VEC) ? (int)min((long long)p.per, (t.n - first) / 1024) : 0;
+    const long long i0 = first + threadIdx.x * 4;
+    __shared__ double sh[4];
+    AdamwRaw<BITS> now, next;
+    if (whole > 0) adamw_read<X, BITS, NT, true>(p, t, i0, now);
+    const float factor = p.factor ? p.factor[0] : p.parts ? adamw_factor(p.part, p.parts, p.grad_scale, p.max_norm, blockIdx.x ? nullptr : p.norm, sh) : p.grad_scale;
+    for (int r = 0; r < whole; ++r) {
+        if (r + 1 < whole) adamw_read<X, BITS, NT, true>(p, t, i0 + (r + 1) * 1024, next);
+        adamw_update<X, BITS, NT, true>(p, t, d, factor, i0 + r * 1024, now);
+        now = next;
+    }
+    for (int r = whole; r < runs; ++r) {
+        adamw_read<X, BITS, NT, false>(p, t, i0 + r * 1024, now);
+        adamw_update<X, BITS, NT, false>(p, t, d, factor, i0 + r * 1024, now);
+    }
+}
+
 // Sums of squares in 64 bits (the squares of floats are exact there), one a block; adamw_kernel adds them in their order.
-template <class X>
+template <class X, bool NT>
 __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwNormP p) {
     const int ti = adamw_tensor(p);
     double s = 0.0;
@@ -224,7 +290,7 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwNormP p) {
             for (; first + (i - first) / 1024 * 1024 + U * 1024 <= end; i += U * 1024) {
                 float g[U][4];
 #pragma unroll
-                for (int u = 0; u < U; ++u) X::load4(t.g, i + u * 1024, g[u]);
+                for (int u = 0; u < U; ++u) X::template load4<NT>(t.g, i + u * 1024, g[u]);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -233,8 +299,8 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwNormP p) {
         }
         for (; i < end; i += 1024) {
             float g[4] = {0.f, 0.f, 0.f, 0.f};
-            if (i + 4 <= end && (t.flags & ADAMW_VEC)) X::load4(t.g, i, g);
-            else for (int k = 0; k < 4; ++k) if (i + k < end) g[k] = X::load1(t.g, i + k);
+            if (i + 4 <= end && (t.flags & ADAMW_VEC)) X::template load4<NT>(t.g, i, g);
+            else for (int k = 0; k < 4; ++k) if (i + k < end) g[k] = adamw_load1<X>(t.g, i + k);
 #pragma unroll
             for (int k = 0; k < 4; ++k) s = fma((double)g[k], (double)g[k], s);
         }
@@ -258,18 +324,18 @@ __global__ void adamw_prep_kernel(AdamwPrepP p) {
     p.dyn[k] = d;
 }
 
-// The values that codes stand for, four a thread: m (blockIdx.y 0) and v.
+// The values that codes stand for, four of each arena a thread.
+template <bool NT>
 __global__ __launch_bounds__(256) void adamw_unpack_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ ms, const uint8_t* __restrict__ v,
                                                            const uint8_t* __restrict__ vs, float* __restrict__ om, float* __restrict__ ov, long long n4) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= n4) return;
-    const bool second = blockIdx.y != 0;
-    const uint32_t c = reinterpret_cast<const uint32_t*>(second ? v : m)[i];
-    const int s = (second ? vs : ms)[i * 4 / ADAMW_BLOCK];
-    float x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = second ? adamw_decode<true>((c >> (8 * k)) & 0xffu, s) : adamw_decode<false>((c >> (8 * k)) & 0xffu, s);
-    AdamwF32::store4(second ? ov : om, i * 4, x);
+    const unsigned cm = adamw_ld<NT, unsigned>(m + i * 4), cv = adamw_ld<NT, unsigned>(v + i * 4);
+    float x[4], y[4];
+    adamw_decode_m(cm, ms[i * 4 / ADAMW_BLOCK], x);
+    adamw_decode_v(cv, vs[i * 4 / ADAMW_BLOCK], y);
+    AdamwF32::store4<NT>(om, i * 4, x);
+    AdamwF32::store4<NT>(ov, i * 4, y);
 }
 
 }  // namespace mcrn

@@ -33,7 +33,8 @@ struct AdamwP {
     void *m, *v;                          // arenas: float, or codes
     uint8_t *ms, *vs;                     // scale bytes, one for each 64 elements
     float* master;                        // arena of fp32 parameters (16-bit ones only)
-    const double* part;                   // sums of squares of the gradients and their number (0: no clipping)
+    const float* factor;                  // what the gradients are multiplied by, or NULL: each block takes it from
+    const double* part;                   // the sums of squares of the gradients; parts = 0: grad_scale, no clipping
     int parts;
     float max_norm;
     float* norm;                          // receives the norm, or NULL
@@ -57,8 +58,10 @@ struct AdamwPrepP {
 };
 
 unsigned adamw_key(unsigned seed, int id, unsigned step);
-hipError_t launch_adamw(const AdamwP& p, unsigned blocks, int dtype, int bits, hipStream_t st);
-hipError_t launch_adamw_norm(const AdamwNormP& p, unsigned blocks, int dtype, hipStream_t st);
+// elements: of the whole step, for the choice of what streams past the caches
+hipError_t launch_adamw(const AdamwP& p, unsigned blocks, long long elements, int dtype, int bits, hipStream_t st);
+hipError_t launch_adamw_norm(const AdamwNormP& p, unsigned blocks, long long elements, int dtype, hipStream_t st);
+hipError_t launch_adamw_factor(const AdamwP& p, float* factor, hipStream_t st);
 hipError_t launch_adamw_prep(const AdamwPrepP& p, hipStream_t st);
 hipError_t launch_adamw_unpack(const uint8_t* m, const uint8_t* ms, const uint8_t* v, const uint8_t* vs, long long n, float* om, float* ov, hipStream_t st);
 

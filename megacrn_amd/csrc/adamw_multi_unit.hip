@@ -5,19 +5,35 @@ namespace mcrn {
 
 unsigned adamw_key(unsigned seed, int id, unsigned step) { return adamw_key_of(seed, id, step); }
 
-hipError_t launch_adamw(const AdamwP& p, unsigned blocks, int dtype, int bits, hipStream_t st) {
+// A step that moves more than this leaves nothing of itself in the last-level cache (256 MB): it streams past the caches
+static const double STREAM = 256e6;
+
+template <bool NT> static void main_kernel(const AdamwP& p, dim3 grid, int dtype, int bits, hipStream_t st) {
+    const dim3 block(256);
+    if (dtype == 0 && bits == 32) hipLaunchKernelGGL((adamw_kernel<AdamwF32, 32, NT>), grid, block, 0, st, p);
+    else if (dtype == 0) hipLaunchKernelGGL((adamw_kernel<AdamwF32, 8, NT>), grid, block, 0, st, p);
+    else if (bits == 32) hipLaunchKernelGGL((adamw_kernel<AdamwBf16, 32, NT>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((adamw_kernel<AdamwBf16, 8, NT>), grid, block, 0, st, p);
+}
+hipError_t launch_adamw(const AdamwP& p, unsigned blocks, long long elements, int dtype, int bits, hipStream_t st) {
     (void)hipGetLastError();
-    const dim3 grid(blocks), block(256);
-    if (dtype == 0 && bits == 32) hipLaunchKernelGGL((adamw_kernel<AdamwF32, 32>), grid, block, 0, st, p);
-    else if (dtype == 0) hipLaunchKernelGGL((adamw_kernel<AdamwF32, 8>), grid, block, 0, st, p);
-    else if (bits == 32) hipLaunchKernelGGL((adamw_kernel<AdamwBf16, 32>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((adamw_kernel<AdamwBf16, 8>), grid, block, 0, st, p);
+    const double each = (dtype == 0 ? 12 : 14) + (bits == 32 ? 16 : 4);
+    if (elements * each > STREAM) main_kernel<true>(p, dim3(blocks), dtype, bits, st);
+    else main_kernel<false>(p, dim3(blocks), dtype, bits, st);
     return hipGetLastError();
 }
-hipError_t launch_adamw_norm(const AdamwNormP& p, unsigned blocks, int dtype, hipStream_t st) {
+hipError_t launch_adamw_norm(const AdamwNormP& p, unsigned blocks, long long elements, int dtype, hipStream_t st) {
     (void)hipGetLastError();
-    if (dtype == 0) hipLaunchKernelGGL((adamw_norm_kernel<AdamwF32>), dim3(blocks), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((adamw_norm_kernel<AdamwBf16>), dim3(blocks), dim3(256), 0, st, p);
+    const bool nt = elements * (dtype == 0 ? 4.0 : 2.0) > STREAM;
+    if (dtype == 0 && nt) hipLaunchKernelGGL((adamw_norm_kernel<AdamwF32, true>), dim3(blocks), dim3(256), 0, st, p);
+    else if (dtype == 0) hipLaunchKernelGGL((adamw_norm_kernel<AdamwF32, false>), dim3(blocks), dim3(256), 0, st, p);
+    else if (nt) hipLaunchKernelGGL((adamw_norm_kernel<AdamwBf16, true>), dim3(blocks), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((adamw_norm_kernel<AdamwBf16, false>), dim3(blocks), dim3(256), 0, st, p);
+    return hipGetLastError();
+}
+hipError_t launch_adamw_factor(const AdamwP& p, float* factor, hipStream_t st) {
+    (void)hipGetLastError();
+    hipLaunchKernelGGL(adamw_factor_kernel, dim3(1), dim3(256), 0, st, p.part, p.parts, p.grad_scale, p.max_norm, p.norm, factor);
     return hipGetLastError();
 }
 hipError_t launch_adamw_prep(const AdamwPrepP& p, hipStream_t st) {
@@ -28,7 +44,9 @@ hipError_t launch_adamw_prep(const AdamwPrepP& p, hipStream_t st) {
 hipError_t launch_adamw_unpack(const uint8_t* m, const uint8_t* ms, const uint8_t* v, const uint8_t* vs, long long n, float* om, float* ov, hipStream_t st) {
     (void)hipGetLastError();
     const long long n4 = n / 4;
-    hipLaunchKernelGGL(adamw_unpack_kernel, dim3((unsigned)((n4 + 255) / 256), 2), dim3(256), 0, st, m, ms, v, vs, om, ov, n4);
+    const dim3 grid((unsigned)((n4 + 255) / 256));
+    if (n * 10.0 > STREAM) hipLaunchKernelGGL((adamw_unpack_kernel<true>), grid, dim3(256), 0, st, m, ms, v, vs, om, ov, n4);
+    else hipLaunchKernelGGL((adamw_unpack_kernel<false>), grid, dim3(256), 0, st, m, ms, v, vs, om, ov, n4);
     return hipGetLastError();
 }
 

@@ -43,8 +43,8 @@ class AdamW:
             raise ValueError("AdamW: a parameter is given twice")
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits must be 8 or 32; got {state_bits}")
-        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1) or not eps > 0:
-            raise ValueError(f"AdamW: betas must lie in [0, 1) and eps above 0; got {betas}, {eps}")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1) or not 1.2e-38 <= eps < 3e38:
+            raise ValueError(f"AdamW: betas must lie in [0, 1) and eps be a normal float32 above 0; got {betas}, {eps}")
         for g in self.param_groups:
             if not (g["lr"] >= 0 and g["weight_decay"] >= 0):
                 raise ValueError("AdamW: lr and weight_decay must not be negative")
