@@ -59,12 +59,20 @@ template <> __device__ __forceinline__ float glr_up<GlrBf16, 4>(const GlrVec<Glr
 template <class X, int V> __device__ __forceinline__ GlrVec<X, V> glr_load(const char* base, uint32_t off) {
     return *reinterpret_cast<const GlrVec<X, V>*>(base + off);
 }
-template <class X, int V> __device__ __forceinline__ void glr_store(char* base, uint32_t off, const float* v) {
+template <int BYTES> struct GlrWord { typedef uint32_t T __attribute__((ext_vector_type(BYTES / 4))); };
+template <> struct GlrWord<4> { typedef uint32_t T; };
+template <> struct GlrWord<2> { typedef uint16_t T; };
+// NT: past the caches, for sequences larger than these
+template <class X, int V, bool NT = false> __device__ __forceinline__ void glr_store(char* base, uint32_t off, const float* v) {
     GlrVec<X, V> r;
 #pragma unroll
     for (int i = 0; i < V; ++i) r.e[i] = X::down(v[i]);
-    *reinterpret_cast<GlrVec<X, V>*>(base + off) = r;
+    typedef typename GlrWord<sizeof(r)>::T T;
+    if (NT) __builtin_nontemporal_store(__builtin_bit_cast(T, r), reinterpret_cast<T*>(base + off));
+    else *reinterpret_cast<GlrVec<X, V>*>(base + off) = r;
 }
+struct GlrYes { static constexpr bool value = true; };
+struct GlrNo { static constexpr bool value = false; };
 // K rows of a thread, from row seg * K of the tile on.  What lies behind the tile's last row `end` reads that one instead: one minimum a
 // row.  ONCE (no loop around it): whole tiles go without, by scalar bases (in a loop the second path costs registers, and spills).
 template <class X, int V, int K, bool ONCE>
@@ -392,16 +400,20 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
             for (int i = 0; i < V; ++i) h[i] = carry[i];
         }
         float o[V];
-        if (live) {
+        auto steps = [&](auto nt) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
+            for (int k = 0; k < K; ++k) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if (SEG > 1) o[i] = fmaf(ww[k][i], h[i], cc[k][i]);
-                else o[i] = h[i] = fmaf(ww[k][i], cc[k][i] - h[i], h[i]);
+                for (int i = 0; i < V; ++i) {
+                    if (SEG > 1) o[i] = fmaf(ww[k][i], h[i], cc[k][i]);
+                    else o[i] = h[i] = fmaf(ww[k][i], cc[k][i] - h[i], h[i]);
+                }
+                if (w.active && p.out && (full || ts + k < w.t1)) glr_store<X, V, decltype(nt)::value>(po + k * rb, lo, o);
             }
-            if (w.active && p.out && (full || ts + k < w.t1)) glr_store<X, V>(po + k * rb, lo, o);
-        }
+        };
+        if (live) {
+            if (p.nt) steps(GlrYes());
+            else steps(GlrNo());
         }
         po += span * rb;
         if (p.ckpt && w.active && ts + K < p.T) {          // the state before step ts + K
@@ -590,32 +602,36 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
 #pragma unroll
             for (int i = 0; i < V; ++i) mu[i] = carry[i];
         }
-        if (live) {
+        auto steps = [&](auto nt) {
 #pragma unroll
-        for (int k = K - 1; k >= 0; --k) {
-            const bool in = w.active && (full || ts + k < w.t1);
-            float dc[V], dg[V];
+            for (int k = K - 1; k >= 0; --k) {
+                const bool in = w.active && (full || ts + k < w.t1);
+                float dc[V], dg[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float lam = mu[i] + dd[k][i];
-                dc[i] = lam * wc[k][i];
-                dg[i] = lam * q[k][i];
-                mu[i] = fmaf(-ww[k][i], lam, lam);
-            }
-            if (in) glr_store<X, V>(pdc + k * rb, ldc, dc);
-            if (!SHARED) {
-                if (in) glr_store<X, VG>(pdg + k * gb, ldg, dg);
-            } else {
-                float s = 0.f;
+                for (int i = 0; i < V; ++i) {
+                    const float lam = mu[i] + dd[k][i];
+                    dc[i] = lam * wc[k][i];
+                    dg[i] = lam * q[k][i];
+                    mu[i] = fmaf(-ww[k][i], lam, lam);
+                }
+                if (in) glr_store<X, V, decltype(nt)::value>(pdc + k * rb, ldc, dc);
+                if (!SHARED) {
+                    if (in) glr_store<X, VG, decltype(nt)::value>(pdg + k * gb, ldg, dg);
+                } else {
+                    float s = 0.f;
 #pragma unroll
-                for (int i = 0; i < V; ++i) s += w.active ? dg[i] : 0.f;
-                s = glr_lane_sum(s, p.L);
-                if (in && w.gl == 0) {
-                    if (p.parts == 1) glr_store<X, 1>(pdg + k * gb, ldg, &s);
-                    else p.part[((((long long)w.b * p.T + ts + k) * p.N + w.n) * p.G + w.gi) * p.parts + w.part] = s;
+                    for (int i = 0; i < V; ++i) s += w.active ? dg[i] : 0.f;
+                    s = glr_lane_sum(s, p.L);
+                    if (in && w.gl == 0) {
+                        if (p.parts == 1) glr_store<X, 1>(pdg + k * gb, ldg, &s);
+                        else p.part[((((long long)w.b * p.T + ts + k) * p.N + w.n) * p.G + w.gi) * p.parts + w.part] = s;
+                    }
                 }
             }
-        }
+        };
+        if (live) {
+            if (p.nt) steps(GlrYes());
+            else steps(GlrNo());
         }
         pdc -= span * rb;
         pdg -= span * gb;

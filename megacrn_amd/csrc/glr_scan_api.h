@@ -33,6 +33,7 @@ struct GlrP {
     int V, K, CL, S, L, parts;              // channels and steps a thread, channel lanes a block, chunks of the time axis,
     int chunk, first;                       // lanes and parts of a shared gate's channels; steps a chunk, first chunk of the launch
     long long nq, tiles;                    // channel vectors of a batch entry, blocks that cover them
+    bool nt;                                // outputs go past the caches
     bool chain;                             // a chunk is one tile and takes its state from the block before it
     float *agg, *part;                      // workspace: chunk aggregates, partial gate gradients,
     unsigned *ticket, *carry;               // chunks taken of each tile, states behind the chunks (chain)
