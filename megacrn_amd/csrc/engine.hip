@@ -2955,11 +2955,12 @@ static bool glr_workspace(GlrP& p, bool backward, void* ws, size_t ws_bytes) {
     glr_place(p, ws);
     return true;
 }
-// A lane addresses its rows with 32 bits behind a base of its block: rows of a tile (128 at most, in time) and the nodes of a row
+// A lane addresses its rows with 32 bits behind a base of its block: the rows of a tile and the nodes of a row
 static bool glr_near(const GlrP& p) {
-    const long long es = p.dtype == GLR_F32 ? 4 : 2, rows = GLR_TILE < p.T ? GLR_TILE : p.T, most = 1ll << 32;
-    auto fits = [&](bool used, long long st, long long sn, long long w, long long size) { return !used || (rows * st + p.N * sn + w) * size < most; };
-    const long long NH = (long long)p.N * p.H;
+    const long long es = p.dtype == GLR_F32 ? 4 : 2, rows = std::min<long long>((long long)glr_tile(p), p.T), NH = (long long)p.N * p.H;
+    auto fits = [&](bool used, long long st, long long sn, long long w, long long size) {
+        return !used || ((rows > 1 ? (rows - 1) * st : 0) + (p.N - 1) * sn + w) * size < (1ll << 32);
+    };
     return fits(true, p.g_st, p.g_sn, p.G, es) && fits(true, p.c_st, p.c_sn, p.H, es) && fits(p.mask, p.m_st, p.m_sn, 1, 1) && fits(p.dout, p.d_st, p.d_sn, p.H, es) &&
            fits(true, NH, 0, NH, 4);
 }
@@ -2979,7 +2980,7 @@ int mcrn_glr_forward(const mcrn_glr_t* d, const void* gate, const void* cand, co
     p.ckpt = p.dtype == GLR_F32 ? nullptr : ckpt;
     if (!glr_aligned(p)) FAIL("glr_forward: a pointer is not aligned to its type");
     if (!glr_plan(p, false)) FAIL("glr_forward: too many sequences");
-    if (!glr_near(p)) FAIL("glr_forward: strides over time or nodes reach over 4 GB within %d steps", GLR_TILE);
+    if (!glr_near(p)) FAIL("glr_forward: strides over time and nodes reach over 4 GB within %d steps", glr_tile(p));
     if (!glr_workspace(p, false, ws, ws_bytes)) FAIL("glr_forward: the workspace is too small or not 256-byte aligned");
     fam(p.chain ? "glr:fwd_chain" : p.S > 1 ? "glr:fwd_split" : p.CL == 256 ? "glr:fwd_stream" : "glr:fwd_tile");
     CK(launch_glr_forward(p, (hipStream_t)stream, &g_launches));
@@ -3000,7 +3001,7 @@ int mcrn_glr_backward(const mcrn_glr_t* d, const void* gate, const void* cand, c
     p.dout = dout; p.dlast = dlast; p.dgate = dgate; p.dcand = dcand; p.dstate = dstate;
     if (!glr_aligned(p)) FAIL("glr_backward: a pointer is not aligned to its type");
     if (!glr_plan(p, true)) FAIL("glr_backward: too many sequences");
-    if (!glr_near(p)) FAIL("glr_backward: strides over time or nodes reach over 4 GB within %d steps", GLR_TILE);
+    if (!glr_near(p)) FAIL("glr_backward: strides over time and nodes reach over 4 GB within %d steps", glr_tile(p));
     if (!glr_workspace(p, true, ws, ws_bytes)) FAIL("glr_backward: the workspace is too small or not 256-byte aligned");
     fam(p.chain ? "glr:bwd_chain" : p.S > 1 ? "glr:bwd_split" : p.CL == 256 ? "glr:bwd_stream" : "glr:bwd_tile");
     CK(launch_glr_backward(p, (hipStream_t)stream, &g_launches));

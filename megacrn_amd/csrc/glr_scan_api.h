@@ -40,11 +40,11 @@ struct GlrP {
 };
 
 constexpr int GLR_K = 8;                    // steps a thread holds in registers, at most = distance of the checkpoints
-constexpr int GLR_TILE = 128;               // steps of a block's tile, at most
 int glr_steps(int T);
 
 bool glr_plan(GlrP& p, bool backward);      // fills the plan; false: too large
 size_t glr_ws_bytes(const GlrP& p, bool backward);
+int glr_tile(const GlrP& p);                 // steps of a block's tile
 void glr_place(GlrP& p, void* ws);          // the plan's parts of the workspace
 hipError_t launch_glr_forward(const GlrP& p, hipStream_t st, int* launches);
 hipError_t launch_glr_backward(const GlrP& p, hipStream_t st, int* launches);

@@ -8,6 +8,8 @@ static long long up_div(long long a, long long b) { return (a + b - 1) / b; }
 // Steps a thread holds.  T alone decides, so that a backward finds the checkpoints of its forward.
 int glr_steps(int T) { return T <= 1 ? 1 : T <= 4 || (T > 8 && T <= 12) ? 4 : GLR_K; }
 
+int glr_tile(const GlrP& p) { return GLR_THREADS / p.CL * p.K; }
+
 bool glr_plan(GlrP& p, bool backward) {
     const size_t size = p.dtype == GLR_F32 ? 4 : 2;
     const int D = p.H / p.G;
@@ -49,15 +51,22 @@ bool glr_plan(GlrP& p, bool backward) {
     long long blocks = cover(256);
     if (p.T > GLR_K && p.K == GLR_K && blocks < 512) {
         const int span = GLR_THREADS / 16 * GLR_K;
-        const int quarter = GLR_THREADS / 64 * GLR_K;     // steps of a wave of the 16-lane form, of a tile of the 64-lane form
-        const bool loose = up_div(p.T, quarter) < 3 * up_div(p.T, span);      // over a quarter of the 16-lane form's waves would idle
+        // From here on fewer than 512 blocks of 256 channel lanes: time is cut over the lanes of a block as well.
+        //  - 64 lanes x 4 segments: up to 32 steps, and where more than a quarter of the 16-lane form's waves would idle behind the last step
+        //    (144 steps: 26 us forward against 36; 48 steps: 28 against 35), if that still makes a block for every compute unit.
+        //  - 16 lanes x 16 segments, a block for every 128 steps, each handing its state to the next (chain), from 64 blocks a chunk on: a hand-over
+        //    takes 1.6 us, so that many chunks of few channels wait (20161 steps: 128 tiles 484 us against 672 split, 64 tiles 321 : 351,
+        //    32 tiles 265 : 185).
+        //  - fewer: the chunks' maps first (they need no state), then every chunk from the maps before it.  Inputs are read twice.
+        const int quarter = GLR_THREADS / 64 * GLR_K;
+        const bool loose = up_div(p.T, quarter) < 3 * up_div(p.T, span);
         if (p.T <= quarter || (loose && cover(64) >= 256)) {
             cover(64);
         } else if ((blocks = cover(16)) >= 64 && p.T > span) {
             p.chain = true;
             p.chunk = span;
             p.S = (int)up_div(p.T, span);
-        } else if (p.T > span) {
+        } else if (p.T > span && !(p.last && p.last == p.h0)) {      // (a split reads h0 in every chunk: not while it is overwritten)
             long long S = up_div(1024, blocks);
             S = S > 256 ? 256 : S;
             const long long most = up_div(p.T, span);

@@ -90,7 +90,15 @@ void strides_of(const Tensor& t, int64_t lead, long long* s) {
     const int64_t at[3] = {0, lead == 3 ? 1 : -1, lead - 1};
     for (int i = 0; i < 3; ++i) s[i] = at[i] < 0 || t.size(at[i]) == 1 ? 0 : t.stride(at[i]);
 }
-Tensor rows(const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// The kernels want a last dimension without gaps, and a tile's rows (128 steps at most) within 4 GB of each other: a copy where that is not so.
+Tensor rows(const Tensor& t, int64_t lead) {
+    if (!t.defined()) return t;
+    long long s[3];
+    strides_of(t, lead, s);
+    const long long steps = lead == 3 ? std::min<int64_t>(t.size(1), 128) : 1;
+    const bool near = ((steps - 1) * s[1] + (t.size(-2) - 1) * s[2] + t.size(-1)) * (long long)t.element_size() < (1ll << 32);
+    return (t.size(-1) == 1 || t.stride(-1) == 1) && near ? t : t.contiguous();
+}
 
 mcrn_glr_t dims_of(const Tensor& gate, const Tensor& cand, const Tensor& mask, const Tensor& dout, int act, int64_t lead) {
     mcrn_glr_t d = {};
@@ -150,7 +158,7 @@ struct GlrNode : torch::autograd::Function<GlrNode> {
         const auto s = ctx->get_saved_variables();
         const Tensor &gate = s[0], &cand = s[1], &h0 = s[2], &mask = s[3], &kept = s[4];
         const at::DeviceGuard guard(cand.device());
-        const Tensor dout = rows(g[0]), dlast = g[1].defined() ? g[1].contiguous() : Tensor();
+        const Tensor dout = rows(g[0], 3), dlast = g[1].defined() ? g[1].contiguous() : Tensor();
         const mcrn_glr_t d = dims_of(gate, cand, mask, dout, (int)ctx->saved_data["act"].toInt(), 3);
         out[0] = at::empty(gate.sizes(), gate.options());
         out[1] = at::empty(cand.sizes(), cand.options());
@@ -174,7 +182,7 @@ std::pair<Tensor, Tensor> glr(const Tensor& gate0, const Tensor& cand0, const Op
         const Tensor last = h0.defined() ? h0.clone() : at::zeros({cand0.size(0), cand0.size(2), cand0.size(3)}, cand0.options().dtype(at::kFloat));
         return {at::empty(cand0.sizes(), cand0.options()), last};
     }
-    const Tensor gate = rows(gate0), cand = rows(cand0);
+    const Tensor gate = rows(gate0, 3), cand = rows(cand0, 3);
     if (at::GradMode::is_enabled() && (gate.requires_grad() || cand.requires_grad() || (h0.defined() && h0.requires_grad()))) {
         auto r = GlrNode::apply(gate, cand, state, mask.defined() ? OptTensor(mask) : OptTensor(), (int64_t)act);
         return {r[0], r[1]};
@@ -191,7 +199,7 @@ Tensor glr_step(const Tensor& gate0, const Tensor& cand0, const OptTensor& state
     const Tensor mask = check_inputs(gate0, cand0, state, mask0.value_or(Tensor()), who, 2);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (gate0.requires_grad() || cand0.requires_grad() || state.requires_grad())), who,
                 " is not differentiable: call it under torch.no_grad()");
-    const Tensor gate = rows(gate0), cand = rows(cand0), out = at::empty(cand.sizes(), cand.options());
+    const Tensor gate = rows(gate0, 2), cand = rows(cand0, 2), out = at::empty(cand.sizes(), cand.options());
     if (out.numel() == 0) return out;
     const at::DeviceGuard guard(cand.device());
     const mcrn_glr_t d = dims_of(gate, cand, mask, Tensor(), act, 2);

@@ -77,8 +77,7 @@ class AdamW:
         self.master = None
         if self.dtype == torch.bfloat16:
             self.master = torch.zeros(n, device=dev)
-            for p, o in zip(self.params, self.offsets):
-                self.master[o:o + p.numel()].copy_(p.detach().reshape(-1))
+            self.sync_masters()
         nb = lib.mcrn_adamw_workspace_bytes(C.byref(self._cfg), self._numel)
         self._ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         self.total_norm = torch.zeros((), device=dev)
@@ -96,6 +95,8 @@ class AdamW:
         now = [(g["lr"], g["weight_decay"]) for g in self.param_groups]
         if now == self._seen:
             return
+        if any(not (lr >= 0 and wd >= 0) for lr, wd in now):
+            raise ValueError(f"AdamW: lr and weight_decay must not be negative; the groups have {now}")
         self._seen, i = now, 0
         for g in self.param_groups:
             lr, wd = g["lr"], g["weight_decay"]
@@ -110,6 +111,12 @@ class AdamW:
         self._read_groups()
         self._dev[0].copy_(torch.tensor(list(self._lr), dtype=torch.float64))
         self._dev[1].copy_(torch.tensor(list(self._wd), dtype=torch.float64))
+
+    def sync_masters(self):
+        """bf16 parameters: takes their values into the fp32 masters - after they were written by anything but `step` (a loaded model)."""
+        if self.master is not None:
+            for p, o in zip(self.params, self.offsets):
+                self.master[o:o + p.numel()].copy_(p.detach().reshape(-1))
 
     # -- the step
     @torch.no_grad()
@@ -148,7 +155,7 @@ class AdamW:
         return list(self._steps) if self._dev is None else self._dev[2].tolist()
 
     def state_dict(self):
-        d = {"state_bits": self.state_bits, "steps": self.steps(), "m": self._m.clone(), "v": self._v.clone(),
+        d = {"state_bits": self.state_bits, "seed": self.seed, "steps": self.steps(), "m": self._m.clone(), "v": self._v.clone(),
              "groups": [{"lr": g["lr"], "weight_decay": g["weight_decay"]} for g in self.param_groups]}
         if self._ms is not None:
             d["m_scale"], d["v_scale"] = self._ms.clone(), self._vs.clone()
@@ -157,7 +164,8 @@ class AdamW:
         return d
 
     def load_state_dict(self, d):
-        """Takes what state_dict() of an optimizer of the same parameters and state_bits gave."""
+        """Takes what state_dict() of an optimizer of the same parameters and state_bits gave: moments, masters, step counts, seed and the
+        groups' rates."""
         if d["state_bits"] != self.state_bits:
             raise ValueError(f"AdamW: the state holds {d['state_bits']}-bit moments, this optimizer {self.state_bits}-bit ones")
         mine = {"m": self._m, "v": self._v}
@@ -176,6 +184,8 @@ class AdamW:
             t.copy_(d[k])
         for i, s in enumerate(d["steps"]):
             self._steps[i] = int(s)
+        self.seed = int(d.get("seed", self.seed))
+        self._cfg.seed = self.seed & 0xFFFFFFFF
         for g, h in zip(self.param_groups, d.get("groups", ())):
             g.update(lr=float(h["lr"]), weight_decay=float(h["weight_decay"]))
         if self._dev is not None:

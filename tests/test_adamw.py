@@ -68,7 +68,7 @@ def test_arena_and_workspace_sizes():
     def cfg(k=4, dtype=0, bits=32):
         return C.byref(Adamw(k, dtype, bits, 0, 0, 0, 0.9, 0.999, 1e-8, 0.0, 1.0))
     assert lib.mcrn_adamw_arena_elements(cfg(), n) == 64 + 64 + 128
-    assert lib.mcrn_adamw_workspace_bytes(cfg(), n) > 256
+    assert lib.mcrn_adamw_workspace_bytes(cfg(), n) > 0
     for bad in (cfg(k=0), cfg(dtype=2), cfg(bits=4)):
         assert lib.mcrn_adamw_arena_elements(bad, n) == -1 and lib.mcrn_adamw_workspace_bytes(bad, n) == 0
     assert lib.mcrn_adamw_arena_elements(cfg(), (C.c_longlong * 4)(1, -1, 65, 0)) == -1
@@ -332,6 +332,10 @@ def test_grad_attribute_views_and_errors():
         opt.step(grads=[p[0].detach(), None, None], grad_scale=0.0)
     assert opt.steps() == [1, 0, 1]
     d = opt.state_dict()
+    opt.param_groups[0]["lr"] = -1.0
+    with pytest.raises(ValueError):
+        opt.step(grads=[None, None, p[2].detach().clone()])
+    opt.param_groups[0]["lr"] = 1e-2
     for broken in (dict(d, state_bits=8), dict(d, m=d["m"][:-1]), dict(d, steps=[1]), dict(d, groups=[]), dict(d, steps=[1, -1, 1])):
         with pytest.raises(ValueError):
             opt.load_state_dict(broken)
@@ -354,7 +358,7 @@ def test_resumed_and_captured_runs(bits, dt):
     first = megacrn_amd.AdamW(qs, **kw)
     for g in grads[:3]:
         first.step(grads=g)
-    second = megacrn_amd.AdamW(qs, **dict(kw, lr=5.0))
+    second = megacrn_amd.AdamW(qs, **dict(kw, lr=5.0, seed=77))
     second.load_state_dict(first.state_dict())
     for g in grads[3:]:
         second.step(grads=g)
@@ -384,6 +388,37 @@ def test_resumed_and_captured_runs(bits, dt):
             opt.step(grads=grads[0])
     torch.cuda.synchronize()
     opt.step(grads=grads[0])                                              # eager work goes on
+
+
+@pytest.mark.gpu
+def test_masters_follow_a_loaded_model():
+    import megacrn_amd
+    p = torch.randn(100, device="cuda").to(torch.bfloat16)
+    opt = megacrn_amd.AdamW([p], lr=1e-3, weight_decay=0.0)
+    p.copy_(torch.ones(100, device="cuda"))
+    opt.sync_masters()
+    opt.step(grads=[torch.ones_like(p)])
+    assert (opt.master[:100] - (1 - 1e-3)).abs().max() <= 4 * O.U and opt.master[100:].abs().max() == 0
+
+
+@pytest.mark.gpu
+def test_wide_range_of_moments_in_8_bits():
+    """Gradients of one block over 36 octaves, the smallest and largest that fp32 squares hold, and zeros: codes against the oracle."""
+    import megacrn_amd
+    g = torch.cat([torch.tensor([2.0 ** (k - 30) for k in range(36)]), torch.zeros(28), torch.tensor([1e-30, 1e-23, 1e-19, 0.0] * 16),
+                   torch.tensor([1e18, 3e18, 1.0, 1e-3] * 16), torch.full((64,), 1e-38)]).cuda()
+    opt = megacrn_amd.AdamW([torch.zeros_like(g)], state_bits=8, seed=5)
+    for step in (1, 2, 3):
+        old = [_piece(a, opt, 0) for a in opt.moments()]
+        opt.step(grads=[g])
+        m, v = O.moments_f32(g.cpu().numpy(), *old, F(1.0))
+        bits = O.random_bits(5, 0, step, g.numel())
+        d = opt.state_dict()
+        for key, x, r, second in (("m", m, bits & 0xFFFF, False), ("v", v, bits >> 16, True)):
+            codes, scales = O.encode(x, r, second)
+            assert (d[key].cpu().numpy() == codes).all() and (d[key + "_scale"].cpu().numpy() == scales).all()
+            assert ((codes > 0) | (x == 0)).all() or not second                # a v above 0 never gets code 0
+    assert torch.isfinite(opt.params[0]).all()
 
 
 @pytest.mark.gpu
