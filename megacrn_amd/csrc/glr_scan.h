@@ -130,6 +130,10 @@ template <bool FINE> __device__ __forceinline__ float glr_tanh(float u) {
     return fabsf(u) < 0.25f ? fmaf(u * q, s, u) : far;
 }
 
+// c - h, what a step goes towards; where it goes nowhere (w = 0: masked, or a gate that is open) an infinite state stays what it is
+__device__ __forceinline__ float glr_diff(float w, float c, float h) { return c - (w == 0.f ? 0.f : h); }
+__device__ __forceinline__ float glr_next(float w, float c, float h) { return fmaf(w, glr_diff(w, c, h), h); }
+
 // ---- where a thread works ----------------------------------------------------------------------------------------------
 struct GlrAt {
     int b, chunk, cl, seg, t0, t1;
@@ -410,7 +414,7 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     if (SEG > 1) o[i] = fmaf(ww[k][i], h[i], cc[k][i]);
-                    else o[i] = h[i] = fmaf(ww[k][i], cc[k][i] - h[i], h[i]);
+                    else o[i] = h[i] = glr_next(ww[k][i], cc[k][i], h[i]);
                 }
                 if (w.active && p.out && (full || ts + k < w.t1)) glr_store<X, V, decltype(nt)::value>(po + k * rb, lo, o);
             }
@@ -567,7 +571,7 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                 for (int k = 0; k < K; ++k)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float c = wc[k][i], diff = c - h[i];
+                        const float c = wc[k][i], diff = glr_diff(ww[k][i], c, h[i]);
                         q[k][i] *= -diff;
                         h[i] = fmaf(ww[k][i], diff, h[i]);
                         wc[k][i] = p.act ? ww[k][i] * fmaf(-c, c, 1.f) : ww[k][i];

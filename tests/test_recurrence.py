@@ -305,6 +305,32 @@ def test_steps_are_the_sequence(dt, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("B,T,N,H", [(2, 1, 3, 8), (2, 5, 3, 8), (2, 30, 3, 8), (2, 300, 3, 8), (1, 300, 40, 64), (64, 20, 40, 256)])
+def test_state_of_a_masked_row_is_kept_whatever_it_is(B, T, N, H, dt):
+    """Infinities and NaN among the states that no step writes; the gradients of masked steps are 0 there too."""
+    import megacrn_amd
+    gate, cand, st, _, _, _ = (None if t is None else t.cuda() for t in _inputs(B, T, N, H, H, dt, False, 3))
+    keep = torch.ones(B, T, N, dtype=torch.bool, device="cuda")
+    keep[-1, :, 1] = False
+    st[-1, 1, :4] = torch.tensor([float("inf"), -float("inf"), 3e38, float("nan")], device="cuda")
+    gate[-1, :, 1], cand[-1, :, 1] = float("nan"), float("inf")
+    gate.requires_grad_(), cand.requires_grad_()
+    out, last = megacrn_amd.gated_linear_recurrence(gate, cand, st, keep)
+    want = st[-1, 1]
+    assert torch.equal(torch.nan_to_num(last[-1, 1], 7.0), torch.nan_to_num(want, 7.0)) and torch.isnan(last).sum() == 1
+    rows = want.to(TORCH[dt]).expand(T, H)
+    assert torch.equal(torch.nan_to_num(out[-1, :, 1], 7.0), torch.nan_to_num(rows, 7.0)) and torch.isnan(out).sum() == T
+    dgate, dcand = torch.autograd.grad(out, (gate, cand), torch.ones_like(out))
+    assert not dgate[-1, :, 1].any() and not dcand[-1, :, 1].any() and torch.isfinite(dcand).all() and torch.isfinite(dgate).all()
+    now = st.clone()
+    with torch.no_grad():
+        step = megacrn_amd.gated_linear_recurrence_step(gate[:, 0], cand[:, 0], now, keep[:, 0])
+    assert torch.equal(torch.nan_to_num(now[-1, 1], 7.0), torch.nan_to_num(want, 7.0)) and torch.isnan(now).sum() == 1
+    assert torch.equal(torch.nan_to_num(step[-1, 1], 7.0), torch.nan_to_num(rows[0], 7.0))
+
+
+@pytest.mark.gpu
 def test_nan_stays_in_its_row():
     """A NaN that is not masked reaches its own channel's later steps and nothing else."""
     import megacrn_amd
