@@ -34,6 +34,9 @@ class AdamW:
         params = list(params)
         if params and not isinstance(params[0], dict):
             params = [{"params": params}]
+        for g in params:
+            if set(g) - {"params", "lr", "weight_decay"}:
+                raise ValueError(f"AdamW: a group has params, lr and weight_decay; got {sorted(g)}")
         self.param_groups = [{"params": list(g["params"]), "lr": float(g.get("lr", lr)),
                               "weight_decay": float(g.get("weight_decay", weight_decay))} for g in params]
         self.params = [p for g in self.param_groups for p in g["params"]]
@@ -54,6 +57,9 @@ class AdamW:
                 raise TypeError("AdamW: parameters must be float32 or bfloat16 tensors, all of one type")
             if p.device != first.device or not p.is_contiguous():
                 raise ValueError("AdamW: parameters must be contiguous tensors on one device")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("AdamW: two parameters share memory")
         _need_gpu(first, "AdamW")
         self.device, self.dtype = first.device, first.dtype
         self.betas, self.eps, self.max_grad_norm = tuple(betas), float(eps), float(max_grad_norm or 0.0)
@@ -87,8 +93,15 @@ class AdamW:
             self._dev = (torch.zeros(k, dtype=torch.float64, device=dev), torch.zeros(k, dtype=torch.float64, device=dev),
                          torch.zeros(k, dtype=torch.int32, device=dev))
             self.sync_lr()
+        self._addresses()
+
+    def _addresses(self):
         self._numel_at = C.addressof(self._numel)
         self._hyper = tuple(C.addressof(a) for a in (self._lr, self._wd, self._steps)) if self._dev is None else tuple(t.data_ptr() for t in self._dev)
+
+    def __setstate__(self, d):                 # a copy (copy.deepcopy, pickle) has arrays of its own
+        self.__dict__.update(d)
+        self._addresses()
 
     # -- learning rates
     def _read_groups(self):

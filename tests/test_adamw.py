@@ -96,6 +96,18 @@ def test_refuses_a_parameter_twice():
         megacrn_amd.AdamW([{"params": [p]}, {"params": [p]}])
 
 
+def test_refuses_shared_memory_and_unknown_group_keys():
+    import megacrn_amd
+    base = torch.zeros(9)
+    for pair in ([base[:5], base[4:]], [base, base.view(3, 3)], [base[4:5], base]):
+        with pytest.raises(ValueError, match="share memory"):
+            megacrn_amd.AdamW(pair)
+    with pytest.raises(RuntimeError, match="MI355X"):                     # neighbours, and an empty one in between: only the device is wrong
+        megacrn_amd.AdamW([base[:4], base[4:], base[2:2]])
+    with pytest.raises(ValueError, match="lr and weight_decay"):
+        megacrn_amd.AdamW([{"params": [torch.zeros(3)], "betas": (0.8, 0.9)}])
+
+
 def test_trainer_and_command_options():
     from megacrn_amd.train import build_parser
     from megacrn_amd.trainer import FlatTrainer
@@ -388,6 +400,25 @@ def test_resumed_and_captured_runs(bits, dt):
             opt.step(grads=grads[0])
     torch.cuda.synchronize()
     opt.step(grads=grads[0])                                              # eager work goes on
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capturable", [False, True])
+def test_copied_optimizer(capturable):
+    """A deep copy (parameters included) goes on by itself: its steps are the original's, and leave the original alone."""
+    import copy
+    import megacrn_amd
+    ps, gs = _make([(65, 3), (4100,)], torch.bfloat16, 9)
+    opt = megacrn_amd.AdamW(ps, lr=1e-2, state_bits=8, max_grad_norm=1.0, capturable=capturable)
+    opt.step(grads=gs)
+    twin = copy.deepcopy(opt)
+    assert all(a is b for a, b in zip(twin.params, twin.param_groups[0]["params"]))
+    before = [p.clone() for p in ps]
+    twin.step(grads=gs)
+    assert opt.steps() == [1, 1] and twin.steps() == [2, 2] and all(torch.equal(p, q) for p, q in zip(ps, before))
+    opt.step(grads=gs)
+    assert opt.steps() == [2, 2] and all(torch.equal(p, q) for p, q in zip(ps, twin.params))
+    assert all(torch.equal(x, y) for x, y in zip(opt.moments(), twin.moments()))
 
 
 @pytest.mark.gpu
