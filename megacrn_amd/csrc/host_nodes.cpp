@@ -11,6 +11,8 @@
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <mutex>
+
 #include "../../include/megacrn_hip.h"
 
 namespace {
@@ -40,7 +42,14 @@ void bind(const pybind11::dict& d) {
     take(d, "mcrn_adamw_unpack", api.adamw_unpack);
 }
 
-void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (rc=", rc, "): ", api.last_error()); }
+// The library takes one host thread at a time.  A backward pass runs on the autograd engine's thread without the interpreter lock, while another
+// thread of the program may take a step: they wait for one another here.
+std::mutex one_at_a_time;
+template <class F> void call(const char* what, F f) {
+    const std::lock_guard<std::mutex> lock(one_at_a_time);
+    const int rc = f();
+    TORCH_CHECK(rc == 0, what, " failed (rc=", rc, "): ", api.last_error());
+}
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void need_gpu(const Tensor& t, const char* who) {
@@ -136,9 +145,10 @@ Sequence glr_run(const Tensor& gate, const Tensor& cand, const Tensor& state, co
         if (const size_t n = api.glr_checkpoint_floats(&d)) r.ckpt = at::empty({(int64_t)n}, f32);
     size_t nb;
     const Tensor ws = workspace(d, 0, cand, nb);
-    check(api.glr_forward(&d, ptr(gate), ptr(cand), (const unsigned char*)ptr(mask), (const float*)ptr(state), ws.defined() ? ws.mutable_data_ptr() : nullptr, nb,
-                          r.out.mutable_data_ptr(), (float*)r.last.mutable_data_ptr(), r.ckpt.defined() ? (float*)r.ckpt.mutable_data_ptr() : nullptr, stream_of(cand)),
-          "mcrn_glr_forward");
+    call("mcrn_glr_forward", [&] {
+        return api.glr_forward(&d, ptr(gate), ptr(cand), (const unsigned char*)ptr(mask), (const float*)ptr(state), ws.defined() ? ws.mutable_data_ptr() : nullptr, nb,
+                               r.out.mutable_data_ptr(), (float*)r.last.mutable_data_ptr(), r.ckpt.defined() ? (float*)r.ckpt.mutable_data_ptr() : nullptr, stream_of(cand));
+    });
     return r;
 }
 
@@ -166,10 +176,11 @@ struct GlrNode : torch::autograd::Function<GlrNode> {
         if (h0.defined()) out[2] = at::empty(h0.sizes(), h0.options());
         size_t nb;
         const Tensor ws = workspace(d, 1, cand, nb);
-        check(api.glr_backward(&d, ptr(gate), ptr(cand), (const unsigned char*)ptr(mask), (const float*)ptr(h0), ptr(kept), ptr(dout), (const float*)ptr(dlast),
-                               ws.defined() ? ws.mutable_data_ptr() : nullptr, nb, out[0].mutable_data_ptr(), out[1].mutable_data_ptr(),
-                               h0.defined() ? (float*)out[2].mutable_data_ptr() : nullptr, stream_of(cand)),
-              "mcrn_glr_backward");
+        call("mcrn_glr_backward", [&] {
+            return api.glr_backward(&d, ptr(gate), ptr(cand), (const unsigned char*)ptr(mask), (const float*)ptr(h0), ptr(kept), ptr(dout), (const float*)ptr(dlast),
+                                    ws.defined() ? ws.mutable_data_ptr() : nullptr, nb, out[0].mutable_data_ptr(), out[1].mutable_data_ptr(),
+                                    h0.defined() ? (float*)out[2].mutable_data_ptr() : nullptr, stream_of(cand));
+        });
         return out;
     }
 };
@@ -205,7 +216,9 @@ Tensor glr_step(const Tensor& gate0, const Tensor& cand0, const OptTensor& state
     const at::DeviceGuard guard(cand.device());
     const mcrn_glr_t d = dims_of(gate, cand, mask, Tensor(), act, 2);
     float* h = (float*)state.mutable_data_ptr();
-    check(api.glr_forward(&d, ptr(gate), ptr(cand), (const unsigned char*)ptr(mask), h, nullptr, 0, out.mutable_data_ptr(), h, nullptr, stream_of(cand)), "mcrn_glr_forward");
+    call("mcrn_glr_forward", [&] {
+        return api.glr_forward(&d, ptr(gate), ptr(cand), (const unsigned char*)ptr(mask), h, nullptr, 0, out.mutable_data_ptr(), h, nullptr, stream_of(cand));
+    });
     changed(state);
     return out;
 }
@@ -243,12 +256,14 @@ void adamw_step(uintptr_t cfg_at, const std::vector<Tensor>& params, const std::
             for (size_t i = 0; i < n; ++i)
                 if (grads[i] && grads[i]->defined()) step[i] += by;
     };
-    count(1);
-    const int rc = api.adamw_step(cfg, p.data(), g.data(), numel, reinterpret_cast<const double*>(lr), reinterpret_cast<const double*>(wd), step, m.mutable_data_ptr(),
-                                  v.mutable_data_ptr(), (unsigned char*)data(ms), (unsigned char*)data(vs), (float*)data(master), ws.mutable_data_ptr(),
-                                  (size_t)ws.numel(), (float*)data(norm), stream_of(m));
-    if (rc) count(-1);                                     // nothing was updated
-    check(rc, "mcrn_adamw_step");
+    call("mcrn_adamw_step", [&] {
+        count(1);
+        const int rc = api.adamw_step(cfg, p.data(), g.data(), numel, reinterpret_cast<const double*>(lr), reinterpret_cast<const double*>(wd), step,
+                                      m.mutable_data_ptr(), v.mutable_data_ptr(), (unsigned char*)data(ms), (unsigned char*)data(vs), (float*)data(master),
+                                      ws.mutable_data_ptr(), (size_t)ws.numel(), (float*)data(norm), stream_of(m));
+        if (rc) count(-1);                                 // nothing was updated
+        return rc;
+    });
     for (size_t i = 0; i < n; ++i)
         if (p[i]) changed(params[i]);
 }
@@ -257,8 +272,9 @@ std::pair<Tensor, Tensor> adamw_unpack(const Tensor& m, const Tensor& ms, const 
     const at::DeviceGuard guard(m.device());
     const Tensor om = at::empty(m.sizes(), m.options().dtype(at::kFloat)), ov = at::empty(v.sizes(), v.options().dtype(at::kFloat));
     auto bytes = [](const Tensor& t) { return (const unsigned char*)t.const_data_ptr(); };
-    check(api.adamw_unpack(bytes(m), bytes(ms), bytes(v), bytes(vs), m.numel(), (float*)om.mutable_data_ptr(), (float*)ov.mutable_data_ptr(), stream_of(m)),
-          "mcrn_adamw_unpack");
+    call("mcrn_adamw_unpack", [&] {
+        return api.adamw_unpack(bytes(m), bytes(ms), bytes(v), bytes(vs), m.numel(), (float*)om.mutable_data_ptr(), (float*)ov.mutable_data_ptr(), stream_of(m));
+    });
     return {om, ov};
 }
 

@@ -8,7 +8,7 @@ Same flags and defaults (``:158-188``), same semantics:
     (``model/utils.py:6-43``);
   * step: ``FlatTrainer.train_step`` = forward, 3-term loss on inverse-transformed tensors (``:118-125``),
     backward, ``clip_grad_norm_(max_grad_norm)``, Adam(lr, eps) (``:104,:129-130``); ``batches_seen`` drives the
-    curriculum (``:117,:127``);
+    curriculum (``:117,:127``); ``--optimizer adamw`` takes decoupled weight decay and moments of 32 or 8 bits instead;
   * epoch: ``MultiStepLR(steps, lr_decay_ratio)`` stepped per epoch (``:105,:132``), val + test evaluation every
     epoch (``:133,:139``), best-val checkpoint of ``state_dict`` (``:141-144``), early stop after ``patience`` bad
     epochs (``:146-150``), reload best and test (``:153-155``);

@@ -478,3 +478,15 @@ def test_flat_trainer_with_adamw(bits):
     for i, (p, g) in enumerate(zip(tr.params, tr._gviews)):
         want = O.adamw_step(before[i], g.double().cpu().numpy().reshape(-1), *mv[i], 2, 0.02, 0.2, eps=1e-3, factor=0.1 / (norm + 1e-6))
         assert (np.abs(p.detach().double().cpu().numpy().reshape(-1) - want[0]) <= want[3]).all(), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", ["32", "8"])
+def test_train_command_with_adamw(bits, tmp_path):
+    from megacrn_amd import train
+    np.random.seed(0); torch.manual_seed(0)
+    hist = train.main(["--synthetic", "48", "--num_nodes", "13", "--rnn_units", "16", "--mem_num", "6", "--mem_dim", "8", "--batch_size", "16",
+                       "--epochs", "2", "--seed", "0", "--save_dir", str(tmp_path), "--seq_len", "4", "--horizon", "4",
+                       "--optimizer", "adamw", "--state_bits", bits, "--weight_decay", "0.05"])
+    assert len(hist) == 2 and all(np.isfinite(v) for row in hist for v in row)
+    assert list(tmp_path.glob("*/MegaCRN.pt"))

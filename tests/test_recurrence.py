@@ -510,6 +510,48 @@ def test_two_sequences_at_once():
 
 
 @pytest.mark.gpu
+def test_two_threads():
+    """One thread trains (its backward passes run on autograd's thread, without the interpreter lock), another one serves and updates:
+    each gets what it gets alone."""
+    import threading
+    import megacrn_amd
+    gate, cand, st, keep, dout, _ = (t.cuda() for t in _inputs(2, 300, 5, 8, 8, "f32", True, 6))
+    gate.requires_grad_(), cand.requires_grad_()
+    w, g = torch.randn(500, device="cuda"), torch.randn(500, device="cuda")
+
+    def train(got):
+        for _ in range(100):
+            out, _ = megacrn_amd.gated_linear_recurrence(gate, cand, st, keep)
+            got[:] = torch.autograd.grad(out, (gate, cand), dout)
+
+    def serve(got):
+        now, p = st.clone(), w.clone()
+        opt = megacrn_amd.AdamW([p], max_grad_norm=1.0, state_bits=8)
+        for t in range(300):
+            with torch.no_grad():
+                megacrn_amd.gated_linear_recurrence_step(gate[:, t], cand[:, t], now, keep[:, t])
+            opt.step(grads=[g])
+        got[:] = [now, p]
+    alone, both, errors = [[], []], [[], []], []
+    train(alone[0]), serve(alone[1])
+
+    def guarded(f, got):
+        try:
+            f(got)
+        except Exception as e:
+            errors.append(e)
+    threads = [threading.Thread(target=guarded, args=(f, got)) for f, got in zip((train, serve), both)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    for a, b in zip(alone, both):
+        assert len(b) == 2 and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
 def test_agl_cell_training_run():
     """The module as it is used: supports -> graph convolution of all steps -> recurrence -> loss -> gradients, against float64; then
     its steps in place against the sequence, and an AdamW update of all its parameters."""
