@@ -3080,8 +3080,10 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
             ++g_launches;
         }
     }
-    // tensors [i, next) of a launch with `per` runs a block; returns its blocks
-    auto fill = [&](int& i, long long& off, AdamwT* t, int& nt, int per) {
+    // tensors [i, next) of a launch with `per` runs a block, with their coefficients if it updates; returns its blocks
+    int at = 0;
+    double bc1 = 1.0, bc2 = 1.0;
+    auto fill = [&](int& i, long long& off, AdamwT* t, int& nt, int per, bool update) {
         unsigned blocks = 0;
         nt = 0;
         for (; i < a->ntensors && nt < ADAMW_TENSORS; ++i) {
@@ -3093,12 +3095,16 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
                 e.p = params[i]; e.g = grads[i]; e.n = n; e.off = off; e.blk0 = blocks; e.id = i; e.pad = 0;
                 e.flags = (((uintptr_t)params[i] | (uintptr_t)grads[i]) % (4 * size)) == 0 ? ADAMW_VEC : 0;
                 e.key = 0; e.step_size = e.inv_bc2 = e.decay = 0.f;
-                if (!a->on_device) {
-                    const double s = step[i];
-                    e.step_size = (float)(lr[i] / (1.0 - pow(a->beta1, s)));
-                    e.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(a->beta2, s)));
+                if (update && !a->on_device) {
+                    if (step[i] != at) {                   // tensors share their step as a rule
+                        at = step[i];
+                        bc1 = 1.0 - pow(a->beta1, at);
+                        bc2 = 1.0 / sqrt(1.0 - pow(a->beta2, at));
+                    }
+                    e.step_size = (float)(lr[i] / bc1);
+                    e.inv_bc2 = (float)bc2;
                     e.decay = (float)(1.0 - lr[i] * weight_decay[i]);
-                    e.key = adamw_key(a->seed, i, (unsigned)step[i]);
+                    e.key = adamw_key(a->seed, i, (unsigned)at);
                 }
                 blocks += (unsigned)nb;
             }
@@ -3110,7 +3116,7 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
         AdamwNormP q;
         long long off = 0;
         for (int i = 0; i < a->ntensors;) {
-            const unsigned blocks = fill(i, off, q.t, q.nt, runs_n);
+            const unsigned blocks = fill(i, off, q.t, q.nt, runs_n, false);
             if (!blocks) continue;
             q.per = runs_n; q.blk0 = parts; q.part = part;
             CK(launch_adamw_norm(q, blocks, live, a->dtype, st));
@@ -3128,7 +3134,7 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     }
     long long off = 0;
     for (int i = 0; i < a->ntensors;) {
-        const unsigned blocks = fill(i, off, q.t, q.nt, runs);
+        const unsigned blocks = fill(i, off, q.t, q.nt, runs, true);
         if (!blocks) continue;
         q.per = runs; q.m = m; q.v = v; q.ms = m_scale; q.vs = v_scale; q.master = master; q.dyn = a->on_device ? dyn : nullptr;
         q.b1 = (float)a->beta1; q.c1 = (float)(1.0 - a->beta1); q.b2 = (float)a->beta2; q.c2 = (float)(1.0 - a->beta2); q.eps = (float)a->eps;
