@@ -29,21 +29,21 @@ struct GlrF32 {
     static constexpr bool FINE = true;
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
-    static __device__ __forceinline__ float inf() { return __builtin_inff(); }
+    static constexpr uint32_t INF = 0x7f800000u;           // a word of infinities
 };
 struct GlrBf16 {
     typedef __bf16 S;
     static constexpr bool FINE = false;
     static __device__ __forceinline__ float up(__bf16 v) { return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, v) << 16); }
     static __device__ __forceinline__ __bf16 down(float f) { return (__bf16)f; }     // to the nearest, ties to even, by the hardware
-    static __device__ __forceinline__ __bf16 inf() { return (__bf16)__builtin_inff(); }
+    static constexpr uint32_t INF = 0x7f807f80u;
 };
 struct GlrF16 {
     typedef _Float16 S;
     static constexpr bool FINE = false;
     static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
     static __device__ __forceinline__ _Float16 down(float f) { return (_Float16)f; }
-    static __device__ __forceinline__ _Float16 inf() { return (_Float16)__builtin_inff(); }
+    static constexpr uint32_t INF = 0x7c007c00u;
 };
 
 template <class X, int V> struct alignas(sizeof(typename X::S) * V) GlrVec { typename X::S e[V]; };
@@ -62,6 +62,18 @@ template <class X, int V> __device__ __forceinline__ GlrVec<X, V> glr_load(const
 template <int BYTES> struct GlrWord { typedef uint32_t T __attribute__((ext_vector_type(BYTES / 4))); };
 template <> struct GlrWord<4> { typedef uint32_t T; };
 template <> struct GlrWord<2> { typedef uint16_t T; };
+// r where `on`, else the pattern `other` in every word: pairs of 16-bit elements are not taken apart for it
+template <class X, int V> __device__ __forceinline__ void glr_only(bool on, GlrVec<X, V>& r, uint32_t other) {
+    typedef typename GlrWord<sizeof(r)>::T T;
+    T w = __builtin_bit_cast(T, r);
+    if constexpr (sizeof(r) > 4) {
+#pragma unroll
+        for (unsigned j = 0; j < sizeof(r) / 4; ++j) w[j] = on ? w[j] : other;
+    } else {
+        w = on ? w : (T)other;
+    }
+    r = __builtin_bit_cast(GlrVec<X, V>, w);
+}
 // NT: past the caches, for sequences larger than these
 template <class X, int V, bool NT = false> __device__ __forceinline__ void glr_store(char* base, uint32_t off, const float* v) {
     GlrVec<X, V> r;
@@ -117,11 +129,12 @@ template <bool FINE> __device__ __forceinline__ void glr_wp(float g, float& w, f
     w = g >= 0.f ? s : r;
     p = s * r;
 }
+constexpr float GLR_2L2E = 2.88539004325866699219f;        // 2 log2(e)
 // 1 - 2 / (1 + e^2u): off by 3 units of 2^-24 whatever u is, which shows relatively near 0.  FINE: Taylor's series below 1/4 (its next term is
 // 2^-26 of the value).  16-bit types: u itself below 2^-8 (off by u^2 / 3 < 2^-17 of the value, the quotient by 2^-14 above: their own steps
 // are 2^-12 and 2^-9) - 5 instructions of 39 fewer in a forward that they bound.
 template <bool FINE> __device__ __forceinline__ float glr_tanh(float u) {
-    const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + glr_exp<false>(2.f * u)), 1.f);
+    const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * GLR_2L2E)), 1.f);
     if (!FINE) return fabsf(u) < 0.00390625f ? u : far;
     const float q = u * u;
     float s = fmaf(q, 62.f / 2835.f, -17.f / 315.f);
@@ -298,10 +311,10 @@ __global__ void glr_clear_kernel(unsigned* __restrict__ words, long long tickets
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
-// Bound: bytes (gate, cand in, out out); a step takes 24 (16-bit) to 33 (f32) vector instructions and 4 transcendental ones an element, so the
+// Bound: bytes (gate, cand in, out out); a step takes 22 (16-bit) to 31 (f32) vector instructions and 4 transcendental ones an element, so the
 // 16-bit types come near the vector rate as well.  Four waves a SIMD (128 registers) hide loads and hand-overs without a second set of
 // buffers, which would halve them.  Measured (MI355X, a large copy runs at 6.2 TB/s): a week of 4 x 207 sensors, f32, 1.28 GB in 217 us = 5.9 TB/s;
-// a month of 325 sensors, bf16, 1.12 GB in 219 us = 5.1 TB/s; a window of 64 x 12 x 207, f32, 122 MB in 22 us.
+// a month of 325 sensors, bf16, 1.12 GB in 212 us = 5.3 TB/s; a window of 64 x 12 x 207, f32, 122 MB in 22 us.
 // WALK: the block walks its chunk tile by tile, from the state that the maps of the chunks before it give (one chunk: from h0).
 // AGG: only the chunk's map is wanted (agg[chunk][b][A | X][N*H]).  CHAIN: the chunk is one tile, its state comes from the block before.
 template <class X, int V, int K, int CL, bool SHARED, int MODE>
@@ -353,10 +366,8 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const bool on = ts + k < w.t1 && (!p.mask || rm[k].e[0] != 0);
-#pragma unroll
-                    for (int i = 0; i < VG; ++i) rg[k].e[i] = on ? rg[k].e[i] : X::inf();
-#pragma unroll
-                    for (int i = 0; i < V; ++i) rc[k].e[i] = on ? rc[k].e[i] : (S)0.f;
+                    glr_only<X, VG>(on, rg[k], X::INF);
+                    glr_only<X, V>(on, rc[k], 0u);
                 }
             }
 #pragma unroll
@@ -372,6 +383,11 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
 #pragma unroll
                     for (int i = 0; i < V; ++i) cc[k][i] = glr_tanh<X::FINE>(cc[k][i]);
             }
+        } else if (SEG > 1) {                              // its map is the identity (a branch around the maps would cost a copy of each)
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) ww[k][i] = cc[k][i] = 0.f;
         }
         GLR_PHASE();
         pg += span * p.g_st * es;
@@ -384,9 +400,8 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
             for (int i = 0; i < V; ++i) {
                 A[i] = 1.f; Xl[i] = 0.f;
             }
-            if (live) {
 #pragma unroll
-                for (int i = 0; i < V; ++i)
+            for (int i = 0; i < V; ++i)
 #pragma unroll
                 for (int k = 0; k < K; ++k) {              // from here on ww, cc hold the maps up to each step
                     A[i] = fmaf(-ww[k][i], A[i], A[i]);
@@ -394,7 +409,6 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
                     ww[k][i] = A[i];
                     cc[k][i] = Xl[i];
                 }
-            }
             float EA[V], EX[V];
             glr_scan_maps<V, CL, REV>(lds[par], w.cl, A, Xl, EA, EX);
             if (CHAIN && w.chunk > 0 && w.active) glr_receive<V>(p.carry + ((long long)(w.chunk - 1) * p.B + w.b) * NH + hoff, carry);
@@ -527,13 +541,9 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const bool in = ts + k < w.t1, on = in && (!p.mask || rm[k].e[0] != 0);
-#pragma unroll
-                    for (int i = 0; i < VG; ++i) rg[k].e[i] = on ? rg[k].e[i] : X::inf();
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        if (!AGG) rc[k].e[i] = on ? rc[k].e[i] : (S)0.f;
-                        rd[k].e[i] = in ? rd[k].e[i] : (S)0.f;
-                    }
+                    glr_only<X, VG>(on, rg[k], X::INF);
+                    if (!AGG) glr_only<X, V>(on, rc[k], 0u);
+                    glr_only<X, V>(in, rd[k], 0u);
                 }
             }
             if (!AGG) {
