@@ -2945,7 +2945,7 @@ size_t mcrn_glr_workspace_bytes(const mcrn_glr_t* d, int backward) {
     GlrP p;
     if (!glr_params(d, p) || (long long)p.B * p.N == 0) return 0;
     size_t most = 0;
-    for (p.one = 0; p.one < 2; ++p.one)        // the alignment of the pointers decides between the two
+    for (p.one = 0; p.one < 2; ++p.one)        // the call's pointers decide between the two
         if (glr_plan(p, backward != 0)) most = std::max(most, glr_ws_bytes(p, backward != 0));
     return most;
 }

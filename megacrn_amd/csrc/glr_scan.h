@@ -30,6 +30,7 @@ struct GlrF32 {
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
     static constexpr uint32_t INF = 0x7f800000u;           // a word of infinities
+    static __device__ __forceinline__ float inf() { return __builtin_inff(); }
 };
 struct GlrBf16 {
     typedef __bf16 S;
@@ -37,6 +38,7 @@ struct GlrBf16 {
     static __device__ __forceinline__ float up(__bf16 v) { return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, v) << 16); }
     static __device__ __forceinline__ __bf16 down(float f) { return (__bf16)f; }     // to the nearest, ties to even, by the hardware
     static constexpr uint32_t INF = 0x7f807f80u;
+    static __device__ __forceinline__ __bf16 inf() { return (__bf16)__builtin_inff(); }
 };
 struct GlrF16 {
     typedef _Float16 S;
@@ -44,9 +46,11 @@ struct GlrF16 {
     static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
     static __device__ __forceinline__ _Float16 down(float f) { return (_Float16)f; }
     static constexpr uint32_t INF = 0x7c007c00u;
+    static __device__ __forceinline__ _Float16 inf() { return (_Float16)__builtin_inff(); }
 };
 
-template <class X, int V> struct alignas(sizeof(typename X::S) * V) GlrVec { typename X::S e[V]; };
+// aligned to its elements only (global memory takes any alignment): what rows of any length need
+template <class X, int V> struct GlrVec { typename X::S e[V]; };
 
 // element i; a pair of bf16 is taken apart in its 32-bit word
 template <class X, int V> __device__ __forceinline__ float glr_up(const GlrVec<X, V>& r, int i) { return X::up(r.e[i]); }
@@ -80,7 +84,8 @@ template <class X, int V, bool NT = false> __device__ __forceinline__ void glr_s
 #pragma unroll
     for (int i = 0; i < V; ++i) r.e[i] = X::down(v[i]);
     typedef typename GlrWord<sizeof(r)>::T T;
-    if (NT) __builtin_nontemporal_store(__builtin_bit_cast(T, r), reinterpret_cast<T*>(base + off));
+    typedef T Loose __attribute__((aligned(sizeof(typename X::S))));
+    if (NT) __builtin_nontemporal_store(__builtin_bit_cast(T, r), reinterpret_cast<Loose*>(base + off));
     else *reinterpret_cast<GlrVec<X, V>*>(base + off) = r;
 }
 struct GlrYes { static constexpr bool value = true; };
@@ -151,12 +156,13 @@ __device__ __forceinline__ float glr_next(float w, float c, float h) { return fm
 struct GlrAt {
     int b, chunk, cl, seg, t0, t1;
     int n, ch;                 // node and first channel of the thread's V channels
+    int n2;                    // node of the last one (FLAT)
     int gi, gl, part;          // its gate's index in (.., G), its lane among the gate's lanes, its part
     bool active;
 };
 // CHAIN: the chunk is the next one of the block's channels that no block has taken yet, so that the block which has to hand over the
 // state has started before; REV: from the last chunk on
-template <int V, int CL, bool SHARED, bool CHAIN, bool REV> __device__ __forceinline__ GlrAt glr_where(const GlrP& p) {
+template <int V, int CL, int GATES, bool CHAIN, bool REV> __device__ __forceinline__ GlrAt glr_where(const GlrP& p) {
     GlrAt w;
     unsigned blk = blockIdx.x;
     const unsigned tile = blk % (unsigned)p.tiles;
@@ -167,7 +173,7 @@ template <int V, int CL, bool SHARED, bool CHAIN, bool REV> __device__ __forcein
     if (CHAIN && threadIdx.x == 0) mine = (int)atomicAdd(p.ticket + (tile + (unsigned)w.b * (unsigned)p.tiles), 1u);
     w.cl = (int)threadIdx.x % CL;
     w.seg = (int)threadIdx.x / CL;
-    if (SHARED) {              // L lanes a (gate, part): channels behind the gate's last stay idle
+    if (GATES == GLR_SHARED) { // L lanes a (gate, part): channels behind the gate's last stay idle
         const unsigned unit = tile * (unsigned)(CL / p.L) + w.cl / p.L;
         const int D = p.H / p.G;
         w.gl = w.cl % p.L;
@@ -178,6 +184,16 @@ template <int V, int CL, bool SHARED, bool CHAIN, bool REV> __device__ __forcein
         w.n = w.active ? (int)(ng / (unsigned)p.G) : 0;
         w.gi = w.active ? (int)(ng % (unsigned)p.G) : 0;
         w.ch = w.active ? w.gi * D + d : 0;
+    } else if (GATES == GLR_FLAT) {      // channels of all nodes behind one another; the last vector reaches back over the one before
+        const unsigned q = tile * CL + w.cl, NH = (unsigned)p.N * (unsigned)p.H;
+        w.active = q < (unsigned)p.nq;
+        const unsigned c = w.active ? min(q * V, NH - V) : 0u;
+        w.n = (int)(c / (unsigned)p.H);
+        w.ch = (int)(c % (unsigned)p.H);
+        w.n2 = w.ch + V > p.H ? w.n + 1 : w.n;
+        w.gi = w.ch;
+        w.gl = 0;
+        w.part = 0;
     } else {
         const unsigned q = tile * CL + w.cl, hv = p.H / V;
         w.active = q < (unsigned)p.nq;
@@ -317,13 +333,13 @@ __global__ void glr_clear_kernel(unsigned* __restrict__ words, long long tickets
 // a month of 325 sensors, bf16, 1.12 GB in 212 us = 5.3 TB/s; a window of 64 x 12 x 207, f32, 122 MB in 22 us.
 // WALK: the block walks its chunk tile by tile, from the state that the maps of the chunks before it give (one chunk: from h0).
 // AGG: only the chunk's map is wanted (agg[chunk][b][A | X][N*H]).  CHAIN: the chunk is one tile, its state comes from the block before.
-template <class X, int V, int K, int CL, bool SHARED, int MODE>
-__global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) void glr_fwd_kernel(GlrP p) {
-    constexpr bool AGG = MODE == GLR_AGG, CHAIN = MODE == GLR_CHAIN, REV = false;
+template <class X, int V, int K, int CL, int GATES, int MODE>
+__global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GATES == GLR_FLAT && X::FINE) ? 3 : 4) void glr_fwd_kernel(GlrP p) {
+    constexpr bool SHARED = GATES == GLR_SHARED, FLAT = GATES == GLR_FLAT, AGG = MODE == GLR_AGG, CHAIN = MODE == GLR_CHAIN, REV = false;
     constexpr int SEG = GLR_THREADS / CL, VG = SHARED ? 1 : V, W = GLR_THREADS / 64, span = SEG * K;
     typedef typename X::S S;
     __shared__ float2 lds[SEG > 1 ? 2 : 1][SEG > 1 ? W * CL * V : 1];
-    const GlrAt w = glr_where<V, CL, SHARED, CHAIN, REV>(p);
+    const GlrAt w = glr_where<V, CL, GATES, CHAIN, REV>(p);
     const long long NH = (long long)p.N * p.H, hoff = (long long)w.n * p.H + w.ch;
     const long long es = sizeof(S), rb = NH * es;          // bytes of an element, of a row of out
     const char* pg = static_cast<const char*>(p.gate) + (w.b * p.g_sb + w.t0 * p.g_st) * es;
@@ -357,17 +373,28 @@ __global__ __launch_bounds__(GLR_THREADS, MODE == GLR_WALK && CL < 256 ? 3 : 4) 
         if (live) {
             GlrVec<X, VG> rg[K];
             GlrVec<X, V> rc[K];
-            GlrVec<GlrByte, 1> rm[K];
+            GlrVec<GlrByte, 1> rm[K], rn[FLAT ? K : 1];    // (FLAT: of the last channel's node)
             const int end = w.t1 - 1 - tb;
             glr_rows<X, VG, K, CHAIN>(rg, pg, lg, (uint32_t)(p.g_st * es), w.seg, full, end);
             glr_rows<X, V, K, CHAIN>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
             if (p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
+            if (FLAT && p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rn, pm, (uint32_t)(w.n2 * p.m_sn), (uint32_t)p.m_st, w.seg, full, end);
             if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give w = 0, c = 0
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-                    const bool on = ts + k < w.t1 && (!p.mask || rm[k].e[0] != 0);
-                    glr_only<X, VG>(on, rg[k], X::INF);
-                    glr_only<X, V>(on, rc[k], 0u);
+                    const bool in = ts + k < w.t1, on = in && (!p.mask || rm[k].e[0] != 0);
+                    if (FLAT && p.mask) {
+                        const bool on2 = in && rn[k].e[0] != 0;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            const bool o = w.ch + i < p.H ? on : on2;
+                            rg[k].e[i] = o ? rg[k].e[i] : X::inf();
+                            rc[k].e[i] = o ? rc[k].e[i] : (S)0.f;
+                        }
+                    } else {
+                        glr_only<X, VG>(on, rg[k], X::INF);
+                        glr_only<X, V>(on, rc[k], 0u);
+                    }
                 }
             }
 #pragma unroll
@@ -479,13 +506,13 @@ __device__ __forceinline__ float glr_lane_sum(float s, int L) {
 // registers between the scan and the second run (a third wave would spill 30 bytes a lane).  Measured: the week above 2.19 GB in 395 us = 5.6 TB/s,
 // the window 208 MB in 36 us = 5.8 TB/s.
 // Walks the time axis from its end; `carry` is mu_{t+1} = a_{t+1} lam_{t+1}, what reaches step t from the steps behind it.
-template <class X, int V, int K, int CL, bool SHARED, int MODE>
+template <class X, int V, int K, int CL, int GATES, int MODE>
 __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
-    constexpr bool AGG = MODE == GLR_AGG, CHAIN = MODE == GLR_CHAIN, REV = true;
+    constexpr bool SHARED = GATES == GLR_SHARED, FLAT = GATES == GLR_FLAT, AGG = MODE == GLR_AGG, CHAIN = MODE == GLR_CHAIN, REV = true;
     constexpr int SEG = GLR_THREADS / CL, VG = SHARED ? 1 : V, W = GLR_THREADS / 64, span = SEG * K;
     typedef typename X::S S;
     __shared__ float2 lds[SEG > 1 ? 2 : 1][SEG > 1 ? W * CL * V : 1];
-    const GlrAt w = glr_where<V, CL, SHARED, CHAIN, REV>(p);
+    const GlrAt w = glr_where<V, CL, GATES, CHAIN, REV>(p);
     const long long NH = (long long)p.N * p.H, NG = (long long)p.N * p.G, hoff = (long long)w.n * p.H + w.ch, nck = (p.T - 1) / K;
     const long long es = sizeof(S), rb = NH * es, gb = NG * es;
     const int ntile = (w.t1 - w.t0 + span - 1) / span, tl = w.t0 + (ntile - 1) * span;      // tiles, first step of the last one
@@ -524,7 +551,7 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
             GlrVec<X, VG> rg[K];
             GlrVec<X, V> rc[K], rd[K];
             GlrVec<GlrF32, V> rs;                          // the state before the segment's first step
-            GlrVec<GlrByte, 1> rm[K];
+            GlrVec<GlrByte, 1> rm[K], rn[FLAT ? K : 1];    // (FLAT: of the last channel's node)
             const int end = w.t1 - 1 - tb;
             glr_rows<X, VG, K, CHAIN>(rg, pg, lg, (uint32_t)(p.g_st * es), w.seg, full, end);
             if (!AGG) glr_rows<X, V, K, CHAIN>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
@@ -537,12 +564,23 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                     for (int i = 0; i < V; ++i) rd[k].e[i] = (S)0.f;
             }
             if (p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
+            if (FLAT && p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rn, pm, (uint32_t)(w.n2 * p.m_sn), (uint32_t)p.m_st, w.seg, full, end);
             if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give w = p = 0, c = 0
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const bool in = ts + k < w.t1, on = in && (!p.mask || rm[k].e[0] != 0);
-                    glr_only<X, VG>(on, rg[k], X::INF);
-                    if (!AGG) glr_only<X, V>(on, rc[k], 0u);
+                    if (FLAT && p.mask) {
+                        const bool on2 = in && rn[k].e[0] != 0;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            const bool o = w.ch + i < p.H ? on : on2;
+                            rg[k].e[i] = o ? rg[k].e[i] : X::inf();
+                            if (!AGG) rc[k].e[i] = o ? rc[k].e[i] : (S)0.f;
+                        }
+                    } else {
+                        glr_only<X, VG>(on, rg[k], X::INF);
+                        if (!AGG) glr_only<X, V>(on, rc[k], 0u);
+                    }
                     glr_only<X, V>(in, rd[k], 0u);
                 }
             }

@@ -8,6 +8,7 @@
 namespace mcrn {
 
 enum { GLR_F32 = 0, GLR_BF16 = 1, GLR_F16 = 2 };
+enum { GLR_OWN = 0, GLR_SHARED = 1, GLR_FLAT = 2 };
 
 // h_t = a_t h_{t-1} + (1 - a_t) phi(cand_t), a_t = sigmoid(gate_t); a step whose mask byte is 0 keeps the state.
 // gate (B,T,N,G), cand (B,T,N,H), D = H / G channels share a gate; strides in elements, the last dimension is contiguous.
@@ -29,7 +30,8 @@ struct GlrP {
     void *dgate, *dcand;                    // (B,T,N,G), (B,T,N,H) contiguous
     float* dstate;                          // (B,N,H) or NULL = not wanted
     // plan (glr_plan)
-    int one;                                // not 0: plan for one channel a thread, whatever the alignment
+    int one;                                // not 0: plan without GLR_FLAT
+    int gates;                              // GLR_OWN: channels of a node; GLR_SHARED: G < H; GLR_FLAT: channels of all nodes behind one another
     int V, K, CL, S, L, parts;              // channels and steps a thread, channel lanes a block, chunks of the time axis,
     int chunk, first;                       // lanes and parts of a shared gate's channels; steps a chunk, first chunk of the launch
     long long nq, tiles;                    // channel vectors of a batch entry, blocks that cover them

@@ -14,18 +14,17 @@ bool glr_plan(GlrP& p, bool backward) {
     const size_t size = p.dtype == GLR_F32 ? 4 : 2;
     const int D = p.H / p.G;
     const bool shared = D > 1;
-    // Four channels a thread (16 bytes of f32, 8 of the 16-bit types) where rows and pointers allow it, else one.
-    auto fits = [&](const void* q, long long a, long long b, long long c) {
-        return !q || (((uintptr_t)q % (4 * size)) == 0 && a % 4 == 0 && b % 4 == 0 && c % 4 == 0);
-    };
-    auto fits32 = [](const void* q) { return ((uintptr_t)q & 15) == 0; };
-    p.V = D % 4 == 0 || !shared ? 4 : 1;
-    if (p.H % 4 || !fits(p.cand, p.c_sb, p.c_st, p.c_sn) || !fits(p.out, 0, 0, 0) || (!shared && !fits(p.gate, p.g_sb, p.g_st, p.g_sn)) ||
-        !fits32(p.ckpt) || !fits32(p.h0))
-        p.V = 1;
-    if (p.one) p.V = 1;
-    if (backward && (!fits(p.dout, p.d_sb, p.d_st, p.d_sn) || !fits(p.dcand, 0, 0, 0) || (!shared && !fits(p.dgate, 0, 0, 0)))) p.V = 1;
-    p.nq = (long long)p.N * (p.H / p.V);
+    // Four channels a thread (16 bytes of f32, 8 of the 16-bit types), at any alignment.  A number of channels that 4 does not divide: vectors run
+    // over the ends of the nodes where these lie behind one another (FLAT), else one channel a thread (3 x 3110 x 206 x 37, f32, both
+    // directions: 906 us so, 606 flat; 11 x 666 x 229 x 42, bf16, forward: 257 : 133).  FLAT's last vector reaches back over channels of the one
+    // before: not while `last` overwrites the state that both read.
+    const long long NH = (long long)p.N * p.H;
+    auto dense = [&](long long sn) { return p.N == 1 || sn == p.H; };
+    const bool flat = !shared && p.H % 4 && p.H >= 3 && NH >= 4 && NH < (1ll << 31) && !p.one && dense(p.g_sn) && dense(p.c_sn) &&
+                      !(p.last && p.last == p.h0) && !(backward && p.dout && !dense(p.d_sn));
+    p.gates = shared ? GLR_SHARED : flat ? GLR_FLAT : GLR_OWN;
+    p.V = flat || (shared ? D : p.H) % 4 == 0 ? 4 : 1;
+    p.nq = flat ? up_div(NH, 4) : (long long)p.N * (p.H / p.V);
     auto cover = [&](int CL) {
         p.CL = CL;
         if (shared) {
@@ -54,15 +53,15 @@ bool glr_plan(GlrP& p, bool backward) {
         // From here on fewer than 512 blocks of 256 channel lanes: time is cut over the lanes of a block as well.
         //  - 64 lanes x 4 segments: up to 32 steps, and where more than a quarter of the 16-lane form's waves would idle behind the last step
         //    (144 steps: 26 us forward against 36; 48 steps: 28 against 35), if that still makes a block for every compute unit.
-        //  - 16 lanes x 16 segments, a block for every 128 steps, each handing its state to the next (chain), from 64 blocks a chunk on: a hand-over
-        //    takes 1.6 us, so that many chunks of few channels wait (20161 steps: 128 tiles 484 us against 672 split, 64 tiles 321 : 351,
-        //    32 tiles 265 : 185).
+        //  - 16 lanes x 16 segments, a block for every 128 steps, each handing its state to the next (chain), while a chunk of all blocks holds
+        //    about as much as the card reads during a hand-over (1.6 us): 64 blocks of 16 bytes a lane and step (f32, 20161 steps: 128 tiles 484 us
+        //    against 672 split, 64 tiles 321 : 351, 32 tiles 265 : 185), more of fewer bytes (f16, 14362 steps, 96 tiles, both directions: 469 : 448 split).
         //  - fewer: the chunks' maps first (they need no state), then every chunk from the maps before it.  Inputs are read twice.
         const int quarter = GLR_THREADS / 64 * GLR_K;
         const bool loose = up_div(p.T, quarter) < 3 * up_div(p.T, span);
         if (p.T <= quarter || (loose && cover(64) >= 256)) {
             cover(64);
-        } else if ((blocks = cover(16)) >= 64 && p.T > span) {
+        } else if ((blocks = cover(16)) * p.V * (long long)size >= 64 * 16 && p.T > span) {
             p.chain = true;
             p.chunk = span;
             p.S = (int)up_div(p.T, span);
@@ -94,7 +93,7 @@ void glr_place(GlrP& p, void* ws) {
     p.part = (float*)((char*)ws + head_bytes(p));
 }
 
-template <class X, int V, int K, int CL, bool SHARED> static hipError_t run(const GlrP& p0, bool backward, hipStream_t st, int* launches) {
+template <class X, int V, int K, int CL, int GATES> static hipError_t run(const GlrP& p0, bool backward, hipStream_t st, int* launches) {
     GlrP p = p0;
     const unsigned one = (unsigned)(p.tiles * p.B);
     const dim3 block(GLR_THREADS);
@@ -102,19 +101,19 @@ template <class X, int V, int K, int CL, bool SHARED> static hipError_t run(cons
     if (CL == 16 && p.chain) {
         const long long words = (long long)chain_words(p);
         hipLaunchKernelGGL(glr_clear_kernel, dim3((unsigned)up_div(words, 256)), dim3(256), 0, st, p.ticket, p.tiles * p.B, words);
-        if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, GLR_K, 16, SHARED, GLR_CHAIN>), dim3(one * p.S), block, 0, st, p);
-        else hipLaunchKernelGGL((glr_fwd_kernel<X, V, GLR_K, 16, SHARED, GLR_CHAIN>), dim3(one * p.S), block, 0, st, p);
+        if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, GLR_K, 16, GATES, GLR_CHAIN>), dim3(one * p.S), block, 0, st, p);
+        else hipLaunchKernelGGL((glr_fwd_kernel<X, V, GLR_K, 16, GATES, GLR_CHAIN>), dim3(one * p.S), block, 0, st, p);
         ++*launches;
     } else {
         if (CL == 16 && p.S > 1) {                        // maps of the chunks that others start from
             p.first = backward ? 1 : 0;
-            if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, GLR_K, 16, SHARED, GLR_AGG>), dim3(one * (p.S - 1)), block, 0, st, p);
-            else hipLaunchKernelGGL((glr_fwd_kernel<X, V, GLR_K, 16, SHARED, GLR_AGG>), dim3(one * (p.S - 1)), block, 0, st, p);
+            if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, GLR_K, 16, GATES, GLR_AGG>), dim3(one * (p.S - 1)), block, 0, st, p);
+            else hipLaunchKernelGGL((glr_fwd_kernel<X, V, GLR_K, 16, GATES, GLR_AGG>), dim3(one * (p.S - 1)), block, 0, st, p);
             p.first = 0;
             ++*launches;
         }
-        if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, K, CL, SHARED, GLR_WALK>), dim3(one * p.S), block, 0, st, p);
-        else hipLaunchKernelGGL((glr_fwd_kernel<X, V, K, CL, SHARED, GLR_WALK>), dim3(one * p.S), block, 0, st, p);
+        if (backward) hipLaunchKernelGGL((glr_bwd_kernel<X, V, K, CL, GATES, GLR_WALK>), dim3(one * p.S), block, 0, st, p);
+        else hipLaunchKernelGGL((glr_fwd_kernel<X, V, K, CL, GATES, GLR_WALK>), dim3(one * p.S), block, 0, st, p);
     }
     ++*launches;
     if (backward && p.parts > 1) {
@@ -125,16 +124,17 @@ template <class X, int V, int K, int CL, bool SHARED> static hipError_t run(cons
     return hipGetLastError();
 }
 
-template <class X, int V, bool SHARED> static hipError_t run_v(const GlrP& p, bool backward, hipStream_t st, int* launches) {
-    if (p.K == 1) return run<X, V, 1, 256, SHARED>(p, backward, st, launches);
-    if (p.K == 4) return run<X, V, 4, 256, SHARED>(p, backward, st, launches);
-    if (p.CL == 256) return run<X, V, GLR_K, 256, SHARED>(p, backward, st, launches);
-    if (p.CL == 64) return run<X, V, GLR_K, 64, SHARED>(p, backward, st, launches);
-    return run<X, V, GLR_K, 16, SHARED>(p, backward, st, launches);
+template <class X, int V, int GATES> static hipError_t run_v(const GlrP& p, bool backward, hipStream_t st, int* launches) {
+    if (p.K == 1) return run<X, V, 1, 256, GATES>(p, backward, st, launches);
+    if (p.K == 4) return run<X, V, 4, 256, GATES>(p, backward, st, launches);
+    if (p.CL == 256) return run<X, V, GLR_K, 256, GATES>(p, backward, st, launches);
+    if (p.CL == 64) return run<X, V, GLR_K, 64, GATES>(p, backward, st, launches);
+    return run<X, V, GLR_K, 16, GATES>(p, backward, st, launches);
 }
 template <class X> static hipError_t run_x(const GlrP& p, bool backward, hipStream_t st, int* launches) {
-    if (p.G != p.H) return p.V == 4 ? run_v<X, 4, true>(p, backward, st, launches) : run_v<X, 1, true>(p, backward, st, launches);
-    return p.V == 4 ? run_v<X, 4, false>(p, backward, st, launches) : run_v<X, 1, false>(p, backward, st, launches);
+    if (p.gates == GLR_SHARED) return p.V == 4 ? run_v<X, 4, GLR_SHARED>(p, backward, st, launches) : run_v<X, 1, GLR_SHARED>(p, backward, st, launches);
+    if (p.gates == GLR_FLAT) return run_v<X, 4, GLR_FLAT>(p, backward, st, launches);
+    return p.V == 4 ? run_v<X, 4, GLR_OWN>(p, backward, st, launches) : run_v<X, 1, GLR_OWN>(p, backward, st, launches);
 }
 static hipError_t launch(const GlrP& p, bool backward, hipStream_t st, int* launches) {
     if (p.dtype == GLR_F32) return run_x<GlrF32>(p, backward, st, launches);

@@ -179,7 +179,7 @@ def test_against_oracle(B, T, N, H, G, dt, act):
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,T,N,H,G,dt,family", [
     (1, 2100, 1, 33, 33, "f32", "split"), (2, 2051, 3, 16, 4, "bf16", "split"), (1, 4100, 2, 8, 1, "f16", "split"), (1, 1025, 1, 260, 1, "f32", "split"),
-    (32, 20, 64, 63, 63, "f32", "stream"), (33, 20, 64, 65, 5, "bf16", "stream"), (64, 1, 17, 64, 64, "f16", "stream"),
+    (32, 20, 64, 63, 63, "f32", "tile"), (64, 13, 130, 63, 63, "f32", "stream"), (33, 20, 64, 65, 5, "bf16", "stream"), (64, 1, 17, 64, 64, "f16", "stream"),
     (8, 12, 100, 64, 64, "f32", "stream"), (8, 14, 100, 64, 64, "f32", "tile"), (1, 500, 30, 64, 64, "f32", "split"), (8, 150, 100, 64, 1, "bf16", "chain"), (16, 200, 64, 64, 64, "f32", "chain"),
     (8, 120, 100, 64, 16, "f16", "tile"), (2, 1000, 300, 63, 63, "f32", "chain"), (1, 1280, 300, 65, 13, "bf16", "chain"),
 ])
@@ -190,6 +190,28 @@ def test_every_variant(B, T, N, H, G, dt, family):
     _against_oracle(*_inputs(B, T, N, H, G, dt, T % 2 == 1, T + H, state=T % 3 != 0), "tanh", dt)
     seen = {k for k, v in _lib.launch_histogram().items() if k.startswith("glr:") and v}
     assert seen == {f"glr:fwd_{family}", f"glr:bwd_{family}"}, seen
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,N,H", [(1, 1, 2, 3), (2, 5, 2, 3), (2, 40, 1, 5), (3, 9, 7, 37), (1, 17, 1, 6), (1, 300, 5, 42), (2, 2100, 3, 9), (2, 260, 150, 33), (1, 700, 130, 106)])
+def test_vectors_over_the_ends_of_nodes(B, T, N, H, dt):
+    """Channels that 4 does not divide: four neighbours may belong to two nodes, whose masks differ."""
+    _against_oracle(*_inputs(B, T, N, H, H, dt, True, B + T + H), "tanh", dt)
+
+
+@pytest.mark.gpu
+def test_vectors_over_the_ends_of_nodes_past_the_caches():
+    import megacrn_amd
+    T, N, H = 4200, 484, 33
+    g = torch.Generator(device="cuda").manual_seed(1)
+    gate, cand = (torch.randn(1, T, N, H, generator=g, device="cuda") for _ in range(2))
+    keep = torch.rand(1, T, N, generator=g, device="cuda") > 0.2
+    out, last = megacrn_amd.gated_linear_recurrence(gate, cand, None, keep)
+    pick = [0, 1, 241, N - 1]
+    want, wlast, eh, _ = O.glr_fwd(*(t[:, :, pick].double().cpu().numpy() for t in (gate, cand)), None, keep[:, :, pick].cpu().numpy())
+    _close(out[:, :, pick], want, eh + O.half_step(want, "f32"), "out")
+    _close(last[:, pick], wlast, eh[:, -1] + O.half_step(wlast, "f32"), "last")
 
 
 @pytest.mark.gpu
@@ -463,7 +485,8 @@ def _c_forward(gate, cand, state, out, last, ws=0, **over):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,T,N,H", [(2, 0, 3, 8), (1, 3000, 1, 12), (1, 700, 80, 64), (3, 5, 2, 8), (1, 100, 3, 8)])
+@pytest.mark.parametrize("B,T,N,H", [(2, 0, 3, 8), (1, 3000, 1, 12), (1, 700, 80, 64), (3, 5, 2, 8), (1, 100, 3, 8),
+                                     (1, 1, 9, 33), (2, 5, 3, 7), (1, 100, 3, 9), (1, 3000, 1, 13)])
 def test_c_entry_in_place_and_without_outputs(B, T, N, H):
     """The state advanced in place over a whole sequence, with no `out`, in every variant (a split would read what it overwrites: not planned)."""
     import megacrn_amd
