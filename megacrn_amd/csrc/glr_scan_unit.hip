@@ -51,15 +51,15 @@ bool glr_plan(GlrP& p, bool backward) {
     if (p.T > GLR_K && p.K == GLR_K && blocks < 512) {
         const int span = GLR_THREADS / 16 * GLR_K;
         // From here on fewer than 512 blocks of 256 channel lanes: time is cut over the lanes of a block as well.
-        //  - 64 lanes x 4 segments: up to 32 steps, and where more than a quarter of the 16-lane form's waves would idle behind the last step
-        //    (144 steps: 26 us forward against 36; 48 steps: 28 against 35), if that still makes a block for every compute unit.
+        //  - 64 lanes x 4 segments, the block walking its tiles: up to 32 steps, and up to 288 where that still makes 400 blocks (462 blocks, 144 steps: 26 us
+        //    forward against 36; 416, 120 steps, bf16 with gradients: 51 : 63; 1131, 162 steps: 78 : 109).  Fewer blocks leave the card idle
+        //    (260, 100 steps: 31 : 26), longer walks lose to chained tiles (675, 1000 steps with gradients: 853 : 722).
         //  - 16 lanes x 16 segments, a block for every 128 steps, each handing its state to the next (chain), while a chunk of all blocks holds
         //    about as much as the card reads during a hand-over (1.6 us): 64 blocks of 16 bytes a lane and step (f32, 20161 steps: 128 tiles 484 us
         //    against 672 split, 64 tiles 321 : 351, 32 tiles 265 : 185), more of fewer bytes (f16, 14362 steps, 96 tiles, both directions: 469 : 448 split).
         //  - fewer: the chunks' maps first (they need no state), then every chunk from the maps before it.  Inputs are read twice.
         const int quarter = GLR_THREADS / 64 * GLR_K;
-        const bool loose = up_div(p.T, quarter) < 3 * up_div(p.T, span);
-        if (p.T <= quarter || (loose && cover(64) >= 256)) {
+        if (p.T <= quarter || (p.T <= 9 * quarter && cover(64) >= 400)) {
             cover(64);
         } else if ((blocks = cover(16)) * p.V * (long long)size >= 64 * 16 && p.T > span) {
             p.chain = true;

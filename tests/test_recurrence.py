@@ -181,6 +181,7 @@ def test_against_oracle(B, T, N, H, G, dt, act):
     (1, 2100, 1, 33, 33, "f32", "split"), (2, 2051, 3, 16, 4, "bf16", "split"), (1, 4100, 2, 8, 1, "f16", "split"), (1, 1025, 1, 260, 1, "f32", "split"),
     (32, 20, 64, 63, 63, "f32", "tile"), (64, 13, 130, 63, 63, "f32", "stream"), (33, 20, 64, 65, 5, "bf16", "stream"), (64, 1, 17, 64, 64, "f16", "stream"),
     (8, 12, 100, 64, 64, "f32", "stream"), (8, 14, 100, 64, 64, "f32", "tile"), (1, 500, 30, 64, 64, "f32", "split"), (8, 150, 100, 64, 1, "bf16", "chain"), (16, 200, 64, 64, 64, "f32", "chain"),
+    (16, 200, 104, 64, 1, "bf16", "tile"), (17, 99, 100, 64, 64, "f32", "tile"),
     (8, 120, 100, 64, 16, "f16", "tile"), (2, 1000, 300, 63, 63, "f32", "chain"), (1, 1280, 300, 65, 13, "bf16", "chain"),
 ])
 def test_every_variant(B, T, N, H, G, dt, family):
