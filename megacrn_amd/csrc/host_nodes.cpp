@@ -59,6 +59,10 @@ void need_gpu(const Tensor& t, const char* who) {
 void changed(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+// The kernels write through pointers, so torch sees no operation that could carry a tangent: a dual tensor is refused, not taken as a constant
+void no_tangent(const Tensor& t, const char* who) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), who, " is differentiable in reverse mode only: an input carries a forward gradient (torch.autograd.forward_ad)");
+}
 int type_of(at::ScalarType t) { return t == at::kFloat ? MCRN_T_F32 : t == at::kBFloat16 ? MCRN_T_BF16 : t == at::kHalf ? MCRN_T_F16 : -1; }
 
 // ---- gated linear recurrence -------------------------------------------------------------------------------------------
@@ -91,6 +95,7 @@ Tensor check_inputs(const Tensor& gate, const Tensor& cand, const Tensor& state,
         TORCH_CHECK_VALUE(fits, who, ": mask must be ", cand.sizes().slice(0, lead), ", with 1 where all share an entry, or lack its last dimension; got ", mask.sizes());
         m = m.expand(cand.sizes().slice(0, lead));
     }
+    for (const Tensor* t : {&gate, &cand, &state}) no_tangent(*t, who);
     need_gpu(cand, who);
     return m;
 }
@@ -244,6 +249,8 @@ void adamw_step(uintptr_t cfg_at, const std::vector<Tensor>& params, const std::
                           " is no longer the contiguous ", type, " tensor that the optimizer was made for");
         TORCH_CHECK_VALUE(b.scalar_type() == type && b.device() == dev && b.layout() == at::kStrided && b.sizes() == a.sizes(), "AdamW.step: gradient ", i,
                           " must be a ", type, " tensor of shape ", a.sizes(), " on ", dev);
+        no_tangent(a, "AdamW.step");
+        no_tangent(b, "AdamW.step");
         p[i] = a.mutable_data_ptr();
         if (b.is_contiguous()) g[i] = b.const_data_ptr();
         else g[i] = held.emplace_back(b.contiguous()).const_data_ptr();

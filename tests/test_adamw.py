@@ -354,6 +354,18 @@ def test_grad_attribute_views_and_errors():
 
 
 @pytest.mark.gpu
+def test_dual_tensors_are_refused():
+    import megacrn_amd
+    from torch.autograd import forward_ad
+    p, g = torch.ones(5, device="cuda"), torch.ones(5, device="cuda")
+    opt = megacrn_amd.AdamW([p])
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward gradient"):
+            opt.step(grads=[forward_ad.make_dual(g, torch.ones_like(g))])
+    assert opt.steps() == [0] and (p == 1).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("bits", [32, 8])
 def test_resumed_and_captured_runs(bits, dt):

@@ -82,6 +82,22 @@ def test_step_refusals(over, kind):
         megacrn_amd.gated_linear_recurrence_step(**a)
 
 
+@pytest.mark.parametrize("which", ["gate", "cand", "state"])
+@pytest.mark.parametrize("where", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_dual_tensors_are_refused(which, where):
+    """A forward-mode tangent is not dropped: the sequence and the step raise, and the step leaves its state alone."""
+    import megacrn_amd
+    from torch.autograd import forward_ad
+    for f, a in ((megacrn_amd.gated_linear_recurrence, _cpu(mask=None)),
+                 (megacrn_amd.gated_linear_recurrence_step, dict(gate=torch.zeros(2, 4, 8), cand=torch.ones(2, 4, 8), state=torch.ones(2, 4, 8)))):
+        a = {k: None if t is None else t.to(where) for k, t in a.items()}
+        with forward_ad.dual_level():
+            a[which] = forward_ad.make_dual(a[which], torch.ones_like(a[which]))
+            with pytest.raises(RuntimeError, match="forward gradient"):
+                f(**a)
+        assert f is megacrn_amd.gated_linear_recurrence or (a["state"] == 1).all()
+
+
 def test_c_sizes():
     """Checkpoints: one state in fp32 before every 8th step (every 4th of up to 4 and of 9 to 12 steps) but the first, 16-bit types only; a
     workspace for long sequences with few channels."""
