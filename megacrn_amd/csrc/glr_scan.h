@@ -1,6 +1,6 @@
 // glr_scan.h - gated linear recurrence over long sequences, forward and backward (gfx950, wave64).
 //
-//   a = sigmoid(gate), c = phi(cand):      h_t = h_{t-1} + (1 - a_t)(c_t - h_{t-1})
+//   a = sigmoid(gate), c = phi(cand):      h_t = a_t h_{t-1} + (1 - a_t) c_t
 //   backward, with lam_t the gradient of h_t:   lam_t = dout_t + a_{t+1} lam_{t+1},   lam_{T-1} += dlast
 //     dcand = lam (1 - a) phi'(c)      dgate = sum over the gate's channels of lam a (1 - a)(h_{t-1} - c)      dstate = a_0 lam_0
 //
@@ -126,14 +126,23 @@ template <bool FINE> __device__ __forceinline__ float glr_exp(float x) {
     const float lo = fmaf(x, L2E_LO, fmaf(x, L2E, -t)) * 0.693147182464599609375f;
     return fabsf(t) < 128.f ? fmaf(e, lo, e) : e;
 }
-// 1 - sigmoid(g): its relative error stays that of the exponential, however little is forgotten
-template <bool FINE> __device__ __forceinline__ float glr_w(float g) { return __builtin_amdgcn_rcpf(1.f + glr_exp<FINE>(g)); }
-// the same and p = sigmoid(g)(1 - sigmoid(g)), from the exponential that cannot overflow
-template <bool FINE> __device__ __forceinline__ void glr_wp(float g, float& w, float& p) {
+// A gate is held as n: |n| is the smaller one of a = sigmoid(g) and w = 1 - a, with the relative error of the exponential (which cannot overflow)
+// however little is kept or forgotten; the sign is g's.  The larger one is 1 - |n| and never formed: a x = x - |n| x for an open gate (n >= 0),
+// |n| x for a closed one.  (a formed as 1 - w has lost all its bits at g = -17, w formed as 1 - a at g = 17.)
+template <bool FINE> __device__ __forceinline__ float glr_gate(float g) {
+    const float e = glr_exp<FINE>(-fabsf(g));
+    return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
+}
+// the same, w, and p = a w
+template <bool FINE> __device__ __forceinline__ void glr_gate(float g, float& n, float& w, float& p) {
     const float e = glr_exp<FINE>(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
+    n = copysignf(s, g);
     w = g >= 0.f ? s : r;
     p = s * r;
 }
+__device__ __forceinline__ bool glr_open(float n) { return (int)__float_as_uint(n) >= 0; }
+// a x
+__device__ __forceinline__ float glr_keep(float n, float x) { return fmaf(-n, x, glr_open(n) ? x : 0.f); }
 constexpr float GLR_2L2E = 2.88539004325866699219f;        // 2 log2(e)
 // 1 - 2 / (1 + e^2u): off by 3 units of 2^-24 whatever u is, which shows relatively near 0.  FINE: Taylor's series below 1/4 (its next term is
 // 2^-26 of the value).  16-bit types: u itself below 2^-8 (off by u^2 / 3 < 2^-17 of the value, the quotient by 2^-14 above: their own steps
@@ -148,9 +157,10 @@ template <bool FINE> __device__ __forceinline__ float glr_tanh(float u) {
     return fabsf(u) < 0.25f ? fmaf(u * q, s, u) : far;
 }
 
-// c - h, what a step goes towards; where it goes nowhere (w = 0: masked, or a gate that is open) an infinite state stays what it is
-__device__ __forceinline__ float glr_diff(float w, float c, float h) { return c - (w == 0.f ? 0.f : h); }
-__device__ __forceinline__ float glr_next(float w, float c, float h) { return fmaf(w, glr_diff(w, c, h), h); }
+// c - h, what a step goes towards; where it goes nowhere (n = 0: masked, or a gate that is open) an infinite state stays what it is
+__device__ __forceinline__ float glr_diff(float n, float c, float h) { return c - (n == 0.f && glr_open(n) ? 0.f : h); }
+// a h + w c, as h + w (c - h) or as c - a (c - h)
+__device__ __forceinline__ float glr_next(float n, float c, float h, float diff) { return fmaf(n, diff, glr_open(n) ? h : c); }
 
 // ---- where a thread works ----------------------------------------------------------------------------------------------
 struct GlrAt {
@@ -369,7 +379,7 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
         const int ts = tb + w.seg * K;
         const bool full = tb + span <= w.t1;
         const bool live = SEG == 1 || tb + wave * (64 / CL) * K < w.t1;       // a wave behind the last step only takes part in the scan
-        float ww[K][V], cc[K][V];                          // 1 - a and phi(cand); a masked step is w = 0, c = 0
+        float nn[K][V], cc[K][V];                          // the gate (glr_gate) and phi(cand); a masked step is n = 0, c = 0
         if (live) {
             GlrVec<X, VG> rg[K];
             GlrVec<X, V> rc[K];
@@ -379,7 +389,7 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
             glr_rows<X, V, K, CHAIN>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
             if (p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
             if (FLAT && p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rn, pm, (uint32_t)(w.n2 * p.m_sn), (uint32_t)p.m_st, w.seg, full, end);
-            if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give w = 0, c = 0
+            if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give n = 0, c = 0
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const bool in = ts + k < w.t1, on = in && (!p.mask || rm[k].e[0] != 0);
@@ -401,7 +411,7 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    ww[k][i] = (SHARED && i) ? ww[k][0] : glr_w<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
+                    nn[k][i] = (SHARED && i) ? nn[k][0] : glr_gate<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
                     cc[k][i] = glr_up<X, V>(rc[k], i);
                 }
             if (p.act) {
@@ -414,7 +424,7 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < V; ++i) ww[k][i] = cc[k][i] = 0.f;
+                for (int i = 0; i < V; ++i) nn[k][i] = cc[k][i] = 0.f;
         }
         GLR_PHASE();
         pg += span * p.g_st * es;
@@ -430,10 +440,10 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
 #pragma unroll
             for (int i = 0; i < V; ++i)
 #pragma unroll
-                for (int k = 0; k < K; ++k) {              // from here on ww, cc hold the maps up to each step
-                    A[i] = fmaf(-ww[k][i], A[i], A[i]);
-                    Xl[i] = fmaf(ww[k][i], cc[k][i] - Xl[i], Xl[i]);
-                    ww[k][i] = A[i];
+                for (int k = 0; k < K; ++k) {              // from here on nn, cc hold the maps up to each step
+                    A[i] = glr_keep(nn[k][i], A[i]);
+                    Xl[i] = glr_next(nn[k][i], cc[k][i], Xl[i], cc[k][i] - Xl[i]);
+                    nn[k][i] = A[i];
                     cc[k][i] = Xl[i];
                 }
             float EA[V], EX[V];
@@ -454,8 +464,8 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
             for (int k = 0; k < K; ++k) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    if (SEG > 1) o[i] = fmaf(ww[k][i], h[i], cc[k][i]);
-                    else o[i] = h[i] = glr_next(ww[k][i], cc[k][i], h[i]);
+                    if (SEG > 1) o[i] = fmaf(nn[k][i], h[i], cc[k][i]);
+                    else o[i] = h[i] = glr_next(nn[k][i], cc[k][i], h[i], glr_diff(nn[k][i], cc[k][i], h[i]));
                 }
                 if (w.active && p.out && (full || ts + k < w.t1)) glr_store<X, V, decltype(nt)::value>(po + k * rb, lo, o);
             }
@@ -546,7 +556,7 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
         const int tb = w.t0 + it * span, ts = tb + w.seg * K;
         const bool full = tb + span <= w.t1;
         const bool live = SEG == 1 || tb + wave * (64 / CL) * K < w.t1;       // a wave behind the last step only takes part in the scan
-        float ww[K][V], wc[K][V], q[K][V], dd[K][V];       // 1 - a, its product with phi', a (1 - a)(h_{t-1} - c), dout
+        float nn[K][V], wc[K][V], q[K][V], dd[K][V];       // the gate, (1 - a) phi', a (1 - a)(h_{t-1} - c), dout
         if (live) {
             GlrVec<X, VG> rg[K];
             GlrVec<X, V> rc[K], rd[K];
@@ -565,7 +575,7 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
             }
             if (p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
             if (FLAT && p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rn, pm, (uint32_t)(w.n2 * p.m_sn), (uint32_t)p.m_st, w.seg, full, end);
-            if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give w = p = 0, c = 0
+            if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give n = p = 0, c = 0
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const bool in = ts + k < w.t1, on = in && (!p.mask || rm[k].e[0] != 0);
@@ -594,13 +604,14 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                     rs = glr_load<GlrF32, V>(reinterpret_cast<const char*>(at), (uint32_t)(hoff * 4) + (uint32_t)(p.dtype == GLR_F32 ? w.seg * K : w.seg) * (uint32_t)(NH * 4));
                 }
             }
+            float ww[K][V];                                // 1 - a
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    if (SHARED && i) { ww[k][i] = ww[k][0]; q[k][i] = q[k][0]; }
-                    else if (AGG) ww[k][i] = glr_w<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
-                    else glr_wp<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i), ww[k][i], q[k][i]);
+                    if (SHARED && i) { nn[k][i] = nn[k][0]; ww[k][i] = ww[k][0]; q[k][i] = q[k][0]; }
+                    else if (AGG) nn[k][i] = glr_gate<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
+                    else glr_gate<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i), nn[k][i], ww[k][i], q[k][i]);
                     dd[k][i] = glr_up<X, V>(rd[k], i);
                     if (!AGG) wc[k][i] = glr_up<X, V>(rc[k], i);
                 }
@@ -619,9 +630,9 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                 for (int k = 0; k < K; ++k)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float c = wc[k][i], diff = glr_diff(ww[k][i], c, h[i]);
+                        const float c = wc[k][i], diff = glr_diff(nn[k][i], c, h[i]);
                         q[k][i] *= -diff;
-                        h[i] = fmaf(ww[k][i], diff, h[i]);
+                        h[i] = glr_next(nn[k][i], c, h[i], diff);
                         wc[k][i] = p.act ? ww[k][i] * fmaf(-c, c, 1.f) : ww[k][i];
                         GLR_HERE(q[k][i]);
                         GLR_HERE(wc[k][i]);
@@ -645,9 +656,8 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                 for (int i = 0; i < V; ++i)
 #pragma unroll
                 for (int k = K - 1; k >= 0; --k) {
-                    A[i] = fmaf(-ww[k][i], A[i], A[i]);
-                    const float lam = Xl[i] + dd[k][i];
-                    Xl[i] = fmaf(-ww[k][i], lam, lam);
+                    A[i] = glr_keep(nn[k][i], A[i]);
+                    Xl[i] = glr_keep(nn[k][i], Xl[i] + dd[k][i]);
                 }
             }
             float EA[V], EX[V];
@@ -672,7 +682,7 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                     const float lam = mu[i] + dd[k][i];
                     dc[i] = lam * wc[k][i];
                     dg[i] = lam * q[k][i];
-                    mu[i] = fmaf(-ww[k][i], lam, lam);
+                    mu[i] = glr_keep(nn[k][i], lam);
                 }
                 if (in) glr_store<X, V, decltype(nt)::value>(pdc + k * rb, ldc, dc);
                 if (!SHARED) {

@@ -6,7 +6,8 @@ import numpy as np
 U = 2.0 ** -24
 
 # Relative errors, in units of u, that the bounds grant an fp32 evaluation of the step's functions:
-#   w = 1 - sigmoid(gate) <= 10: exponential 4, sum 1, reciprocal 2, product 1, 1 - w 1, one spare
+#   the smaller one of a = sigmoid(gate) and w = 1 - a <= 10: exponential 4, and half of it again through the sum, sum 1, reciprocal 2, product 1;
+#   the larger one enters as 1 - that, so what it multiplies is off by the smaller one's error and a rounding of the result
 #   tanh <= 12: exponential 4 (its weight is at most 1 where the quotient is used), difference 1, sum 3, reciprocal 2, product 1, one spare
 #   a (1 - a) = z - z^2 <= 40: z 8, twice through z - z^2 with z <= 1/2 (condition 2 at the most), roundings 2
 KW, KC, KP = 10, 12, 40
@@ -45,7 +46,7 @@ def glr_fwd(gate, cand, state=None, mask=None, act="tanh", dt="f32"):
     for t in range(T):
         prev[:, t] = h
         span = np.abs(c[:, t]) + size
-        e = a[:, t] * e + U * w[:, t] * ((KW + 2) * span + _c_error(c[:, t], act, dt))
+        e = a[:, t] * e + U * ((KW + 2) * np.minimum(a[:, t], w[:, t]) * span + w[:, t] * _c_error(c[:, t], act, dt))
         size = a[:, t] * size + w[:, t] * np.abs(c[:, t])
         e = e + U * size
         h = a[:, t] * h + w[:, t] * c[:, t]
@@ -74,7 +75,7 @@ def glr_bwd(cache, dout=None, dlast=None):
         eg[:, t] = p * (2 * el * np.abs(diff) + np.abs(lam) * (before + U * (_c_error(c[:, t], act, dt) + np.abs(prev[:, t]) + (KP + 3) * np.abs(diff))))
         mu = a[:, t] * lam
         size = a[:, t] * big
-        e = a[:, t] * el + U * ((KW + 1) * w[:, t] * big + size)
+        e = a[:, t] * el + U * ((KW + 1) * np.minimum(a[:, t], w[:, t]) * big + size)
     D = H // G
     terms = np.abs(dg).reshape(B, T, N, G, D).sum(-1)
     dgate = dg.reshape(B, T, N, G, D).sum(-1)

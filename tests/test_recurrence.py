@@ -240,6 +240,19 @@ def test_long_memory():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("G", [12, 3, 1])
+@pytest.mark.parametrize("B,T,N", [(2, 1, 3), (1, 3, 2), (1, 8, 2), (2, 40, 3), (1, 130, 3), (1, 2100, 1), (4, 200, 130)])
+def test_closed_gates_keep_their_share(B, T, N, G):
+    """Gates of -25 .. -4 among open ones, states of 1e6: a = sigmoid(gate) has to keep its own relative precision (1 - a rounds to 1 below -17), in
+    outputs, state gradients and gradients that cross a reset."""
+    gate, cand, st, _, dout, dlast = _inputs(B, T, N, 12, G, "f32", False, T + G)
+    g = torch.Generator().manual_seed(T)
+    closed = torch.rand(gate.shape, generator=g) < (1.0 if T < 4 else 0.3)
+    gate = torch.where(closed, -4 - 21 * torch.rand(gate.shape, generator=g), gate)
+    _against_oracle(gate, cand, st * 1e6, None, dout, dlast, "tanh", "f32")
+
+
+@pytest.mark.gpu
 def test_extreme_gates_and_small_candidates():
     """Gates of +-100 and +-inf hold or replace the state exactly; tanh of 1e-6 .. 1e-2 keeps its relative precision."""
     import megacrn_amd
