@@ -29,24 +29,18 @@ struct GlrF32 {
     static constexpr bool FINE = true;
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
-    static constexpr uint32_t INF = 0x7f800000u;           // a word of infinities
-    static __device__ __forceinline__ float inf() { return __builtin_inff(); }
 };
 struct GlrBf16 {
     typedef __bf16 S;
     static constexpr bool FINE = false;
     static __device__ __forceinline__ float up(__bf16 v) { return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, v) << 16); }
     static __device__ __forceinline__ __bf16 down(float f) { return (__bf16)f; }     // to the nearest, ties to even, by the hardware
-    static constexpr uint32_t INF = 0x7f807f80u;
-    static __device__ __forceinline__ __bf16 inf() { return (__bf16)__builtin_inff(); }
 };
 struct GlrF16 {
     typedef _Float16 S;
     static constexpr bool FINE = false;
     static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
     static __device__ __forceinline__ _Float16 down(float f) { return (_Float16)f; }
-    static constexpr uint32_t INF = 0x7c007c00u;
-    static __device__ __forceinline__ _Float16 inf() { return (_Float16)__builtin_inff(); }
 };
 
 // aligned to its elements only (global memory takes any alignment): what rows of any length need
@@ -66,15 +60,15 @@ template <class X, int V> __device__ __forceinline__ GlrVec<X, V> glr_load(const
 template <int BYTES> struct GlrWord { typedef uint32_t T __attribute__((ext_vector_type(BYTES / 4))); };
 template <> struct GlrWord<4> { typedef uint32_t T; };
 template <> struct GlrWord<2> { typedef uint16_t T; };
-// r where `on`, else the pattern `other` in every word: pairs of 16-bit elements are not taken apart for it
-template <class X, int V> __device__ __forceinline__ void glr_only(bool on, GlrVec<X, V>& r, uint32_t other) {
+// r where `on`, else zeros: pairs of 16-bit elements are not taken apart for it
+template <class X, int V> __device__ __forceinline__ void glr_only(bool on, GlrVec<X, V>& r) {
     typedef typename GlrWord<sizeof(r)>::T T;
     T w = __builtin_bit_cast(T, r);
     if constexpr (sizeof(r) > 4) {
 #pragma unroll
-        for (unsigned j = 0; j < sizeof(r) / 4; ++j) w[j] = on ? w[j] : other;
+        for (unsigned j = 0; j < sizeof(r) / 4; ++j) w[j] = on ? w[j] : 0u;
     } else {
-        w = on ? w : (T)other;
+        w = on ? w : (T)0;
     }
     r = __builtin_bit_cast(GlrVec<X, V>, w);
 }
@@ -116,6 +110,30 @@ struct GlrByte {
     typedef uint8_t S;
 };
 
+// Steps that keep the state - masked, or behind the last one (`left` steps are there): bit k of a word is 1 where step k moves it, and the candidate of
+// one that does not becomes 0.  FLAT: a word for each channel, since these may belong to two nodes (`over` of them to the second, rn); their candidates
+// become 0 behind the conversion (elements of a pair are not taken apart for it).
+template <int V, bool FLAT> struct GlrMoves {
+    unsigned w[FLAT ? V : 1];
+    __device__ __forceinline__ bool at(int k, int i) const { return (w[FLAT ? i : 0] >> k) & 1u; }
+};
+template <class X, int V, int K, bool FLAT>
+__device__ __forceinline__ void glr_masked(GlrMoves<V, FLAT>& m, int left, bool mask, int over, const GlrVec<GlrByte, 1>* rm, const GlrVec<GlrByte, 1>* rn,
+                                           GlrVec<X, V>* rc) {
+    unsigned one = 0, two = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        one |= (k < left && (!mask || rm[k].e[0] != 0) ? 1u : 0u) << k;
+        if (FLAT) two |= (k < left && (!mask || rn[k].e[0] != 0) ? 1u : 0u) << k;
+        if (!FLAT) glr_only<X, V>((one >> k) & 1u, rc[k]);
+    }
+    m.w[0] = one;
+    if (FLAT) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) m.w[i] = V - i > over ? one : two;
+    }
+}
+
 // ---- the functions of a step -----------------------------------------------------------------------------------------
 // 2^(x log2 e).  The product's rounding is an error of |x| u in the exponent; FINE carries it along (the guard keeps infinities).
 template <bool FINE> __device__ __forceinline__ float glr_exp(float x) {
@@ -128,7 +146,7 @@ template <bool FINE> __device__ __forceinline__ float glr_exp(float x) {
 }
 // A gate is held as n: |n| is the smaller one of a = sigmoid(g) and w = 1 - a, with the relative error of the exponential (which cannot overflow)
 // however little is kept or forgotten; the sign is g's.  The larger one is 1 - |n| and never formed: a x = x - |n| x for an open gate (n >= 0),
-// |n| x for a closed one.  (a formed as 1 - w has lost all its bits at g = -17, w formed as 1 - a at g = 17.)
+// |n| x for a closed one.  GLR_HOLD is the closed gate with a = 1, a step that is masked: it keeps x whatever x is, infinities among it.  (a formed as 1 - w has lost all its bits at g = -17, w formed as 1 - a at g = 17.)
 template <bool FINE> __device__ __forceinline__ float glr_gate(float g) {
     const float e = glr_exp<FINE>(-fabsf(g));
     return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
@@ -140,6 +158,7 @@ template <bool FINE> __device__ __forceinline__ void glr_gate(float g, float& n,
     w = g >= 0.f ? s : r;
     p = s * r;
 }
+constexpr float GLR_HOLD = -1.f;
 __device__ __forceinline__ bool glr_open(float n) { return (int)__float_as_uint(n) >= 0; }
 // a x
 __device__ __forceinline__ float glr_keep(float n, float x) { return fmaf(-n, x, glr_open(n) ? x : 0.f); }
@@ -157,7 +176,7 @@ template <bool FINE> __device__ __forceinline__ float glr_tanh(float u) {
     return fabsf(u) < 0.25f ? fmaf(u * q, s, u) : far;
 }
 
-// c - h, what a step goes towards; where it goes nowhere (n = 0: masked, or a gate that is open) an infinite state stays what it is
+// c - h, what a step goes towards; where it goes nowhere (n = 0: a gate that is wholly open) an infinite state stays what it is
 __device__ __forceinline__ float glr_diff(float n, float c, float h) { return c - (n == 0.f && glr_open(n) ? 0.f : h); }
 // a h + w c, as h + w (c - h) or as c - a (c - h)
 __device__ __forceinline__ float glr_next(float n, float c, float h, float diff) { return fmaf(n, diff, glr_open(n) ? h : c); }
@@ -379,7 +398,7 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
         const int ts = tb + w.seg * K;
         const bool full = tb + span <= w.t1;
         const bool live = SEG == 1 || tb + wave * (64 / CL) * K < w.t1;       // a wave behind the last step only takes part in the scan
-        float nn[K][V], cc[K][V];                          // the gate (glr_gate) and phi(cand); a masked step is n = 0, c = 0
+        float nn[K][V], cc[K][V];                          // the gate (glr_gate) and phi(cand); a masked step is GLR_HOLD, c = 0
         if (live) {
             GlrVec<X, VG> rg[K];
             GlrVec<X, V> rc[K];
@@ -389,24 +408,8 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
             glr_rows<X, V, K, CHAIN>(rc, pc, lc, (uint32_t)(p.c_st * es), w.seg, full, end);
             if (p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
             if (FLAT && p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rn, pm, (uint32_t)(w.n2 * p.m_sn), (uint32_t)p.m_st, w.seg, full, end);
-            if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give n = 0, c = 0
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    const bool in = ts + k < w.t1, on = in && (!p.mask || rm[k].e[0] != 0);
-                    if (FLAT && p.mask) {
-                        const bool on2 = in && rn[k].e[0] != 0;
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            const bool o = w.ch + i < p.H ? on : on2;
-                            rg[k].e[i] = o ? rg[k].e[i] : X::inf();
-                            rc[k].e[i] = o ? rc[k].e[i] : (S)0.f;
-                        }
-                    } else {
-                        glr_only<X, VG>(on, rg[k], X::INF);
-                        glr_only<X, V>(on, rc[k], 0u);
-                    }
-                }
-            }
+            GlrMoves<V, FLAT> moves = {};
+            if (p.mask || !full) glr_masked<X, V, K, FLAT>(moves, w.t1 - ts, p.mask, w.ch + V - p.H, rm, rn, rc);
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -414,6 +417,15 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
                     nn[k][i] = (SHARED && i) ? nn[k][0] : glr_gate<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
                     cc[k][i] = glr_up<X, V>(rc[k], i);
                 }
+            if (p.mask || !full) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        nn[k][i] = moves.at(k, i) ? nn[k][i] : GLR_HOLD;
+                        if (FLAT) cc[k][i] = moves.at(k, i) ? cc[k][i] : 0.f;
+                    }
+            }
             if (p.act) {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
@@ -556,6 +568,7 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
         const int tb = w.t0 + it * span, ts = tb + w.seg * K;
         const bool full = tb + span <= w.t1;
         const bool live = SEG == 1 || tb + wave * (64 / CL) * K < w.t1;       // a wave behind the last step only takes part in the scan
+        GlrMoves<V, FLAT> moves = {};
         float nn[K][V], wc[K][V], q[K][V], dd[K][V];       // the gate, (1 - a) phi', a (1 - a)(h_{t-1} - c), dout
         if (live) {
             GlrVec<X, VG> rg[K];
@@ -575,24 +588,10 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
             }
             if (p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rm, pm, lm, (uint32_t)p.m_st, w.seg, full, end);
             if (FLAT && p.mask) glr_rows<GlrByte, 1, K, CHAIN>(rn, pm, (uint32_t)(w.n2 * p.m_sn), (uint32_t)p.m_st, w.seg, full, end);
-            if (p.mask || !full) {                         // a step that keeps the state: gate = inf, cand = 0 give n = p = 0, c = 0
+            if (p.mask || !full) {
+                glr_masked<X, V, K, FLAT>(moves, w.t1 - ts, p.mask, w.ch + V - p.H, rm, rn, rc);
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    const bool in = ts + k < w.t1, on = in && (!p.mask || rm[k].e[0] != 0);
-                    if (FLAT && p.mask) {
-                        const bool on2 = in && rn[k].e[0] != 0;
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            const bool o = w.ch + i < p.H ? on : on2;
-                            rg[k].e[i] = o ? rg[k].e[i] : X::inf();
-                            if (!AGG) rc[k].e[i] = o ? rc[k].e[i] : (S)0.f;
-                        }
-                    } else {
-                        glr_only<X, VG>(on, rg[k], X::INF);
-                        if (!AGG) glr_only<X, V>(on, rc[k], 0u);
-                    }
-                    glr_only<X, V>(in, rd[k], 0u);
-                }
+                for (int k = 0; k < K; ++k) glr_only<X, V>(ts + k < w.t1, rd[k]);      // behind the last step dout is 0
             }
             if (!AGG) {
 #pragma unroll
@@ -615,6 +614,15 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                     dd[k][i] = glr_up<X, V>(rd[k], i);
                     if (!AGG) wc[k][i] = glr_up<X, V>(rc[k], i);
                 }
+            if (p.mask || !full) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        nn[k][i] = moves.at(k, i) ? nn[k][i] : GLR_HOLD;
+                        if (FLAT && !AGG) wc[k][i] = moves.at(k, i) ? wc[k][i] : 0.f;
+                    }
+            }
             if (!AGG && p.act) {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
@@ -672,7 +680,7 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
 #pragma unroll
             for (int i = 0; i < V; ++i) mu[i] = carry[i];
         }
-        auto steps = [&](auto nt) {
+        auto steps = [&](auto nt, auto masked) {
 #pragma unroll
             for (int k = K - 1; k >= 0; --k) {
                 const bool in = w.active && (full || ts + k < w.t1);
@@ -683,6 +691,11 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                     dc[i] = lam * wc[k][i];
                     dg[i] = lam * q[k][i];
                     mu[i] = glr_keep(nn[k][i], lam);
+                    if (decltype(masked)::value) {         // 0, whatever lam is and the step holds
+                        const bool o = moves.at(k, i);
+                        dc[i] = o ? dc[i] : 0.f;
+                        dg[i] = o ? dg[i] : 0.f;
+                    }
                 }
                 if (in) glr_store<X, V, decltype(nt)::value>(pdc + k * rb, ldc, dc);
                 if (!SHARED) {
@@ -700,8 +713,13 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
             }
         };
         if (live) {
-            if (p.nt) steps(GlrYes());
-            else steps(GlrNo());
+            if (p.mask) {
+                if (p.nt) steps(GlrYes(), GlrYes());
+                else steps(GlrNo(), GlrYes());
+            } else {
+                if (p.nt) steps(GlrYes(), GlrNo());
+                else steps(GlrNo(), GlrNo());
+            }
         }
         pdc -= span * rb;
         pdg -= span * gb;

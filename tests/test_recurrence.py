@@ -383,6 +383,39 @@ def test_state_of_a_masked_row_is_kept_whatever_it_is(B, T, N, H, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,N,H,G", [(2, 1, 3, 8, 8), (2, 5, 3, 8, 4), (2, 8, 3, 7, 7), (2, 30, 3, 8, 8), (2, 33, 5, 12, 1), (2, 300, 3, 8, 2), (2, 2100, 3, 9, 9),
+                                       (2, 300, 40, 64, 64), (2, 300, 100, 64, 1), (2, 300, 150, 33, 33), (64, 20, 40, 256, 256), (33, 20, 64, 65, 5)])
+def test_infinite_gradients_of_masked_steps(B, T, N, H, G, dt):
+    """Gradients that are not finite pass a masked step as they are and leave its own gradients 0, in every variant and whether T fills its tiles
+    or not; every other row is what it is without them."""
+    import megacrn_amd
+    gate, cand, st, _, dout, dlast = (None if t is None else t.cuda() for t in _inputs(B, T, N, H, G, dt, False, 3))
+    keep = torch.rand(B, T, N, generator=torch.Generator().manual_seed(T)).cuda() > 0.2
+    keep[-1, :, 1] = False                                                 # never moved
+    keep[0, T // 2:, 2] = False                                            # masked towards the end
+    gate[-1, :, 1], cand[-1, :, 1] = float("nan"), -float("inf")
+
+    def run(dout, dlast):
+        leaves = [t.detach().requires_grad_() for t in (gate, cand, st)]
+        out, last = megacrn_amd.gated_linear_recurrence(*leaves, keep)
+        return torch.autograd.grad((out, last), leaves, (dout, dlast))
+    want = run(dout, dlast)
+    assert all(torch.isfinite(t).all() for t in want)
+    bad = torch.tensor([float("inf"), -float("inf"), float("nan")], device="cuda").repeat((H + 2) // 3)[:H]
+    dlast2, dout2 = dlast.clone(), dout.clone()
+    dlast2[-1, 1] = bad
+    dout2[0, -1, 2] = bad.to(dout.dtype)
+    got = run(dout2, dlast2)
+    assert torch.equal(torch.nan_to_num(got[2][-1, 1], 7.0), torch.nan_to_num(bad, 7.0))
+    for g, w in zip(got[:2], want[:2]):
+        assert not g[-1, :, 1].any() and not g[0, T // 2:, 2].any()
+        g[0, :, 2] = w[0, :, 2]
+    got[2][0, 2], got[2][-1, 1] = want[2][0, 2], want[2][-1, 1]
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_nan_stays_in_its_row():
     """A NaN that is not masked reaches its own channel's later steps and nothing else."""
     import megacrn_amd
