@@ -23,22 +23,18 @@ constexpr int GLR_THREADS = 256;
 enum { GLR_WALK = 0, GLR_AGG = 1, GLR_CHAIN = 2 };
 
 // ---- storage types --------------------------------------------------------------------------------------------------
-// FINE: the step's functions keep all of fp32 (16-bit types: what their own rounding leaves of it, and fewer instructions)
 struct GlrF32 {
     typedef float S;
-    static constexpr bool FINE = true;
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
 };
 struct GlrBf16 {
     typedef __bf16 S;
-    static constexpr bool FINE = false;
     static __device__ __forceinline__ float up(__bf16 v) { return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, v) << 16); }
     static __device__ __forceinline__ __bf16 down(float f) { return (__bf16)f; }     // to the nearest, ties to even, by the hardware
 };
 struct GlrF16 {
     typedef _Float16 S;
-    static constexpr bool FINE = false;
     static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
     static __device__ __forceinline__ _Float16 down(float f) { return (_Float16)f; }
 };
@@ -135,51 +131,51 @@ __device__ __forceinline__ void glr_masked(GlrMoves<V, FLAT>& m, int left, bool 
 }
 
 // ---- the functions of a step -----------------------------------------------------------------------------------------
-// 2^(x log2 e).  The product's rounding is an error of |x| u in the exponent; FINE carries it along (the guard keeps infinities).
-template <bool FINE> __device__ __forceinline__ float glr_exp(float x) {
-    const float L2E = 1.44269502162933349609f, L2E_LO = 1.92596299112661746887e-8f;    // log2(e) = L2E + L2E_LO
-    const float t = x * L2E;
-    const float e = __builtin_amdgcn_exp2f(t);
-    if (!FINE) return e;
-    const float lo = fmaf(x, L2E_LO, fmaf(x, L2E, -t)) * 0.693147182464599609375f;
-    return fabsf(t) < 128.f ? fmaf(e, lo, e) : e;
+// The arithmetic is fp32 whatever the inputs' type: the states behind it are.
+// e^x, x <= 0.  The rounding of t = x log2 e would be an error of |x| u; x - t ln 2 is what it left out.  The factor is above log2 e by a little more than
+// that rounding, so the rest is never negative and a clamp to [0, 1] (part of the instruction) only drops the NaN of an infinite x.  Off by 4 u, 7 u below -17.
+__device__ __forceinline__ float glr_exp(float x) {
+    const float t = x * 1.44269514083862304688f, e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, __builtin_amdgcn_fmed3f(fmaf(t, -0.693147182464599609375f, x), 0.f, 1.f), e);
 }
 // A gate is held as n: |n| is the smaller one of a = sigmoid(g) and w = 1 - a, with the relative error of the exponential (which cannot overflow)
 // however little is kept or forgotten; the sign is g's.  The larger one is 1 - |n| and never formed: a x = x - |n| x for an open gate (n >= 0),
 // |n| x for a closed one.  GLR_HOLD is the closed gate with a = 1, a step that is masked: it keeps x whatever x is, infinities among it.  (a formed as 1 - w has lost all its bits at g = -17, w formed as 1 - a at g = 17.)
-template <bool FINE> __device__ __forceinline__ float glr_gate(float g) {
-    const float e = glr_exp<FINE>(-fabsf(g));
+__device__ __forceinline__ float glr_gate(float g) {
+    const float e = glr_exp(-fabsf(g));
     return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
 }
 // the same, w, and p = a w
-template <bool FINE> __device__ __forceinline__ void glr_gate(float g, float& n, float& w, float& p) {
-    const float e = glr_exp<FINE>(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
+__device__ __forceinline__ void glr_gate(float g, float& n, float& w, float& p) {
+    const float e = glr_exp(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
     n = copysignf(s, g);
     w = g >= 0.f ? s : r;
     p = s * r;
 }
 constexpr float GLR_HOLD = -1.f;
 __device__ __forceinline__ bool glr_open(float n) { return (int)__float_as_uint(n) >= 0; }
+// Open: x, closed: y - by the sign's mask and one bit-select (the empty statement keeps the compiler from comparing, twice, and selecting through VCC)
+__device__ __forceinline__ float glr_pick(float n, float x, float y) {
+    int closed = (int)__float_as_uint(n) >> 31;
+    asm("" : "+v"(closed));
+    return __uint_as_float(((unsigned)closed & __float_as_uint(y)) | (~(unsigned)closed & __float_as_uint(x)));
+}
 // a x
-__device__ __forceinline__ float glr_keep(float n, float x) { return fmaf(-n, x, glr_open(n) ? x : 0.f); }
+__device__ __forceinline__ float glr_keep(float n, float x) { return fmaf(-n, x, glr_pick(n, x, 0.f)); }
 constexpr float GLR_2L2E = 2.88539004325866699219f;        // 2 log2(e)
-// 1 - 2 / (1 + e^2u): off by 3 units of 2^-24 whatever u is, which shows relatively near 0.  FINE: Taylor's series below 1/4 (its next term is
-// 2^-26 of the value).  16-bit types: u itself below 2^-8 (off by u^2 / 3 < 2^-17 of the value, the quotient by 2^-14 above: their own steps
-// are 2^-12 and 2^-9) - 5 instructions of 39 fewer in a forward that they bound.
-template <bool FINE> __device__ __forceinline__ float glr_tanh(float u) {
+// 1 - 2 / (1 + e^2u): off by 3 units of 2^-24 whatever u is, which shows relatively near 0: below 3/8 the odd polynomial of degree 7 whose largest
+// relative error there is smallest (1.2 u, 2.2 u with its roundings; the coefficients by linear programming over 3000 Chebyshev points).
+__device__ __forceinline__ float glr_tanh(float u) {
     const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * GLR_2L2E)), 1.f);
-    if (!FINE) return fabsf(u) < 0.00390625f ? u : far;
     const float q = u * u;
-    float s = fmaf(q, 62.f / 2835.f, -17.f / 315.f);
-    s = fmaf(q, s, 2.f / 15.f);
-    s = fmaf(q, s, -1.f / 3.f);
-    return fabsf(u) < 0.25f ? fmaf(u * q, s, u) : far;
+    const float s = fmaf(q, fmaf(q, -0.04848729074001312256f, 0.13289725780487060547f), -0.33332332968711853027f);
+    return fabsf(u) < 0.375f ? fmaf(u * q, s, u) : far;
 }
 
 // c - h, what a step goes towards; where it goes nowhere (n = 0: a gate that is wholly open) an infinite state stays what it is
 __device__ __forceinline__ float glr_diff(float n, float c, float h) { return c - (n == 0.f && glr_open(n) ? 0.f : h); }
 // a h + w c, as h + w (c - h) or as c - a (c - h)
-__device__ __forceinline__ float glr_next(float n, float c, float h, float diff) { return fmaf(n, diff, glr_open(n) ? h : c); }
+__device__ __forceinline__ float glr_next(float n, float c, float h, float diff) { return fmaf(n, diff, glr_pick(n, h, c)); }
 
 // ---- where a thread works ----------------------------------------------------------------------------------------------
 struct GlrAt {
@@ -363,7 +359,7 @@ __global__ void glr_clear_kernel(unsigned* __restrict__ words, long long tickets
 // WALK: the block walks its chunk tile by tile, from the state that the maps of the chunks before it give (one chunk: from h0).
 // AGG: only the chunk's map is wanted (agg[chunk][b][A | X][N*H]).  CHAIN: the chunk is one tile, its state comes from the block before.
 template <class X, int V, int K, int CL, int GATES, int MODE>
-__global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GATES == GLR_FLAT && X::FINE) ? 3 : 4) void glr_fwd_kernel(GlrP p) {
+__global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GATES == GLR_FLAT && sizeof(typename X::S) == 4) ? 3 : 4) void glr_fwd_kernel(GlrP p) {
     constexpr bool SHARED = GATES == GLR_SHARED, FLAT = GATES == GLR_FLAT, AGG = MODE == GLR_AGG, CHAIN = MODE == GLR_CHAIN, REV = false;
     constexpr int SEG = GLR_THREADS / CL, VG = SHARED ? 1 : V, W = GLR_THREADS / 64, span = SEG * K;
     typedef typename X::S S;
@@ -414,7 +410,7 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    nn[k][i] = (SHARED && i) ? nn[k][0] : glr_gate<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
+                    nn[k][i] = (SHARED && i) ? nn[k][0] : glr_gate(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
                     cc[k][i] = glr_up<X, V>(rc[k], i);
                 }
             if (p.mask || !full) {
@@ -430,7 +426,7 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
 #pragma unroll
                 for (int k = 0; k < K; ++k)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) cc[k][i] = glr_tanh<X::FINE>(cc[k][i]);
+                    for (int i = 0; i < V; ++i) cc[k][i] = glr_tanh(cc[k][i]);
             }
         } else if (SEG > 1) {                              // its map is the identity (a branch around the maps would cost a copy of each)
 #pragma unroll
@@ -609,9 +605,8 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     if (SHARED && i) { nn[k][i] = nn[k][0]; ww[k][i] = ww[k][0]; q[k][i] = q[k][0]; }
-                    else if (AGG) nn[k][i] = glr_gate<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
-                    else glr_gate<X::FINE>(glr_up<X, VG>(rg[k], SHARED ? 0 : i), nn[k][i], ww[k][i], q[k][i]);
-                    dd[k][i] = glr_up<X, V>(rd[k], i);
+                    else if (AGG) nn[k][i] = glr_gate(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
+                    else glr_gate(glr_up<X, VG>(rg[k], SHARED ? 0 : i), nn[k][i], ww[k][i], q[k][i]);
                     if (!AGG) wc[k][i] = glr_up<X, V>(rc[k], i);
                 }
             if (p.mask || !full) {
@@ -627,7 +622,7 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) wc[k][i] = glr_tanh<X::FINE>(wc[k][i]);
+                    for (int i = 0; i < V; ++i) wc[k][i] = glr_tanh(wc[k][i]);
             }
             GLR_PHASE();
             if (!AGG) {
@@ -645,7 +640,12 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                         GLR_HERE(q[k][i]);
                         GLR_HERE(wc[k][i]);
                     }
+                GLR_PHASE();
             }
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) dd[k][i] = glr_up<X, V>(rd[k], i);
         }
         GLR_PHASE();
         pg -= span * p.g_st * es;

@@ -6,14 +6,13 @@ import numpy as np
 U = 2.0 ** -24
 
 # Relative errors, in units of u, that the bounds grant an fp32 evaluation of the step's functions:
-#   the smaller one of a = sigmoid(gate) and w = 1 - a <= 10: exponential 4, and half of it again through the sum, sum 1, reciprocal 2, product 1;
-#   the larger one enters as 1 - that, so what it multiplies is off by the smaller one's error and a rounding of the result
+#   the smaller one of a = sigmoid(gate) and w = 1 - a <= 10: exponential 4, and half of it again through the sum, sum 1, reciprocal 2, product 1 (a gate
+#   beyond 17: exponential up to 7, the others exact); the larger one enters as 1 - that, so what it multiplies is off by the smaller one's error
+#   and a rounding of the result
 #   tanh <= 12: exponential 4 (its weight is at most 1 where the quotient is used), difference 1, sum 3, reciprocal 2, product 1, one spare
-#   a (1 - a) = z - z^2 <= 40: z 8, twice through z - z^2 with z <= 1/2 (condition 2 at the most), roundings 2
-KW, KC, KP = 10, 12, 40
-# tanh of 16-bit inputs: 1 - 2 / (1 + e^2u) throughout, absolutely off by 2 (0.25 rcp + 0.25 sum + 0.5 exponential) + 1 + spare <= 4 u, and below
-# |u| = 2^-8 by u^2 / 3 <= 2^-17.5 of the value
-KA16, KR16 = 4, 2.0 ** (24 - 17.5)
+#   a w <= 17: the smaller one 10, the other 5, product 1, one spare
+# of inputs of any type: they are converted to fp32 first.
+KW, KC, KP = 10, 12, 17
 
 
 def _gates(gate, cand, mask, act):
@@ -29,15 +28,14 @@ def _gates(gate, cand, mask, act):
     return a, w, c
 
 
-def _c_error(c, act, dt):
+def _c_error(c, act):
     """Error granted to phi(cand), in units of u."""
-    if act != "tanh":
-        return np.zeros_like(c)
-    return KC * np.abs(c) if dt == "f32" else np.where(np.abs(c) < 2.0 ** -8, KR16 * np.abs(c), KA16)
+    return KC * np.abs(c) if act == "tanh" else np.zeros_like(c)
 
 
 def glr_fwd(gate, cand, state=None, mask=None, act="tanh", dt="f32"):
-    """gate (B,T,N,G), cand (B,T,N,H), state (B,N,H), mask (B,T,N) -> out, last, bound of |error| of out in fp32, cache."""
+    """gate (B,T,N,G), cand (B,T,N,H), state (B,N,H), mask (B,T,N) -> out, last, bound of |error| of out in fp32, cache.
+    dt: the inputs' type; the arithmetic is fp32 for all of them, so the bounds do not depend on it."""
     B, T, N, H = cand.shape
     a, w, c = _gates(gate, cand, mask, act)
     h = np.zeros((B, N, H)) if state is None else state.astype(np.float64)
@@ -46,18 +44,18 @@ def glr_fwd(gate, cand, state=None, mask=None, act="tanh", dt="f32"):
     for t in range(T):
         prev[:, t] = h
         span = np.abs(c[:, t]) + size
-        e = a[:, t] * e + U * ((KW + 2) * np.minimum(a[:, t], w[:, t]) * span + w[:, t] * _c_error(c[:, t], act, dt))
+        e = a[:, t] * e + U * ((KW + 2) * np.minimum(a[:, t], w[:, t]) * span + w[:, t] * _c_error(c[:, t], act))
         size = a[:, t] * size + w[:, t] * np.abs(c[:, t])
         e = e + U * size
         h = a[:, t] * h + w[:, t] * c[:, t]
         out[:, t], err[:, t] = h, e
     # a step's rounding enters twice where maps of segments are composed before the steps are run
-    return out, h, 2 * err, (a, w, c, prev, 2 * err, act, gate.shape[-1], dt)
+    return out, h, 2 * err, (a, w, c, prev, 2 * err, act, gate.shape[-1])
 
 
 def glr_bwd(cache, dout=None, dlast=None):
     """-> dgate, dcand, dstate and bounds of their errors in fp32 (the same order)."""
-    a, w, c, prev, eh, act, G, dt = cache
+    a, w, c, prev, eh, act, G = cache
     B, T, N, H = a.shape
     mu = np.zeros((B, N, H)) if dlast is None else dlast.astype(np.float64)
     size, e = np.abs(mu), np.zeros((B, N, H))
@@ -68,11 +66,11 @@ def glr_bwd(cache, dout=None, dlast=None):
         el = e + U * big                                # error of lam
         slope = 1 - c[:, t] ** 2 if act == "tanh" else np.ones_like(lam)
         dc[:, t] = lam * w[:, t] * slope
-        ec[:, t] = w[:, t] * (slope * (2 * el + U * (KW + 4) * np.abs(lam)) + U * (2 * np.abs(c[:, t]) * _c_error(c[:, t], act, dt) + 2) * np.abs(lam) * (act == "tanh"))
+        ec[:, t] = w[:, t] * (slope * (2 * el + U * (KW + 4) * np.abs(lam)) + U * (2 * np.abs(c[:, t]) * _c_error(c[:, t], act) + 2) * np.abs(lam) * (act == "tanh"))
         p, diff = a[:, t] * w[:, t], prev[:, t] - c[:, t]
         before = eh[:, t - 1] if t else 0.0
         dg[:, t] = lam * p * diff
-        eg[:, t] = p * (2 * el * np.abs(diff) + np.abs(lam) * (before + U * (_c_error(c[:, t], act, dt) + np.abs(prev[:, t]) + (KP + 3) * np.abs(diff))))
+        eg[:, t] = p * (2 * el * np.abs(diff) + np.abs(lam) * (before + U * (_c_error(c[:, t], act) + np.abs(prev[:, t]) + (KP + 3) * np.abs(diff))))
         mu = a[:, t] * lam
         size = a[:, t] * big
         e = a[:, t] * el + U * ((KW + 1) * np.minimum(a[:, t], w[:, t]) * big + size)

@@ -253,6 +253,18 @@ def test_closed_gates_keep_their_share(B, T, N, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("B,T,N,G", [(2, 1, 3, 12), (1, 8, 2, 3), (2, 40, 3, 12), (1, 2100, 1, 1), (4, 200, 130, 12)])
+def test_16_bit_inputs_have_fp32_states(B, T, N, G, dt):
+    """Small candidates (tanh near 0) and gates far from 0 of 16-bit types: the fp32 state is as exact as that of fp32 inputs."""
+    gate, cand, st, _, dout, dlast = _inputs(B, T, N, 12, G, dt, False, T + G)
+    g = torch.Generator().manual_seed(T)
+    cand = (cand.float() * 10.0 ** (-3 * torch.rand(cand.shape, generator=g))).to(TORCH[dt])
+    gate = torch.where(torch.rand(gate.shape, generator=g) < 0.3, -25 + 50 * torch.rand(gate.shape, generator=g), gate.float()).to(TORCH[dt])
+    _against_oracle(gate, cand, st * 1e-3, None, dout, dlast, "tanh", dt)
+
+
+@pytest.mark.gpu
 def test_extreme_gates_and_small_candidates():
     """Gates of +-100 and +-inf hold or replace the state exactly; tanh of 1e-6 .. 1e-2 keeps its relative precision."""
     import megacrn_amd
