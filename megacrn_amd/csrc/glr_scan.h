@@ -393,7 +393,9 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
     for (int tb = w.t0; tb < w.t1; tb += span) {
         const int ts = tb + w.seg * K;
         const bool full = tb + span <= w.t1;
-        const bool live = SEG == 1 || tb + wave * (64 / CL) * K < w.t1;       // a wave behind the last step only takes part in the scan
+        // a wave behind the last step only takes part in the scan (CHAIN: as its steps are masked; the other path's zeros would be written to 64
+        // registers by every wave)
+        const bool live = SEG == 1 || CHAIN || tb + wave * (64 / CL) * K < w.t1;
         float nn[K][V], cc[K][V];                          // the gate (glr_gate) and phi(cand); a masked step is GLR_HOLD, c = 0
         if (live) {
             GlrVec<X, VG> rg[K];
