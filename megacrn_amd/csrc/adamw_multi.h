@@ -198,13 +198,25 @@ __device__ __forceinline__ void adamw_update(const AdamwP& p, const AdamwT& t, c
         adamw_decode_m(r.cm, r.sm, r.m);
         adamw_decode_v(r.cv, r.sv, r.v);
     }
+    float root[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const float g = r.g[k] * factor;
         r.m[k] = p.b1 * r.m[k] + p.c1 * g;
         r.v[k] = p.b2 * r.v[k] + (p.c2 * g) * g;
         // root and reciprocal by the hardware, each off by one unit of the last place: below the rounding of the update itself
-        const float q = r.m[k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(r.v[k]) * h.inv_bc2 + p.eps);
+        root[k] = __builtin_amdgcn_sqrtf(r.v[k]);
+    }
+    // The hardware's root of a subnormal v (below 2^-126) is 0.  That moves the denominator by less than 2^-63 inv_bc2: below its rounding with any eps
+    // above 2^-38 inv_bc2 (1.2e-10 at b2 = 0.999).  A smaller eps has small v scaled.
+    if (__builtin_amdgcn_readfirstlane(h.inv_bc2 * 0x1p-38f > p.eps)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (r.v[k] < 0x1p-96f) root[k] = __builtin_amdgcn_sqrtf(r.v[k] * 0x1p64f) * 0x1p-32f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float q = r.m[k] * __builtin_amdgcn_rcpf(root[k] * h.inv_bc2 + p.eps);
         r.w[k] = __builtin_fmaf(-h.step_size, q, r.w[k] * h.decay);
     }
     const bool some = WHOLE || i < t.n;

@@ -292,6 +292,22 @@ def test_large_tensor_and_groups(bits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("eps", [1.2e-38, 1e-30, 1e-20, 1e-12, 1e-10, 1e-8])
+def test_small_eps_and_subnormal_moments(eps):
+    """Gradients down to 1e-21, whose v is subnormal: its root is no 0 that the update would be divided by.  Three steps in 32 bits within the oracle's
+    bounds."""
+    import megacrn_amd
+    g = torch.cat([torch.tensor([10.0 ** -(k / 4) for k in range(85)]), torch.zeros(3)]).cuda()
+    w = torch.randn(g.numel(), device="cuda")
+    opt = megacrn_amd.AdamW([w], lr=1e-2, eps=eps)
+    for step in range(1, 4):
+        before, mv = w.double().cpu().numpy(), [_piece(a, opt, 0) for a in opt.moments()]
+        opt.step(grads=[g])
+        want = O.adamw_step(before, g.double().cpu().numpy(), *mv, step, 1e-2, 1e-2, eps=eps)
+        assert (np.abs(w.double().cpu().numpy() - want[0]) <= want[3]).all(), (step, (np.abs(w.double().cpu().numpy() - want[0]) / want[3]).max())
+
+
+@pytest.mark.gpu
 def test_not_finite_gradients():
     """Unclipped, a NaN or infinite gradient spoils its own element and, in 8 bits, no other of its block; clipped, the norm is not
     finite: NaN reaches every element, infinity its own (the others' factor is 0)."""
