@@ -184,7 +184,7 @@ int mcrn_flat_clip_adam(float* p, float* g, float* m, float* v, long long n, flo
  * gate (B,T,N,G), cand (B,T,N,H), G divides H (gate j is shared by the channels j*H/G .. (j+1)*H/G - 1), mask (B,T,N) bytes
  * or NULL: any strides (in elements, >= 0) over B, T and N, the last dimension of gate and cand contiguous.  state (B,N,H)
  * fp32 or NULL (zeros).  out (B,T,N,H) of the inputs' type, last (B,N,H) fp32.  Arithmetic and states are fp32.
- * B, T, N may be 0.  T <= 2^30; rows and nodes within a tile of at most 128 steps lie within 4 GB (strides of less than that).  `ws` belongs to
+ * B, T, N may be 0.  T <= 2^30, at most 2^24 - 1 blocks a launch (a block for 256 vectors of 4 channels of a sequence, at least one a sequence); rows and nodes within a tile of at most 128 steps lie within 4 GB (strides of less than that).  `ws` belongs to
  * the call until its kernels have run; it needs no initial contents. */
 #define MCRN_T_F32 0
 #define MCRN_T_BF16 1
@@ -213,7 +213,7 @@ int mcrn_glr_backward(const mcrn_glr_t* d, const void* gate, const void* cand, c
 /* ---- AdamW over many tensors, beside the flat clip + Adam above ----
  *   g' = factor g, factor = grad_scale * min(1, max_norm / (|| grad_scale g || + 1e-6)) over ALL tensors (max_norm <= 0: grad_scale)
  *   m = b1 m + (1 - b1) g' ; v = b2 v + (1 - b2) g' g' ; p = (1 - lr wd) p - lr / (1 - b1^s) * m / (sqrt(v) / sqrt(1 - b2^s) + eps)
- * Tensors are contiguous, fp32, or bf16 with fp32 masters that carry the update (p = their rounding).  The moments of all
+ * Tensors are contiguous, of at most 2^34 - 1024 elements, fp32, or bf16 with fp32 masters that carry the update (p = their rounding).  The moments of all
  * tensors lie in two arenas in the tensors' order, each tensor filled up with zeros to whole blocks of 64 elements
  * (mcrn_adamw_arena_elements): fp32, or one byte an element and one scale byte a block (value = code * 2^(scale - 127); m: sign, 4
  * exponent bits (bias 7), 3 mantissa bits; v: 5 exponent bits (bias 15), 3 mantissa bits; 0x7f and 0xff: NaN).  8-bit moments are

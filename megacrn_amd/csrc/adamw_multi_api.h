@@ -10,6 +10,8 @@ namespace mcrn {
 constexpr int ADAMW_BLOCK = 64;           // elements that share a scale of the 8-bit moments; the arenas' tensors start on it
 constexpr int ADAMW_TENSORS = 60;         // tensors a launch carries in its arguments (64 B each, below the 4 KB an argument block holds)
 
+constexpr long long ADAMW_BLOCKS = (1ll << 24) - 1;   // a launch counts its work items in 32 bits: blocks of 256, 1024 elements each
+
 enum { ADAMW_VEC = 1 };                   // AdamwT::flags: parameter and gradient can be read four elements at a time
 
 struct AdamwT {                           // one tensor of a launch

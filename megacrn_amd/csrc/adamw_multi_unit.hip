@@ -43,10 +43,13 @@ hipError_t launch_adamw_prep(const AdamwPrepP& p, hipStream_t st) {
 }
 hipError_t launch_adamw_unpack(const uint8_t* m, const uint8_t* ms, const uint8_t* v, const uint8_t* vs, long long n, float* om, float* ov, hipStream_t st) {
     (void)hipGetLastError();
-    const long long n4 = n / 4;
-    const dim3 grid((unsigned)((n4 + 255) / 256));
-    if (n * 10.0 > STREAM) hipLaunchKernelGGL((adamw_unpack_kernel<true>), grid, dim3(256), 0, st, m, ms, v, vs, om, ov, n4);
-    else hipLaunchKernelGGL((adamw_unpack_kernel<false>), grid, dim3(256), 0, st, m, ms, v, vs, om, ov, n4);
+    const bool nt = n * 10.0 > STREAM;
+    for (long long at = 0, most = 1ll << 33; at < n; at += most) {            // half of what a launch can hold, whole blocks of 64
+        const long long n4 = (n - at < most ? n - at : most) / 4;
+        const dim3 grid((unsigned)((n4 + 255) / 256));
+        if (nt) hipLaunchKernelGGL((adamw_unpack_kernel<true>), grid, dim3(256), 0, st, m + at, ms + at / ADAMW_BLOCK, v + at, vs + at / ADAMW_BLOCK, om + at, ov + at, n4);
+        else hipLaunchKernelGGL((adamw_unpack_kernel<false>), grid, dim3(256), 0, st, m + at, ms + at / ADAMW_BLOCK, v + at, vs + at / ADAMW_BLOCK, om + at, ov + at, n4);
+    }
     return hipGetLastError();
 }
 

@@ -2979,7 +2979,7 @@ int mcrn_glr_forward(const mcrn_glr_t* d, const void* gate, const void* cand, co
     p.gate = gate; p.cand = cand; p.mask = mask; p.h0 = state; p.out = out; p.last = last;
     p.ckpt = p.dtype == GLR_F32 ? nullptr : ckpt;
     if (!glr_aligned(p)) FAIL("glr_forward: a pointer is not aligned to its type");
-    if (!glr_plan(p, false)) FAIL("glr_forward: too many sequences");
+    if (!glr_plan(p, false)) FAIL("glr_forward: too many sequences (%d of %d channels): a launch holds %lld blocks", p.B, p.N * p.H, GLR_BLOCKS);
     if (!glr_near(p)) FAIL("glr_forward: strides over time and nodes reach over 4 GB within %d steps", glr_tile(p));
     if (!glr_workspace(p, false, ws, ws_bytes)) FAIL("glr_forward: the workspace is too small or not 256-byte aligned");
     fam(p.chain ? "glr:fwd_chain" : p.S > 1 ? "glr:fwd_split" : p.CL == 256 ? "glr:fwd_stream" : "glr:fwd_tile");
@@ -3000,7 +3000,7 @@ int mcrn_glr_backward(const mcrn_glr_t* d, const void* gate, const void* cand, c
     else p.ckpt = (float*)const_cast<void*>(kept);
     p.dout = dout; p.dlast = dlast; p.dgate = dgate; p.dcand = dcand; p.dstate = dstate;
     if (!glr_aligned(p)) FAIL("glr_backward: a pointer is not aligned to its type");
-    if (!glr_plan(p, true)) FAIL("glr_backward: too many sequences");
+    if (!glr_plan(p, true)) FAIL("glr_backward: too many sequences (%d of %d channels): a launch holds %lld blocks", p.B, p.N * p.H, GLR_BLOCKS);
     if (!glr_near(p)) FAIL("glr_backward: strides over time and nodes reach over 4 GB within %d steps", glr_tile(p));
     if (!glr_workspace(p, true, ws, ws_bytes)) FAIL("glr_backward: the workspace is too small or not 256-byte aligned");
     fam(p.chain ? "glr:bwd_chain" : p.S > 1 ? "glr:bwd_split" : p.CL == 256 ? "glr:bwd_stream" : "glr:bwd_tile");
@@ -3015,7 +3015,7 @@ static bool adamw_ok(const mcrn_adamw_t* a, const long long* numel) {
         return false;
     long long sum = 0;
     for (int i = 0; i < a->ntensors; ++i) {
-        if (numel[i] < 0 || numel[i] > (1ll << 40)) return false;
+        if (numel[i] < 0 || numel[i] > ADAMW_BLOCKS * 1024) return false;      // one launch reaches all of a tensor
         sum += (numel[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;
         if (sum > (1ll << 40)) return false;
     }
@@ -3090,7 +3090,7 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
             const long long n = numel[i], room = (n + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;
             if (grads[i] && n) {
                 const long long nb = (n + 1024ll * per - 1) / (1024ll * per);
-                if (nb + blocks >= (1ll << 31)) break;
+                if (nb + blocks > ADAMW_BLOCKS) break;     // (the next launch's first)
                 AdamwT& e = t[nt++];
                 e.p = params[i]; e.g = grads[i]; e.n = n; e.off = off; e.blk0 = blocks; e.id = i; e.pad = 0;
                 e.flags = (((uintptr_t)params[i] | (uintptr_t)grads[i]) % (4 * size)) == 0 ? ADAMW_VEC : 0;

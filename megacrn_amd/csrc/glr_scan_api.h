@@ -41,6 +41,7 @@ struct GlrP {
     unsigned *ticket, *carry;               // chunks taken of each tile, states behind the chunks (chain)
 };
 
+constexpr long long GLR_BLOCKS = (1ll << 24) - 1;     // a launch counts its work items in 32 bits: blocks of 256
 constexpr int GLR_K = 8;                    // steps a thread holds in registers, at most = distance of the checkpoints
 int glr_steps(int T);
 

@@ -61,7 +61,7 @@ bool glr_plan(GlrP& p, bool backward) {
         const int quarter = GLR_THREADS / 64 * GLR_K;
         if (p.T <= quarter || (p.T <= 9 * quarter && cover(64) >= 400)) {
             cover(64);
-        } else if ((blocks = cover(16)) * p.V * (long long)size >= 64 * 16 && p.T > span) {
+        } else if ((blocks = cover(16)) * p.V * (long long)size >= 64 * 16 && p.T > span && blocks * up_div(p.T, span) <= GLR_BLOCKS) {
             p.chain = true;
             p.chunk = span;
             p.S = (int)up_div(p.T, span);
@@ -74,7 +74,10 @@ bool glr_plan(GlrP& p, bool backward) {
             p.S = (int)up_div(p.T, p.chunk);
         }
     }
-    return p.tiles * p.CL < (1ll << 31) && (long long)p.N * p.G * p.parts < (1ll << 31) && p.tiles * p.B * p.S < (1ll << 31);
+    // indexes in 32 bits; the grids of the walk, of the chain's clearing and of the gates' parts
+    const long long words = p.chain ? p.tiles * p.B + (long long)p.S * p.B * NH : 0, sums = backward && p.parts > 1 ? (long long)p.B * p.T * p.N * p.G : 0;
+    return p.tiles * p.CL < (1ll << 31) && (long long)p.N * p.G * p.parts < (1ll << 31) && p.tiles * p.B * p.S <= GLR_BLOCKS &&
+           up_div(words, GLR_THREADS) <= GLR_BLOCKS && up_div(sums, GLR_THREADS) <= GLR_BLOCKS;
 }
 
 // [tickets | states] or [chunk aggregates], then the partial gate gradients; each part 256-byte aligned

@@ -268,7 +268,7 @@ void adamw_step(uintptr_t cfg_at, const std::vector<Tensor>& params, const std::
         const int rc = api.adamw_step(cfg, p.data(), g.data(), numel, reinterpret_cast<const double*>(lr), reinterpret_cast<const double*>(wd), step,
                                       m.mutable_data_ptr(), v.mutable_data_ptr(), (unsigned char*)data(ms), (unsigned char*)data(vs), (float*)data(master),
                                       ws.mutable_data_ptr(), (size_t)ws.numel(), (float*)data(norm), stream_of(m));
-        if (rc) count(-1);                                 // nothing was updated
+        if (rc) count(-1);                                 // refused before the first launch: nothing was updated
         return rc;
     });
     for (size_t i = 0; i < n; ++i)

@@ -69,6 +69,8 @@ class AdamW:
         self._cfg = Adamw(k, T_F32 if self.dtype == torch.float32 else T_BF16, state_bits, self.seed & 0xFFFFFFFF, int(self.capturable), 0, self.betas[0],
                           self.betas[1], self.eps, self.max_grad_norm, 1.0)
         n = lib.mcrn_adamw_arena_elements(C.byref(self._cfg), self._numel)
+        if n < 0:
+            raise ValueError("AdamW: a parameter has more than 2^34 - 1024 elements, or there are more than 2^20")
         dev = self.device
         if state_bits == 32:
             self._m, self._v = torch.zeros(n, device=dev), torch.zeros(n, device=dev)

@@ -74,6 +74,19 @@ def test_arena_and_workspace_sizes():
     assert lib.mcrn_adamw_arena_elements(cfg(), (C.c_longlong * 4)(1, -1, 65, 0)) == -1
 
 
+def test_sizes_that_no_launch_holds():
+    """A launch has fewer than 2^32 work items, 2^24 blocks of 256 threads and 1024 elements: what lies beyond is refused with the sizes, not by a
+    launch after others have updated their tensors."""
+    import ctypes as C
+    from megacrn_amd._lib import lib, Adamw
+    cfg = C.byref(Adamw(2, 1, 8, 0, 0, 0, 0.9, 0.999, 1e-8, 1.0, 1.0))
+    most = 2 ** 34 - 1024
+    for n, ok in ((most, True), (most + 1, False), (2 ** 40, False)):
+        sizes = (C.c_longlong * 2)(100, n)
+        assert lib.mcrn_adamw_arena_elements(cfg, sizes) == ((128 + most) if ok else -1)
+        assert (lib.mcrn_adamw_workspace_bytes(cfg, sizes) > 0) == ok
+
+
 P = torch.nn.Parameter
 
 

@@ -128,6 +128,20 @@ def test_c_sizes():
         assert ws(*bad) == 0
 
 
+def test_c_sizes_of_many_chunks():
+    """300 sequences of 2^23 steps and one channel: chained chunks of 128 steps would be 300 x 2^16 blocks, more than a launch holds (2^24 - 1), so
+    they are split (at most 256 chunks, two floats each); half as long they are chained."""
+    import ctypes as C
+    from megacrn_amd._lib import lib
+
+    class Glr(C.Structure):                                # mcrn_glr_t
+        _fields_ = [("i", C.c_int * 8), ("s", C.c_longlong * 12)]
+    f = lib.mcrn_glr_workspace_bytes
+    f.restype, f.argtypes = C.c_size_t, [C.POINTER(Glr), C.c_int]
+    ws = [f(C.byref(Glr((C.c_int * 8)(300, T, 1, 1, 1, 0, 1, 0))), back) for T in (2 ** 23, 2 ** 22) for back in (0, 1)]
+    assert max(ws[:2]) <= 256 * 300 * 2 * 4 + 256 and min(ws[2:]) >= 300 * 2 ** 15 * 4
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # on the GPU
 # ---------------------------------------------------------------------------------------------------------------------
@@ -523,6 +537,20 @@ def test_many_elements():
     for b in range(B):
         assert torch.equal(out[b], cand[b])
     assert torch.equal(last, cand[:, -1].float())
+
+
+@pytest.mark.gpu
+def test_as_many_sequences_as_a_launch_holds():
+    """2^24 - 1 sequences of one channel are one launch; one more is refused before it."""
+    import megacrn_amd
+    B = 2 ** 24 - 1
+    cand = torch.arange(B, device="cuda", dtype=torch.float32).view(B, 1, 1, 1)
+    gate = torch.full((1, 1, 1, 1), -200.0, device="cuda")
+    out, last = megacrn_amd.gated_linear_recurrence(gate.expand(B, 1, 1, 1), cand, activation="none")
+    assert torch.equal(out, cand) and torch.equal(last, cand[:, 0])
+    many = torch.zeros(1, 1, 1, 1, device="cuda").expand(B + 1, 1, 1, 1)
+    with pytest.raises(RuntimeError, match="too many sequences"):
+        megacrn_amd.gated_linear_recurrence(many, many)
 
 
 @pytest.mark.gpu
