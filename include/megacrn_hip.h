@@ -21,9 +21,9 @@
  *  - Return value: 0 on success, otherwise a hipError_t (>0) or
  *    MCRN_EINVAL (-1) for unsupported arguments; mcrn_last_error() returns a
  *    static message.
- *  - Process model: ONE host thread and ONE device per process (one process per GPU).  The library keeps a
- *    process-wide helper stream, tile cache and profiler; every compute entry point refuses (MCRN_EINVAL) a call
- *    that arrives while another host thread is inside the library, or on a different device than the first call.
+ *  - Process model: ONE device per process (one process per GPU).  The library keeps a process-wide helper stream, tile
+ *    cache and profiler; calls of several host threads take turns, and every compute entry point refuses (MCRN_EINVAL) a
+ *    call on a different device than the first one's.  mcrn_last_error() is that of the calling thread.
  *  - Supported: cheb_k in 2 .. 8 (model/MegaCRN.py:21-22 recurses for any cheb_k >= 2; 2 and 3 have the fused fast
  *    paths, larger orders run the recursion step by step on the tiled GEMM; MCRN_BF16: 2 or 3); any B,N,H,
  *    input/output/ycov dims >= 1; num_layers == 1 in the fused model entry points (multi-layer models are

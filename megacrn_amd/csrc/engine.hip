@@ -17,7 +17,7 @@
 #include <map>
 #include <algorithm>
 #include <stdlib.h>
-#include <atomic>
+#include <mutex>
 #include <vector>
 
 #include "../../include/megacrn_hip.h"
@@ -40,7 +40,7 @@ static bool g_prop_bf16 = false;        // MCRN_BF16: propagation / its transpos
                                         // (gemm_bf16.h); every other contraction keeps the bf16x3 arithmetic
 static bool g_x3r = false;              // ... with hi/lo operand PAIRS and three MFMAs per product (gemm_bf16.h, nterm = 3): what a bf16x3 session
                                         // runs on the large graphs since round 5 - the bf16 mode's data flow in the 1e-4 arithmetic (ModelPlan::x3r)
-static char g_err[512] = "";
+static thread_local char g_err[512] = "";      // of the calling thread's last failure
 static int g_launches = 0;
 
 #define CK(expr)                                                                              \
@@ -71,20 +71,14 @@ static int g_launches = 0;
     } while (0)
 
 // ---- process-global state guard ------------------------------------------------------------------
-// The library keeps ONE helper stream, tile cache, profiler and arithmetic mode per process:
-// its launch model is one process per GPU with one host thread driving it.  A second host thread inside the
-// library at the same time, or a call on a second device, would silently share that state - both are refused.
-static std::atomic<int> g_busy{0};
+// The library keeps ONE helper stream, tile cache, profiler and arithmetic mode per process: its launch model is one process per GPU.
+// Calls of several host threads take turns (a call only enqueues, autotuning apart): a backward pass runs on autograd's thread while another
+// one of the program may serve.  A call on a second device would silently share that state and is refused.
+static std::mutex g_turn;
 static int g_device = -1;
 struct CallGuard {
-    bool entered = false;
+    std::lock_guard<std::mutex> lock{g_turn};
     int enter() {
-        if (g_busy.exchange(1, std::memory_order_acquire) != 0) {
-            // (g_err is shared too: the message is best-effort, the return code is what counts)
-            snprintf(g_err, sizeof g_err, "libmegacrn_hip: concurrent call from a second host thread (one host thread per process)");
-            return MCRN_EINVAL;
-        }
-        entered = true;
         int dev = -1;
         if (hipGetDevice(&dev) != hipSuccess) { snprintf(g_err, sizeof g_err, "hipGetDevice failed"); return MCRN_EINVAL; }
         if (g_device < 0) g_device = dev;
@@ -95,7 +89,6 @@ struct CallGuard {
         }
         return 0;
     }
-    ~CallGuard() { if (entered) g_busy.store(0, std::memory_order_release); }
 };
 #define ENTER()                                                                               \
     CallGuard guard__;                                                                        \

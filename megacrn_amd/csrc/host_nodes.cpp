@@ -11,8 +11,6 @@
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
-#include <mutex>
-
 #include "../../include/megacrn_hip.h"
 
 namespace {
@@ -42,11 +40,9 @@ void bind(const pybind11::dict& d) {
     take(d, "mcrn_adamw_unpack", api.adamw_unpack);
 }
 
-// The library takes one host thread at a time.  A backward pass runs on the autograd engine's thread without the interpreter lock, while another
-// thread of the program may take a step: they wait for one another here.
-std::mutex one_at_a_time;
+// A backward pass runs on the autograd engine's thread without the interpreter lock, while another thread of the program may take a step: they take
+// turns in the library, whose last error is the calling thread's own.
 template <class F> void call(const char* what, F f) {
-    const std::lock_guard<std::mutex> lock(one_at_a_time);
     const int rc = f();
     TORCH_CHECK(rc == 0, what, " failed (rc=", rc, "): ", api.last_error());
 }

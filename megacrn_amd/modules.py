@@ -40,20 +40,20 @@ def _p(t):
 
 
 class _WsPool:
-    """Free-list of workspace buffers keyed by size.  A buffer that holds saved activations is
-    owned by the autograd node until its backward has run."""
+    """Free-list of workspace buffers keyed by size and stream (a buffer is given back while the kernels that read it are still
+    queued there).  A buffer that holds saved activations is owned by the autograd node until its backward has run."""
 
     def __init__(self):
         self.free = {}
 
     def take(self, nbytes: int, device) -> torch.Tensor:
-        lst = self.free.get((nbytes, str(device)))
+        lst = self.free.get((nbytes, str(device), _stream()))
         if lst:
             return lst.pop()
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
     def give(self, ws: torch.Tensor) -> None:
-        self.free.setdefault((ws.numel(), str(ws.device)), []).append(ws)
+        self.free.setdefault((ws.numel(), str(ws.device), _stream()), []).append(ws)
 
 
 _pool = _WsPool()

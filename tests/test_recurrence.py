@@ -678,6 +678,53 @@ def test_two_threads():
 
 
 @pytest.mark.gpu
+def test_cells_on_two_threads_and_streams():
+    """A cell trains on one thread and stream while another one serves on its own: the graph convolution's calls and workspaces are part of it."""
+    import threading
+    import megacrn_amd
+    torch.manual_seed(5)
+    B, T, N, C, H, K = 2, 12, 20, 3, 16, 3
+    cells = [megacrn_amd.AGLRCell(N, C, H, K).cuda() for _ in range(2)]
+    sup = [torch.softmax(torch.randn(N, N, device="cuda"), -1) for _ in range(2)]
+    x, st = torch.randn(B, T, N, C, device="cuda"), torch.randn(B, N, H, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def train(got):
+        with torch.cuda.stream(streams[0]):
+            for _ in range(60):
+                out, last = cells[0](x, st, sup)
+                got[:] = [out.detach(), *torch.autograd.grad(out.sum() + last.sum(), list(cells[0].parameters()))]
+
+    def serve(got):
+        with torch.cuda.stream(streams[1]):
+            for _ in range(20):
+                now = st.clone()
+                for t in range(T):
+                    cells[1].step(x[:, t], now, sup)
+                out, _ = cells[1](x, st, sup)              # the training thread's sizes, its own workspace
+                got[:] = [now, out.detach()]
+    alone, both, errors = [[], []], [[], []], []
+    train(alone[0]), serve(alone[1])
+    torch.cuda.synchronize()
+
+    def guarded(f, got):
+        try:
+            f(got)
+        except Exception as e:
+            errors.append(e)
+    threads = [threading.Thread(target=guarded, args=(f, got)) for f, got in zip((train, serve), both)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    for a, b in zip(alone, both):
+        assert len(a) == len(b) and all(torch.allclose(p, q, rtol=1e-5, atol=1e-6 * p.abs().max().item()) for p, q in zip(a, b))
+
+
+@pytest.mark.gpu
 def test_agl_cell_training_run():
     """The module as it is used: supports -> graph convolution of all steps -> recurrence -> loss -> gradients, against float64; then
     its steps in place against the sequence, and an AdamW update of all its parameters."""
