@@ -154,12 +154,23 @@ def _load():
 lib = _load()
 
 
+class _NoHost:
+    """Stands for host nodes that are not there: the recurrence and AdamW raise, the rest of the package does without them."""
+
+    def __init__(self, why):
+        self._why = why
+
+    def __getattr__(self, name):
+        raise ImportError(f"megacrn_amd/_host.so is missing or does not load ({self._why}): the gated linear recurrence and AdamW need it; "
+                          "build it with `make -C megacrn_amd/csrc host`")
+
+
 def _load_host():
     """The C++ host nodes (csrc/host_nodes.cpp) call the library that is loaded here, through the addresses they get."""
     try:
         from . import _host
     except ImportError as e:
-        raise ImportError(f"megacrn_amd/_host.so is missing or does not load ({e}): build it with `make -C megacrn_amd/csrc host`") from e
+        return _NoHost(str(e))
     _host.bind({s: C.cast(getattr(lib, s), C.c_void_p).value
                 for s in ("mcrn_last_error", "mcrn_glr_checkpoint_floats", "mcrn_glr_workspace_bytes", "mcrn_glr_forward",
                           "mcrn_glr_backward", "mcrn_adamw_step", "mcrn_adamw_unpack")})

@@ -60,6 +60,7 @@ class AdamW:
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("AdamW: two parameters share memory")
+        host.adamw_step                        # raises where the host nodes are not built
         _need_gpu(first, "AdamW")
         self.device, self.dtype = first.device, first.dtype
         self.betas, self.eps, self.max_grad_norm = tuple(betas), float(eps), float(max_grad_norm or 0.0)

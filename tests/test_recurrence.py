@@ -128,6 +128,26 @@ def test_c_sizes():
         assert ws(*bad) == 0
 
 
+def test_package_without_its_host_nodes():
+    """_host.so missing: the package imports, its recurrence and optimizer say what to build."""
+    import subprocess
+    import sys
+    code = ("import sys; sys.modules['megacrn_amd._host'] = None\n"
+            "import torch, megacrn_amd\n"
+            "megacrn_amd.AGCN(1, 2, 3)\n"
+            "x = torch.zeros(1, 1, 1, 1)\n"
+            "for f in (lambda: megacrn_amd.gated_linear_recurrence(x, x), lambda: megacrn_amd.gated_linear_recurrence_step(x[0], x[0], x[0]),\n"
+            "          lambda: megacrn_amd.AdamW([x])):\n"
+            "    try:\n"
+            "        f()\n"
+            "    except ImportError as e:\n"
+            "        assert 'make -C megacrn_amd/csrc host' in str(e)\n"
+            "    else:\n"
+            "        raise SystemExit('no error')\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_c_sizes_of_many_chunks():
     """300 sequences of 2^23 steps and one channel: chained chunks of 128 steps would be 300 x 2^16 blocks, more than a launch holds (2^24 - 1), so
     they are split (at most 256 chunks, two floats each); half as long they are chained."""
