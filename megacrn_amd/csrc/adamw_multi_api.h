@@ -31,7 +31,7 @@ struct AdamwDyn { float step_size, inv_bc2, decay; unsigned key; };   // the sam
 
 struct AdamwP {
     AdamwT t[ADAMW_TENSORS];
-    int nt, per;                          // tensors; runs of 1024 elements a block
+    int nt;                               // tensors; a block works on 1024 elements
     void *m, *v;                          // arenas: float, or codes
     uint8_t *ms, *vs;                     // scale bytes, one for each 64 elements
     float* master;                        // arena of fp32 parameters (16-bit ones only)
@@ -45,7 +45,7 @@ struct AdamwP {
 };
 struct AdamwNormP {
     AdamwT t[ADAMW_TENSORS];
-    int nt, per;
+    int nt, per;                          // tensors; runs of 1024 elements a block
     unsigned blk0;                        // first partial sum of this launch
     double* part;
 };

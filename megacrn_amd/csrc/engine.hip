@@ -3057,8 +3057,6 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     AdamwDyn* dyn = (AdamwDyn*)((char*)part + (elements / (1024ll * runs_n) + a->ntensors) * 8);
     const bool clip = a->max_norm > 0;
     unsigned parts = 0;
-    // One run a block: 634 us at 132 M fp32 parameters, 654 - 671 with 2 - 8; 353 against 362 - 408 in bf16 with 8-bit moments.
-    const int runs = 1;
     const bool many = live > (4ll << 20);      // over 4096 blocks: the factor is worth a launch of its own (adamw_factor_kernel)
 
     if (a->on_device) {
@@ -3127,9 +3125,9 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     }
     long long off = 0;
     for (int i = 0; i < a->ntensors;) {
-        const unsigned blocks = fill(i, off, q.t, q.nt, runs, true);
+        const unsigned blocks = fill(i, off, q.t, q.nt, 1, true);
         if (!blocks) continue;
-        q.per = runs; q.m = m; q.v = v; q.ms = m_scale; q.vs = v_scale; q.master = master; q.dyn = a->on_device ? dyn : nullptr;
+        q.m = m; q.v = v; q.ms = m_scale; q.vs = v_scale; q.master = master; q.dyn = a->on_device ? dyn : nullptr;
         q.b1 = (float)a->beta1; q.c1 = (float)(1.0 - a->beta1); q.b2 = (float)a->beta2; q.c2 = (float)(1.0 - a->beta2); q.eps = (float)a->eps;
         fam(a->state_bits == 8 ? "adamw:8bit" : "adamw:32bit");
         CK(launch_adamw(q, blocks, live, a->dtype, a->state_bits, st));
