@@ -3042,11 +3042,13 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     const size_t need = mcrn_adamw_workspace_bytes(a, numel);
     if (ws_bytes < need) FAIL("adamw_step: the workspace needs %zu bytes", need);
     const uintptr_t size = a->dtype == MCRN_T_F32 ? 4 : 2;
-    long long elements = 0, live = 0;
+    long long elements = 0, live = 0, runs = 0, tensors = 0;
     for (int i = 0; i < a->ntensors; ++i) {
         elements += (numel[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK * ADAMW_BLOCK;
         if (!grads[i] || !numel[i]) continue;
         live += numel[i];
+        runs += (numel[i] + 1023) / 1024;
+        ++tensors;
         if (!params[i] || ((uintptr_t)params[i] | (uintptr_t)grads[i]) % size) FAIL("adamw_step: tensor %d has no parameter, or one that is not aligned to its type", i);
         if (!a->on_device && step[i] < 1) FAIL("adamw_step: step of tensor %d is %d, the first is 1", i, step[i]);
     }
@@ -3057,8 +3059,6 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     AdamwDyn* dyn = (AdamwDyn*)((char*)part + (elements / (1024ll * runs_n) + a->ntensors) * 8);
     const bool clip = a->max_norm > 0;
     unsigned parts = 0;
-    const bool many = live > (4ll << 20);      // over 4096 blocks: the factor is worth a launch of its own (adamw_factor_kernel)
-
     if (a->on_device) {
         for (int base = 0; base < a->ntensors; base += 4096) {
             AdamwPrepP q;
@@ -3118,7 +3118,10 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
     AdamwP q;
     q.part = part; q.parts = (int)parts; q.max_norm = (float)a->max_norm; q.norm = clip ? total_norm : nullptr; q.grad_scale = (float)a->grad_scale;
     q.factor = nullptr;
-    if (clip && many) {
+    // Every block adding the sums for itself saves a launch (adamw_factor_kernel), and costs more than one above 2^21 additions in all (4 M elements: 4096
+    // blocks, 512 sums) or where many launches of small tensors wait for it one after the other (700 tensors of 300 elements: 79 us either way; 800: 78
+    // and 92, 2000: 175 and 223, 10000: 990 and 1783)
+    if (clip && (runs * parts > (1ll << 21) || tensors * parts > 60 * 8192)) {
         CK(launch_adamw_factor(q, (float*)ws, st));
         ++g_launches;
         q.factor = (const float*)ws;

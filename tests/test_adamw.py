@@ -277,6 +277,26 @@ def test_more_tensors_than_a_launch_carries(count):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("count", [701, 900, 1500])
+def test_many_small_tensors(count, dt):
+    """As many sums as tensors, added by every block or (from 702 on) once: one norm, one factor for all."""
+    import megacrn_amd
+    shapes = [(1 + (7 * i) % 20,) for i in range(count)]
+    ps, gs = _make(shapes, dt, 5)
+    opt = megacrn_amd.AdamW(ps, lr=1e-2, max_grad_norm=0.5)
+    before = torch.cat([p.double() for p in ps])
+    opt.step(grads=gs)
+    g = torch.cat([x.double() for x in gs])
+    norm = g.norm().item()
+    assert abs(opt.total_norm.item() - norm) <= 1.01 * O.U * norm
+    z = np.zeros(g.numel())
+    want = O.adamw_step(before.cpu().numpy(), g.cpu().numpy(), z, z, 1, 1e-2, 1e-2, factor=min(1.0, 0.5 / (norm + 1e-6)))
+    got = ps if opt.master is None else [opt.master[o:o + p.numel()] for o, p in zip(opt.offsets, ps)]
+    assert (np.abs(torch.cat([p.double() for p in got]).cpu().numpy() - want[0]) <= want[3]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_large_tensor_and_groups(bits):
     """Blocks of several runs (over 4 M elements), two groups with rates and decays of their own, and the same numbers whichever way
