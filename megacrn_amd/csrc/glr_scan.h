@@ -384,6 +384,10 @@ __global__ __launch_bounds__(GLR_THREADS, (MODE == GLR_WALK && CL < 256) || (GAT
 #pragma unroll
             for (int i = 0; i < V; ++i) carry[i] = p.h0[w.b * NH + hoff + i];
         }
+        if (SEG > 1 && p.last == p.h0) {                   // in place: every wave has its state before the first barrier, behind which another may overwrite it
+#pragma unroll
+            for (int i = 0; i < V; ++i) GLR_HERE(carry[i]);
+        }
         if (!CHAIN && CL == 16 && w.chunk > 0) {           // the chunks before this one
             const long long step = (long long)p.B * 2 * NH;
             glr_chunks_before<V, CL>(lds[1], w, p.agg + (long long)w.b * 2 * NH + hoff, step, NH, w.chunk, carry);
