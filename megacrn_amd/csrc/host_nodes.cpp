@@ -6,6 +6,7 @@
 // threads), where the kernels of a METR-LA training window take 60.  A serving step: 18 us before, 4.5 now.
 // The library is not linked: `bind` takes the addresses of its entry points from the one that Python has loaded.
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
 #include <ATen/DeviceGuard.h>
@@ -69,6 +70,7 @@ int activation_of(const std::string& name, const char* who) {
 
 // Everything that the C entry points cannot see in raw pointers; returns the mask expanded to (B, T, N) or (B, N).
 Tensor check_inputs(const Tensor& gate, const Tensor& cand, const Tensor& state, const Tensor& mask, const char* who, int64_t lead) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), who, " cannot be traced: a trace would hold the allocation of its outputs and not what fills them");
     for (const Tensor* t : {&gate, &cand})
         TORCH_CHECK_TYPE(type_of(t->scalar_type()) >= 0, who, ": gate and cand must be float32, bfloat16 or float16; got ", t->scalar_type());
     TORCH_CHECK_VALUE(cand.dim() == lead + 1 && gate.dim() == lead + 1 && gate.sizes().slice(0, lead) == cand.sizes().slice(0, lead), who,

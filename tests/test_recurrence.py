@@ -128,6 +128,39 @@ def test_c_sizes():
         assert ws(*bad) == 0
 
 
+@pytest.mark.parametrize("where", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_tracing_is_refused(where):
+    """torch.jit.trace would record that outputs are allocated, and nothing else."""
+    import warnings
+    import megacrn_amd
+    a = [torch.zeros(2, 3, 4, 8, device=where) for _ in range(2)]
+    b = [t[:, 0].contiguous() for t in (*a, a[0])]
+    for f, args in ((lambda x, y: megacrn_amd.gated_linear_recurrence(x, y)[0], a), (lambda x, y, s: megacrn_amd.gated_linear_recurrence_step(x, y, s), b)):
+        with warnings.catch_warnings(), pytest.raises(RuntimeError, match="cannot be traced"):
+            warnings.simplefilter("ignore")
+            torch.jit.trace(f, tuple(args), check_trace=False)
+
+
+@pytest.mark.gpu
+def test_transforms_are_refused():
+    """Tensors that stand for others (vmap, functional gradients, fake ones) have no memory that a kernel could read: an error, no numbers."""
+    import megacrn_amd
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x = torch.zeros(2, 2, 3, 4, 8, device="cuda")
+    f = megacrn_amd.gated_linear_recurrence
+    with pytest.raises(Exception):
+        torch.vmap(lambda t: f(t, t)[0])(x)
+    with pytest.raises(Exception):
+        torch.func.grad(lambda t: f(t, t)[0].sum())(x[0])
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda t: f(t, t)[0], (x[0],), (x[0],))
+    one = x[0].clone()
+    with FakeTensorMode() as mode:
+        t = mode.from_tensor(one)
+        with pytest.raises(Exception):
+            f(t, t)
+
+
 def test_package_without_its_host_nodes():
     """_host.so missing: the package imports, its recurrence and optimizer say what to build."""
     import subprocess
