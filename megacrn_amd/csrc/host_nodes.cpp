@@ -206,6 +206,15 @@ std::pair<Tensor, Tensor> glr(const Tensor& gate0, const Tensor& cand0, const Op
     return {r.out, r.last};
 }
 
+// The input, or a copy where it lies in memory that the step overwrites: a thread advances its channel while another one still reads
+Tensor apart(const Tensor& t, const Tensor& state) {
+    if (!t.defined() || !t.is_alias_of(state) || t.numel() == 0) return t;
+    int64_t reach = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) reach += (t.size(i) - 1) * t.stride(i);
+    const auto at = (uintptr_t)t.const_data_ptr(), to = (uintptr_t)state.const_data_ptr();
+    return at < to + state.nbytes() && to < at + reach * t.element_size() ? t.clone() : t;
+}
+
 Tensor glr_step(const Tensor& gate0, const Tensor& cand0, const OptTensor& state0, const OptTensor& mask0, const std::string& activation) {
     const char* who = "gated_linear_recurrence_step";
     const int act = activation_of(activation, who);
@@ -214,7 +223,7 @@ Tensor glr_step(const Tensor& gate0, const Tensor& cand0, const OptTensor& state
     const Tensor mask = check_inputs(gate0, cand0, state, mask0.value_or(Tensor()), who, 2);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (gate0.requires_grad() || cand0.requires_grad() || state.requires_grad())), who,
                 " is not differentiable: call it under torch.no_grad()");
-    const Tensor gate = rows(gate0, 2), cand = rows(cand0, 2), out = at::empty(cand.sizes(), cand.options());
+    const Tensor gate = rows(apart(gate0, state), 2), cand = rows(apart(cand0, state), 2), out = at::empty(cand.sizes(), cand.options());
     if (out.numel() == 0) return out;
     const at::DeviceGuard guard(cand.device());
     const mcrn_glr_t d = dims_of(gate, cand, mask, Tensor(), act, 2);

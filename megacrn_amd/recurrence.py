@@ -36,7 +36,7 @@ def gated_linear_recurrence(gate, cand, state=None, mask=None, activation="tanh"
 
 def gated_linear_recurrence_step(gate, cand, state, mask=None, activation="tanh"):
     """One step of the recurrence for serving: gate (B, N, G), cand (B, N, H), mask (B, N) or (B,).  `state` (B, N, H) float32,
-    contiguous, is advanced in place; returns it in the inputs' type as a new tensor.  Not differentiable."""
+    contiguous, is advanced in place (inputs may lie in its memory); returns it in the inputs' type as a new tensor.  Not differentiable."""
     return host.glr_step(gate, cand, state, mask, activation)
 
 

@@ -436,6 +436,21 @@ def test_steps_are_the_sequence(dt, G):
 
 
 @pytest.mark.gpu
+def test_step_whose_inputs_lie_in_its_state():
+    """A gate or a candidate that is a view of the state, or of memory that overlaps it, is what it was before the step."""
+    import megacrn_amd
+    N, H = 300, 1100
+    buf = torch.randn(1, N + 1, H, device="cuda")
+    for pick in (lambda b: (b[:, :N, :1], b[:, 1:]), lambda b: (b[:, 1:], b[:, :N, :]), lambda b: (b[:, :N], b[:, :N]), lambda b: (b[:, 1:], b[:, :1].expand(1, N, H)),
+                 lambda b: (b[:, -1:].expand(1, N, H), b[:, :1].expand(1, N, H))):
+        a, want = buf.clone(), buf.clone()
+        ref = want[:, :N].clone()
+        out_ref = megacrn_amd.gated_linear_recurrence_step(*(t.clone() for t in pick(want)), ref)
+        out = megacrn_amd.gated_linear_recurrence_step(*pick(a), a[:, :N])
+        assert torch.equal(out, out_ref) and torch.equal(a[:, :N], ref) and torch.equal(a[:, N:], buf[:, N:])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("B,T,N,H", [(2, 1, 3, 8), (2, 5, 3, 8), (2, 30, 3, 8), (2, 300, 3, 8), (1, 300, 40, 64), (64, 20, 40, 256)])
 def test_state_of_a_masked_row_is_kept_whatever_it_is(B, T, N, H, dt):
