@@ -103,8 +103,11 @@ void strides_of(const Tensor& t, int64_t lead, long long* s) {
     const int64_t at[3] = {0, lead == 3 ? 1 : -1, lead - 1};
     for (int i = 0; i < 3; ++i) s[i] = at[i] < 0 || t.size(at[i]) == 1 ? 0 : t.stride(at[i]);
 }
+// A view that is negative by a bit (the imaginary part of a conjugate): its memory holds the other sign
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // The kernels want a last dimension without gaps, and a tile's rows (128 steps at most) within 4 GB of each other: a copy where that is not so.
-Tensor rows(const Tensor& t, int64_t lead) {
+Tensor rows(const Tensor& t0, int64_t lead) {
+    const Tensor t = plain(t0);
     if (!t.defined()) return t;
     long long s[3];
     strides_of(t, lead, s);
@@ -157,7 +160,7 @@ Sequence glr_run(const Tensor& gate, const Tensor& cand, const Tensor& state, co
 
 struct GlrNode : torch::autograd::Function<GlrNode> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, Tensor gate, Tensor cand, OptTensor state, OptTensor mask, int64_t act) {
-        Tensor h0 = state ? state->contiguous() : Tensor(), m = mask.value_or(Tensor());
+        Tensor h0 = state ? plain(*state).contiguous() : Tensor(), m = mask.value_or(Tensor());
         const Sequence r = glr_run(gate, cand, h0, m, (int)act, true);
         // fp32: the backward reads the states before every 8th step from `out` itself; the 16-bit types keep those in fp32
         ctx->save_for_backward({gate, cand, h0, m, cand.scalar_type() == at::kFloat ? r.out : r.ckpt});
@@ -172,7 +175,7 @@ struct GlrNode : torch::autograd::Function<GlrNode> {
         const auto s = ctx->get_saved_variables();
         const Tensor &gate = s[0], &cand = s[1], &h0 = s[2], &mask = s[3], &kept = s[4];
         const at::DeviceGuard guard(cand.device());
-        const Tensor dout = rows(g[0], 3), dlast = g[1].defined() ? g[1].contiguous() : Tensor();
+        const Tensor dout = rows(g[0], 3), dlast = g[1].defined() ? plain(g[1]).contiguous() : Tensor();
         const mcrn_glr_t d = dims_of(gate, cand, mask, dout, (int)ctx->saved_data["act"].toInt(), 3);
         out[0] = at::empty(gate.sizes(), gate.options());
         out[1] = at::empty(cand.sizes(), cand.options());
@@ -202,7 +205,7 @@ std::pair<Tensor, Tensor> glr(const Tensor& gate0, const Tensor& cand0, const Op
         auto r = GlrNode::apply(gate, cand, state, mask.defined() ? OptTensor(mask) : OptTensor(), (int64_t)act);
         return {r[0], r[1]};
     }
-    const Sequence r = glr_run(gate, cand, h0.defined() ? h0.contiguous() : h0, mask, act, false);
+    const Sequence r = glr_run(gate, cand, h0.defined() ? plain(h0).contiguous() : h0, mask, act, false);
     return {r.out, r.last};
 }
 
@@ -219,7 +222,7 @@ Tensor glr_step(const Tensor& gate0, const Tensor& cand0, const OptTensor& state
     const char* who = "gated_linear_recurrence_step";
     const int act = activation_of(activation, who);
     const Tensor state = state0.value_or(Tensor());
-    TORCH_CHECK_VALUE(state.defined() && state.is_contiguous(), who, ": state must be a contiguous tensor; it is advanced in place");
+    TORCH_CHECK_VALUE(state.defined() && state.is_contiguous() && !state.is_neg(), who, ": state must be a contiguous tensor; it is advanced in place");
     const Tensor mask = check_inputs(gate0, cand0, state, mask0.value_or(Tensor()), who, 2);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (gate0.requires_grad() || cand0.requires_grad() || state.requires_grad())), who,
                 " is not differentiable: call it under torch.no_grad()");
@@ -252,15 +255,15 @@ void adamw_step(uintptr_t cfg_at, const std::vector<Tensor>& params, const std::
     for (size_t i = 0; i < n; ++i) {
         if (!grads[i] || !grads[i]->defined()) continue;
         const Tensor &a = params[i], &b = *grads[i];
-        TORCH_CHECK_VALUE(a.scalar_type() == type && a.device() == dev && a.is_contiguous() && a.numel() == numel[i], "AdamW.step: parameter ", i,
+        TORCH_CHECK_VALUE(a.scalar_type() == type && a.device() == dev && a.is_contiguous() && !a.is_neg() && a.numel() == numel[i], "AdamW.step: parameter ", i,
                           " is no longer the contiguous ", type, " tensor that the optimizer was made for");
         TORCH_CHECK_VALUE(b.scalar_type() == type && b.device() == dev && b.layout() == at::kStrided && b.sizes() == a.sizes(), "AdamW.step: gradient ", i,
                           " must be a ", type, " tensor of shape ", a.sizes(), " on ", dev);
         no_tangent(a, "AdamW.step");
         no_tangent(b, "AdamW.step");
         p[i] = a.mutable_data_ptr();
-        if (b.is_contiguous()) g[i] = b.const_data_ptr();
-        else g[i] = held.emplace_back(b.contiguous()).const_data_ptr();
+        if (b.is_contiguous() && !b.is_neg()) g[i] = b.const_data_ptr();
+        else g[i] = held.emplace_back(plain(b).contiguous()).const_data_ptr();
     }
     auto data = [](const OptTensor& t) { return t ? t->mutable_data_ptr() : nullptr; };
     const at::DeviceGuard guard(dev);

@@ -436,18 +436,44 @@ def test_steps_are_the_sequence(dt, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H", [8, 1])
+def test_views_that_are_negative_by_a_bit(H):
+    """The imaginary part of a conjugate holds its numbers with the other sign in memory; a last dimension of 1 is read in place whatever its stride."""
+    import megacrn_amd
+    torch.manual_seed(1)
+    z = torch.randn(5, 2, 7, 3, H, dtype=torch.complex64, device="cuda")
+    neg = z.conj().imag
+    assert neg.is_neg()
+    real = neg.resolve_neg()
+    grads = []
+    for t in (neg, real):
+        leaves = [t[0].detach().requires_grad_(), t[1].detach(), t[2, :, 0].detach()]
+        out, last = megacrn_amd.gated_linear_recurrence(*leaves)
+        (g,) = torch.autograd.grad((out, last), leaves[:1], (t[3], t[4, :, 0]))
+        now = real[2, :, 0].contiguous()
+        with torch.no_grad():
+            grads.append((out, last, g, megacrn_amd.gated_linear_recurrence_step(t[0, :, 0], t[1, :, 0], now), now, megacrn_amd.gated_linear_recurrence(*leaves)[0]))
+        p = torch.ones(2, 7, 3, H, device="cuda")
+        megacrn_amd.AdamW([p]).step(grads=[t[0]])
+        grads[-1] += (p,)
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    with pytest.raises(ValueError):
+        megacrn_amd.gated_linear_recurrence_step(real[0, :, 0], real[1, :, 0], torch._neg_view(torch.empty(2, 3, H, device="cuda")))
+
+
+@pytest.mark.gpu
 def test_step_whose_inputs_lie_in_its_state():
     """A gate or a candidate that is a view of the state, or of memory that overlaps it, is what it was before the step."""
     import megacrn_amd
-    N, H = 300, 1100
+    N, H = 20000, 1100
     buf = torch.randn(1, N + 1, H, device="cuda")
-    for pick in (lambda b: (b[:, :N, :1], b[:, 1:]), lambda b: (b[:, 1:], b[:, :N, :]), lambda b: (b[:, :N], b[:, :N]), lambda b: (b[:, 1:], b[:, :1].expand(1, N, H)),
-                 lambda b: (b[:, -1:].expand(1, N, H), b[:, :1].expand(1, N, H))):
+    for pick in (lambda b: (b[:, :N, :1], b[:, 1:]), lambda b: (b[:, 1:], b[:, :N]), lambda b: (b[:, 1:], b[:, 1:]), lambda b: (b[:, 1:], b[:, 1:2].expand(1, N, H)),
+                 lambda b: (b[:, 1:2].expand(1, N, H), b[:, -1:].expand(1, N, H))):
         a, want = buf.clone(), buf.clone()
-        ref = want[:, :N].clone()
+        ref = want[:, 1:].clone()
         out_ref = megacrn_amd.gated_linear_recurrence_step(*(t.clone() for t in pick(want)), ref)
-        out = megacrn_amd.gated_linear_recurrence_step(*pick(a), a[:, :N])
-        assert torch.equal(out, out_ref) and torch.equal(a[:, :N], ref) and torch.equal(a[:, N:], buf[:, N:])
+        out = megacrn_amd.gated_linear_recurrence_step(*pick(a), a[:, 1:])
+        assert torch.equal(out, out_ref) and torch.equal(a[:, 1:], ref) and torch.equal(a[:, :1], buf[:, :1])
 
 
 @pytest.mark.gpu
