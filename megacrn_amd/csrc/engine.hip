@@ -3033,8 +3033,8 @@ int mcrn_adamw_step(const mcrn_adamw_t* a, void* const* params, const void* cons
                     unsigned char* v_scale, float* master, void* ws, size_t ws_bytes, float* total_norm, void* stream) {
     ENTER();
     if (!adamw_ok(a, numel)) FAIL("adamw_step: bad number of tensors, sizes, type or state_bits");
-    if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1 && a->eps >= 1.2e-38 && a->eps < 3e38 && a->grad_scale > 0 && a->grad_scale < 3e38))
-        FAIL("adamw_step: betas in [0, 1), eps >= 1.2e-38 and grad_scale > 0 are needed");
+    if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1 && a->eps >= 1.2e-38 && a->eps < 3e38 && a->grad_scale > 0 && a->grad_scale < 3e38) || isnan(a->max_norm))
+        FAIL("adamw_step: betas in [0, 1), eps >= 1.2e-38, grad_scale > 0 and a max_norm that is a number are needed");
     if (!params || !grads || !lr || !weight_decay || !step || !m || !v || !ws) FAIL("adamw_step: a null pointer");
     if (a->state_bits == 8 && (!m_scale || !v_scale)) FAIL("adamw_step: 8-bit moments need their scales");
     if (a->dtype == MCRN_T_BF16 && !master) FAIL("adamw_step: bf16 parameters need fp32 masters");

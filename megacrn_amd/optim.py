@@ -51,6 +51,8 @@ class AdamW:
         for g in self.param_groups:
             if not (g["lr"] >= 0 and g["weight_decay"] >= 0):
                 raise ValueError("AdamW: lr and weight_decay must not be negative")
+        if max_grad_norm != max_grad_norm:
+            raise ValueError("AdamW: max_grad_norm is NaN")
         first = self.params[0]
         for p in self.params:
             if not isinstance(p, torch.Tensor) or p.dtype not in (torch.float32, torch.bfloat16) or p.dtype != first.dtype:

@@ -93,6 +93,7 @@ P = torch.nn.Parameter
 @pytest.mark.parametrize("params,kw,kind", [
     ([], {}, ValueError), ([torch.zeros(3)], dict(state_bits=16), ValueError), ([torch.zeros(3)], dict(betas=(0.9, 1.0)), ValueError),
     ([torch.zeros(3)], dict(eps=0.0), ValueError), ([torch.zeros(3)], dict(lr=-1.0), ValueError), ([torch.zeros(3)], dict(weight_decay=-1.0), ValueError),
+    ([torch.zeros(3)], dict(max_grad_norm=float("nan")), ValueError),
     ([torch.zeros(3, dtype=torch.float16)], {}, TypeError), ([torch.zeros(3), torch.zeros(3, dtype=torch.bfloat16)], {}, TypeError),
     ([torch.zeros(3, 4).t()], {}, ValueError), (["x"], {}, TypeError), ([torch.zeros(3)], {}, RuntimeError),
 ])
@@ -400,6 +401,18 @@ def test_grad_attribute_views_and_errors():
     for broken in (dict(d, state_bits=8), dict(d, m=d["m"][:-1]), dict(d, steps=[1]), dict(d, groups=[]), dict(d, steps=[1, -1, 1])):
         with pytest.raises(ValueError):
             opt.load_state_dict(broken)
+
+
+@pytest.mark.gpu
+def test_a_norm_that_is_no_number_is_refused():
+    """Set later, it would switch the clipping off."""
+    import megacrn_amd
+    p = torch.ones(5, device="cuda")
+    opt = megacrn_amd.AdamW([p], max_grad_norm=1.0)
+    opt.max_grad_norm = float("nan")
+    with pytest.raises(RuntimeError, match="max_norm"):
+        opt.step(grads=[torch.ones_like(p)])
+    assert opt.steps() == [0] and (p == 1).all()
 
 
 @pytest.mark.gpu
