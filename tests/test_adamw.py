@@ -298,6 +298,59 @@ def test_many_small_tensors(count, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,bits,n", [(torch.float32, 32, 66_000_321), (torch.float32, 8, 27_000_321), (torch.bfloat16, 32, 9_000_321), (torch.bfloat16, 8, 130_000_321)])
+def test_steps_that_stream_past_the_caches(dt, bits, n):
+    """Steps that move more than 256 MB (the norm's gradients with the first and the last), an aligned tensor and one that is not: every element of two
+    steps' parameters from zero moments against float64 on the device, the moments too; 8-bit codes of blocks all over the tensors against the
+    oracle's.  Bounds: those of the oracle's step, which are elementwise in its operations."""
+    import megacrn_amd
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    ps, gs = [], []
+    for k, off in ((n, 0), (n // 9, 1)):
+        for lst, std in ((ps, 1.0), (gs, 1e-3)):
+            lst.append((torch.randn(k + off, generator=gen, device="cuda") * std).to(dt)[off:])
+    opt = megacrn_amd.AdamW(ps, lr=1e-2, max_grad_norm=1.0, state_bits=bits, seed=3)
+    for step in (1, 2):
+        old = [[a[o:o + p.numel()].double() for a in opt.moments()] for p, o in zip(ps, opt.offsets)]
+        before = [(p if opt.master is None else opt.master[o:o + p.numel()]).double() for p, o in zip(ps, opt.offsets)]
+        opt.step(grads=gs)
+        norm = sum(g.double().pow(2).sum().item() for g in gs) ** 0.5
+        assert norm > 1 and abs(opt.total_norm.item() - norm) <= 1.01 * O.U * norm
+        f = 1.0 / (norm + 1e-6)
+        for i, (p, g, o) in enumerate(zip(ps, gs, opt.offsets)):
+            # O.adamw_step, its operations on device tensors
+            x, k = g.double() * f, p.numel()
+            big_m, v = 0.9 * old[i][0].abs() + 0.1 * x.abs(), 0.999 * old[i][1] + 0.001 * x * x
+            m = 0.9 * old[i][0] + 0.1 * x
+            em, ev = 5 * O.U * big_m + 2.0 ** -148, 7 * O.U * v + 2.0 ** -148
+            c = (1 - 0.999 ** step) ** 0.5
+            denom, size = v.sqrt() / c + 1e-8, 1e-2 / (1 - 0.9 ** step)
+            upd = size * m / denom
+            ed = torch.where(v > 2.0 ** -120, 0.5 * ev / v.clamp(min=2.0 ** -120).sqrt(), ev.sqrt()) / c + 4 * O.U * denom
+            ep = size / denom * em + upd.abs() * ed / denom + 4 * O.U * upd.abs() + 3 * O.U * before[i].abs()
+            got = (p if opt.master is None else opt.master[o:o + k]).double()
+            assert not ((got - (before[i] * (1 - 1e-4) - upd)).abs() > ep).any(), (step, i)
+            if opt.master is not None:
+                assert torch.equal(p, opt.master[o:o + k].to(dt))
+            if bits == 32:
+                for a, w, e in zip(opt.moments(), (m, v), (em, ev)):
+                    assert not ((a[o:o + k].double() - w).abs() > e).any(), (step, i)
+                continue
+            d, values = opt.state_dict(), opt.moments()
+            F1 = F(opt.total_norm.item()) + F(1e-6)
+            for b in [0, 1, k // 128, (k - 1) // 64 - 1, (k - 1) // 64] + list(range(7, k // 64, k // 64 // 20)):
+                at, to = b * 64, min(b * 64 + 64, k)
+                mm, vv = O.moments_f32(g[at:to].float().cpu().numpy(), old[i][0][at:to].cpu().numpy(), old[i][1][at:to].cpu().numpy(), F(1.0) / F1)
+                key = O.mix(3 + 0x9E3779B9 * (i + 1) + O.mix(step))
+                r = np.array([O.mix(q * 0x9E3779B9 + key) for q in range(at, to)], dtype=np.int64)
+                for second, q, bits16 in ((False, mm, r & 0xFFFF), (True, vv, r >> 16)):
+                    codes, scales = O.encode(q, bits16, second)
+                    name = "v" if second else "m"
+                    assert (d[name][o + at:o + to].cpu().numpy() == codes).all() and d[name + "_scale"][(o + at) // 64].item() == scales[0], (step, i, b)
+                    assert (values[second][o + at:o + to].cpu().numpy() == O.decode(codes, scales, second).astype(F)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_large_tensor_and_groups(bits):
     """Blocks of several runs (over 4 M elements), two groups with rates and decays of their own, and the same numbers whichever way
