@@ -299,6 +299,29 @@ def test_vectors_over_the_ends_of_nodes_past_the_caches():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mask", [False, True])
+@pytest.mark.parametrize("B,T,N,H,G,dt", [(4, 640, 207, 64, 64, "f32"), (4, 1300, 400, 64, 1, "bf16"), (1, 700, 3000, 33, 33, "f16"), (64, 13, 650, 64, 64, "f32")])
+def test_gradients_past_the_caches(B, T, N, H, G, dt, mask):
+    """Gradients that are more than 256 MB: some nodes (the channels of others do not reach them) against the oracle."""
+    import megacrn_amd
+    g = torch.Generator(device="cuda").manual_seed(T)
+    gate, cand, dout = ((torch.randn(B, T, N, w, generator=g, device="cuda") + m).to(TORCH[dt]) for w, m in ((G, 1.5), (H, 0.0), (H, 0.0)))
+    st, dlast = (torch.randn(B, N, H, generator=g, device="cuda") for _ in range(2))
+    keep = torch.rand(B, T, N, generator=g, device="cuda") > 0.2 if mask else None
+    leaves = [t.requires_grad_() for t in (gate, cand, st)]
+    out, last = megacrn_amd.gated_linear_recurrence(*leaves, keep)
+    grads = torch.autograd.grad((out, last), leaves, (dout, dlast))
+    assert all(torch.isfinite(t).all() for t in grads)
+    pick = [0, 1, N // 2, N - 1]
+    host = [t[..., pick, :].detach().double().cpu().numpy() for t in (gate, cand, st, dout, dlast)]
+    want, wlast, eh, cache = O.glr_fwd(*host[:3], None if keep is None else keep[:, :, pick].cpu().numpy(), "tanh", dt)
+    dg, dc, ds, eg, ec, es = O.glr_bwd(cache, *host[3:])
+    for got, w, e, t, what in ((out, want, eh, dt, "out"), (last, wlast, eh[:, -1], "f32", "last"), (grads[0], dg, eg, dt, "dgate"), (grads[1], dc, ec, dt, "dcand"),
+                               (grads[2], ds, es, "f32", "dstate")):
+        _close(got[..., pick, :], w, e + O.half_step(w, t), what)
+
+
+@pytest.mark.gpu
 def test_long_memory():
     """Gates that hardly forget (1 - a down to e^-12) over 3000 steps: 1 - a has to keep its own relative precision."""
     gate, cand, st, keep, dout, dlast = _inputs(1, 3000, 2, 12, 12, "f32", False, 5)
