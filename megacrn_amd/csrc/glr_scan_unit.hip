@@ -16,7 +16,7 @@ bool glr_plan(GlrP& p, bool backward) {
     const bool shared = D > 1;
     // Four channels a thread (16 bytes of f32, 8 of the 16-bit types), at any alignment.  A number of channels that 4 does not divide: vectors run
     // over the ends of the nodes where these lie behind one another (FLAT), else one channel a thread (3 x 3110 x 206 x 37, f32, both
-    // directions: 906 us so, 606 flat; 11 x 666 x 229 x 42, bf16, forward: 257 : 133).  FLAT's last vector reaches back over channels of the one
+    // directions: 947 us so, 611 flat; 11 x 666 x 229 x 42, bf16, forward: 269 : 149).  FLAT's last vector reaches back over channels of the one
     // before: not while `last` overwrites the state that both read.
     const long long NH = (long long)p.N * p.H;
     auto dense = [&](long long sn) { return p.N == 1 || sn == p.H; };
@@ -40,7 +40,7 @@ bool glr_plan(GlrP& p, bool backward) {
         return p.tiles * p.B;
     };
     // What is written leaves nothing of itself in the last-level cache (256 MB) when it is larger: past the caches then.  A week of 4 x 207 sensors,
-    // both directions: 611 us so, 647 without; a window of 12 steps, whose outputs the caches hold: 85 so with the loads too, 80 without.
+    // both directions: 622 us so, 652 without; a window of 12 steps, whose outputs the caches hold: 85 so with the loads too, 80 without.
     p.nt = (double)p.B * p.T * p.N * (p.H + (backward ? p.G : 0)) * size > 256e6;
     p.S = 1;
     p.first = 0;
@@ -51,12 +51,15 @@ bool glr_plan(GlrP& p, bool backward) {
     if (p.T > GLR_K && p.K == GLR_K && blocks < 512) {
         const int span = GLR_THREADS / 16 * GLR_K;
         // From here on fewer than 512 blocks of 256 channel lanes: time is cut over the lanes of a block as well.
-        //  - 64 lanes x 4 segments, the block walking its tiles: up to 32 steps, and up to 288 where that still makes 400 blocks (462 blocks, 144 steps: 26 us
-        //    forward against 36; 416, 120 steps, bf16 with gradients: 51 : 63; 1131, 162 steps: 78 : 109).  Fewer blocks leave the card idle
-        //    (260, 100 steps: 31 : 26), longer walks lose to chained tiles (675, 1000 steps with gradients: 853 : 722).
+        //  - 64 lanes x 4 segments, the block walking its tiles: up to 32 steps, and up to 288 where that still makes 400 blocks.  Fewer blocks leave the
+        //    card idle (260, 100 steps: 28.5 us forward so, 25.8 in 16 lanes; with gradients 208 blocks 53 : 50, 312 blocks 65 : 63, 432 blocks, 96
+        //    steps, 68 : 78).  How long such a walk pays depends on how many rounds the blocks take: both directions, 64 lanes : 16 lanes at 160, 224, 288, 320
+        //    and 512 steps, 432 blocks f32 109 : 138, 162 : 178, 204 : 235, 224 : 242, 349 : 365; 462 blocks bf16, a gate a node, 75 : 96, 100 : 107,
+        //    125 : 143, 139 : 153, 218 : 213; 828 blocks f32 228 : 250, 324 : 287, 415 : 404, 457 : 412, 728 : 619.  288 stands between where the last two cross.
         //  - 16 lanes x 16 segments, a block for every 128 steps, each handing its state to the next (chain), while a chunk of all blocks holds
-        //    about as much as the card reads during a hand-over (1.6 us): 64 blocks of 16 bytes a lane and step (f32, 20161 steps: 128 tiles 484 us
-        //    against 672 split, 64 tiles 321 : 351, 32 tiles 265 : 185), more of fewer bytes (f16, 14362 steps, 96 tiles, both directions: 469 : 448 split).
+        //    about as much as the card reads during a hand-over (1.6 us): 64 blocks of 16 bytes a lane and step (f32, 20161 steps, both directions, chain : split:
+        //    128 tiles 1184 us : 1531, 64 tiles 702 : 781 (forward alone 336 : 324), 32 tiles 515 : 407), more of fewer bytes (f16, 14362 steps, 128 tiles
+        //    564 : 600, 96 tiles 470 : 455).
         //  - fewer: the chunks' maps first (they need no state), then every chunk from the maps before it.  Inputs are read twice.
         const int quarter = GLR_THREADS / 64 * GLR_K;
         if (p.T <= quarter || (p.T <= 9 * quarter && cover(64) >= 400)) {
