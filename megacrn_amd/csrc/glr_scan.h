@@ -68,11 +68,12 @@ template <class X, int V> __device__ __forceinline__ void glr_only(bool on, GlrV
     }
     r = __builtin_bit_cast(GlrVec<X, V>, w);
 }
-// NT: past the caches, for sequences larger than these
-template <class X, int V, bool NT = false> __device__ __forceinline__ void glr_store(char* base, uint32_t off, const float* v) {
+// NT: past the caches, for sequences larger than these; `on`: else zeros
+template <class X, int V, bool NT = false> __device__ __forceinline__ void glr_store(char* base, uint32_t off, const float* v, bool on = true) {
     GlrVec<X, V> r;
 #pragma unroll
     for (int i = 0; i < V; ++i) r.e[i] = X::down(v[i]);
+    glr_only<X, V>(on, r);
     typedef typename GlrWord<sizeof(r)>::T T;
     typedef T Loose __attribute__((aligned(sizeof(typename X::S))));
     if (NT) __builtin_nontemporal_store(__builtin_bit_cast(T, r), reinterpret_cast<Loose*>(base + off));
@@ -697,20 +698,21 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                     dc[i] = lam * wc[k][i];
                     dg[i] = lam * q[k][i];
                     mu[i] = glr_keep(nn[k][i], lam);
-                    if (decltype(masked)::value) {         // 0, whatever lam is and the step holds
+                    if (FLAT && decltype(masked)::value) {
                         const bool o = moves.at(k, i);
                         dc[i] = o ? dc[i] : 0.f;
                         dg[i] = o ? dg[i] : 0.f;
                     }
                 }
-                if (in) glr_store<X, V, decltype(nt)::value>(pdc + k * rb, ldc, dc);
+                const bool on = FLAT || !decltype(masked)::value || moves.at(k, 0);        // masked: 0, whatever lam is and the step holds
+                if (in) glr_store<X, V, decltype(nt)::value>(pdc + k * rb, ldc, dc, on);
                 if (!SHARED) {
-                    if (in) glr_store<X, VG, decltype(nt)::value>(pdg + k * gb, ldg, dg);
+                    if (in) glr_store<X, VG, decltype(nt)::value>(pdg + k * gb, ldg, dg, on);
                 } else {
                     float s = 0.f;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) s += w.active ? dg[i] : 0.f;
-                    s = glr_lane_sum(s, p.L);
+                    for (int i = 0; i < V; ++i) s += dg[i];
+                    s = glr_lane_sum(w.active && on ? s : 0.f, p.L);
                     if (in && w.gl == 0) {
                         if (p.parts == 1) glr_store<X, 1>(pdg + k * gb, ldg, &s);
                         else p.part[((((long long)w.b * p.T + ts + k) * p.N + w.n) * p.G + w.gi) * p.parts + w.part] = s;
