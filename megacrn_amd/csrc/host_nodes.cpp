@@ -106,14 +106,16 @@ void strides_of(const Tensor& t, int64_t lead, long long* s) {
 // A view that is negative by a bit (the imaginary part of a conjugate): its memory holds the other sign
 Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // The kernels want a last dimension without gaps, and a tile's rows (128 steps at most) within 4 GB of each other: a copy where that is not so.
-Tensor rows(const Tensor& t0, int64_t lead) {
-    const Tensor t = plain(t0);
-    if (!t.defined()) return t;
+bool near(const Tensor& t, int64_t lead, int64_t width) {
     long long s[3];
     strides_of(t, lead, s);
     const long long steps = lead == 3 ? std::min<int64_t>(t.size(1), 128) : 1;
-    const bool near = ((steps - 1) * s[1] + (t.size(-2) - 1) * s[2] + t.size(-1)) * (long long)t.element_size() < (1ll << 32);
-    return (t.size(-1) == 1 || t.stride(-1) == 1) && near ? t : t.contiguous();
+    return ((steps - 1) * s[1] + (t.size(lead - 1) - 1) * s[2] + width) * (long long)t.element_size() < (1ll << 32);
+}
+Tensor rows(const Tensor& t0, int64_t lead) {
+    const Tensor t = plain(t0);
+    if (!t.defined()) return t;
+    return (t.size(-1) == 1 || t.stride(-1) == 1) && near(t, lead, t.size(-1)) ? t : t.contiguous();
 }
 
 mcrn_glr_t dims_of(const Tensor& gate, const Tensor& cand, const Tensor& mask, const Tensor& dout, int act, int64_t lead) {
@@ -195,12 +197,13 @@ std::pair<Tensor, Tensor> glr(const Tensor& gate0, const Tensor& cand0, const Op
     const char* who = "gated_linear_recurrence";
     const int act = activation_of(activation, who);
     const Tensor h0 = state.value_or(Tensor());
-    const Tensor mask = check_inputs(gate0, cand0, h0, mask0.value_or(Tensor()), who, 3);
+    Tensor mask = check_inputs(gate0, cand0, h0, mask0.value_or(Tensor()), who, 3);
     if (cand0.numel() == 0) {                              // nothing to read, or no step to take
         const Tensor last = h0.defined() ? h0.clone() : at::zeros({cand0.size(0), cand0.size(2), cand0.size(3)}, cand0.options().dtype(at::kFloat));
         return {at::empty(cand0.sizes(), cand0.options()), last};
     }
     const Tensor gate = rows(gate0, 3), cand = rows(cand0, 3);
+    if (mask.defined() && !near(mask, 3, 1)) mask = mask.contiguous();
     if (at::GradMode::is_enabled() && (gate.requires_grad() || cand.requires_grad() || (h0.defined() && h0.requires_grad()))) {
         auto r = GlrNode::apply(gate, cand, state, mask.defined() ? OptTensor(mask) : OptTensor(), (int64_t)act);
         return {r[0], r[1]};
@@ -223,11 +226,12 @@ Tensor glr_step(const Tensor& gate0, const Tensor& cand0, const OptTensor& state
     const int act = activation_of(activation, who);
     const Tensor state = state0.value_or(Tensor());
     TORCH_CHECK_VALUE(state.defined() && state.is_contiguous() && !state.is_neg(), who, ": state must be a contiguous tensor; it is advanced in place");
-    const Tensor mask = check_inputs(gate0, cand0, state, mask0.value_or(Tensor()), who, 2);
+    Tensor mask = check_inputs(gate0, cand0, state, mask0.value_or(Tensor()), who, 2);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (gate0.requires_grad() || cand0.requires_grad() || state.requires_grad())), who,
                 " is not differentiable: call it under torch.no_grad()");
     const Tensor gate = rows(apart(gate0, state), 2), cand = rows(apart(cand0, state), 2), out = at::empty(cand.sizes(), cand.options());
     if (out.numel() == 0) return out;
+    if (mask.defined() && !near(mask, 2, 1)) mask = mask.contiguous();
     const at::DeviceGuard guard(cand.device());
     const mcrn_glr_t d = dims_of(gate, cand, mask, Tensor(), act, 2);
     float* h = (float*)state.mutable_data_ptr();

@@ -657,6 +657,24 @@ def test_many_elements():
 
 
 @pytest.mark.gpu
+def test_masks_that_lie_far_apart():
+    """A mask whose nodes are 4 GB from each other is copied as the inputs are."""
+    import megacrn_amd
+    far = torch.zeros(2 ** 32 + 64, dtype=torch.bool, device="cuda").as_strided((1, 3, 2), (64, 8, 2 ** 32))
+    near = torch.tensor([[[True, False], [False, True], [True, True]]], device="cuda")
+    far.copy_(near)
+    x = torch.randn(1, 3, 2, 4, device="cuda", requires_grad=True)
+    a, b = (megacrn_amd.gated_linear_recurrence(x, x, None, m) for m in (far, near))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    assert all(torch.equal(p, q) for p, q in zip(*(torch.autograd.grad(t[0].sum(), x) for t in (a, b))))
+    states = [torch.ones(1, 2, 4, device="cuda") for _ in range(2)]
+    with torch.no_grad():
+        for st, m in zip(states, (far, near)):
+            megacrn_amd.gated_linear_recurrence_step(x[:, 1], x[:, 1], st, m[:, 1])
+    assert torch.equal(*states)
+
+
+@pytest.mark.gpu
 def test_as_many_sequences_as_a_launch_holds():
     """2^24 - 1 sequences of one channel are one launch; one more is refused before it."""
     import megacrn_amd
