@@ -25,7 +25,8 @@ class AdamW:
     `state_bits`: 32, or 8 for moments in one byte with a scale for each 64 elements, rounded at random but reproducibly by `seed`.
 
     `step()` takes `.grad` of each parameter, `step(grads=[...])` the given tensors; None leaves a tensor and its moments alone.
-    Learning rates are read from `param_groups` at each step.  `capturable=True` keeps step counts and learning rates on the
+    Learning rates and decays are read from `param_groups` at each step, `max_grad_norm` too; betas and eps are fixed.  (Not a torch.optim.Optimizer, which
+    torch's schedulers ask for: set `param_groups[i]["lr"]`, as the trainer does.)  `capturable=True` keeps step counts and learning rates on the
     device, so that a step captured into a HIP graph can be replayed; there a changed learning rate takes effect by `sync_lr()`
     outside the capture.  One optimizer belongs to one sequence of steps on one stream at a time."""
 
@@ -65,7 +66,7 @@ class AdamW:
         host.adamw_step                        # raises where the host nodes are not built
         _need_gpu(first, "AdamW")
         self.device, self.dtype = first.device, first.dtype
-        self.betas, self.eps, self.max_grad_norm = tuple(betas), float(eps), float(max_grad_norm or 0.0)
+        self._betas, self._eps, self.max_grad_norm = tuple(betas), float(eps), float(max_grad_norm or 0.0)
         self.state_bits, self.seed, self.capturable = state_bits, int(seed), bool(capturable)
         k = len(self.params)
         self._numel = (C.c_longlong * k)(*[p.numel() for p in self.params])
@@ -100,6 +101,9 @@ class AdamW:
             self.sync_lr()
         self._addresses()
 
+    betas = property(lambda self: self._betas, doc="of the constructor; step counts and moments belong to them")
+    eps = property(lambda self: self._eps, doc="of the constructor")
+
     def _addresses(self):
         self._numel_at = C.addressof(self._numel)
         self._hyper = tuple(C.addressof(a) for a in (self._lr, self._wd, self._steps)) if self._dev is None else tuple(t.data_ptr() for t in self._dev)
@@ -110,14 +114,13 @@ class AdamW:
 
     # -- learning rates
     def _read_groups(self):
-        now = [(g["lr"], g["weight_decay"]) for g in self.param_groups]
+        now = [(float(g["lr"]), float(g["weight_decay"])) for g in self.param_groups]      # (a tensor may change in place)
         if now == self._seen:
             return
         if any(not (lr >= 0 and wd >= 0) for lr, wd in now):
             raise ValueError(f"AdamW: lr and weight_decay must not be negative; the groups have {now}")
         self._seen, i = now, 0
-        for g in self.param_groups:
-            lr, wd = g["lr"], g["weight_decay"]
+        for g, (lr, wd) in zip(self.param_groups, now):
             for _ in g["params"]:
                 self._lr[i], self._wd[i] = lr, wd
                 i += 1

@@ -457,6 +457,26 @@ def test_grad_attribute_views_and_errors():
 
 
 @pytest.mark.gpu
+def test_rates_that_change_in_place_and_fixed_constants():
+    """A rate held in a tensor is read at each step, whatever happened to it in place; betas and eps cannot be set without effect."""
+    import megacrn_amd
+    p, q = torch.ones(70, device="cuda"), torch.ones(70, device="cuda")
+    g = torch.full_like(p, 0.5)
+    a, b = megacrn_amd.AdamW([p], lr=1e-2), megacrn_amd.AdamW([q], lr=1e-2)
+    rate = torch.tensor(1e-2, dtype=torch.float64)
+    a.param_groups[0]["lr"] = rate
+    for lr in (1e-2, 3e-3, 0.0):
+        rate.fill_(lr)
+        b.param_groups[0]["lr"] = lr
+        a.step(grads=[g]), b.step(grads=[g])
+        assert torch.equal(p, q)
+    for name, value in (("betas", (0.5, 0.9)), ("eps", 1e-3)):
+        with pytest.raises(AttributeError):
+            setattr(a, name, value)
+    assert a.betas == (0.9, 0.999) and a.eps == 1e-8
+
+
+@pytest.mark.gpu
 def test_a_norm_that_is_no_number_is_refused():
     """Set later, it would switch the clipping off."""
     import megacrn_amd
