@@ -146,13 +146,6 @@ __device__ __forceinline__ float glr_gate(float g) {
     const float e = glr_exp(-fabsf(g));
     return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
 }
-// the same, w, and p = a w
-__device__ __forceinline__ void glr_gate(float g, float& n, float& w, float& p) {
-    const float e = glr_exp(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
-    n = copysignf(s, g);
-    w = g >= 0.f ? s : r;
-    p = s * r;
-}
 constexpr float GLR_HOLD = -1.f;
 __device__ __forceinline__ bool glr_open(float n) { return (int)__float_as_uint(n) >= 0; }
 // Open: x, closed: y - by the sign's mask and one bit-select (the empty statement keeps the compiler from comparing, twice, and selecting through VCC)
@@ -161,6 +154,9 @@ __device__ __forceinline__ float glr_pick(float n, float x, float y) {
     asm("" : "+v"(closed));
     return __uint_as_float(((unsigned)closed & __float_as_uint(y)) | (~(unsigned)closed & __float_as_uint(x)));
 }
+// w = 1 - a, and a w: the larger one of a and w has all its bits as 1 - |n|
+__device__ __forceinline__ float glr_w(float n) { return glr_pick(n, 0.f, 1.f) + n; }
+__device__ __forceinline__ float glr_aw(float n) { return fmaf(-fabsf(n), fabsf(n), fabsf(n)); }
 // a x
 __device__ __forceinline__ float glr_keep(float n, float x) { return fmaf(-n, x, glr_pick(n, x, 0.f)); }
 constexpr float GLR_2L2E = 2.88539004325866699219f;        // 2 log2(e)
@@ -606,14 +602,11 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                     rs = glr_load<GlrF32, V>(reinterpret_cast<const char*>(at), (uint32_t)(hoff * 4) + (uint32_t)(p.dtype == GLR_F32 ? w.seg * K : w.seg) * (uint32_t)(NH * 4));
                 }
             }
-            float ww[K][V];                                // 1 - a
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    if (SHARED && i) { nn[k][i] = nn[k][0]; ww[k][i] = ww[k][0]; q[k][i] = q[k][0]; }
-                    else if (AGG) nn[k][i] = glr_gate(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
-                    else glr_gate(glr_up<X, VG>(rg[k], SHARED ? 0 : i), nn[k][i], ww[k][i], q[k][i]);
+                    nn[k][i] = (SHARED && i) ? nn[k][0] : glr_gate(glr_up<X, VG>(rg[k], SHARED ? 0 : i));
                     if (!AGG) wc[k][i] = glr_up<X, V>(rc[k], i);
                 }
             if (p.mask || !full) {
@@ -640,10 +633,10 @@ __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
                 for (int k = 0; k < K; ++k)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float c = wc[k][i], diff = glr_diff(nn[k][i], c, h[i]);
-                        q[k][i] *= -diff;
-                        h[i] = glr_next(nn[k][i], c, h[i], diff);
-                        wc[k][i] = p.act ? ww[k][i] * fmaf(-c, c, 1.f) : ww[k][i];
+                        const float n = nn[k][i], c = wc[k][i], diff = glr_diff(n, c, h[i]);
+                        q[k][i] = glr_aw(n) * -diff;
+                        h[i] = glr_next(n, c, h[i], diff);
+                        wc[k][i] = p.act ? glr_w(n) * fmaf(-c, c, 1.f) : glr_w(n);
                         GLR_HERE(q[k][i]);
                         GLR_HERE(wc[k][i]);
                     }

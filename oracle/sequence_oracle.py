@@ -10,7 +10,7 @@ U = 2.0 ** -24
 #   beyond 17: exponential up to 7, the others exact); the larger one enters as 1 - that, so what it multiplies is off by the smaller one's error
 #   and a rounding of the result
 #   tanh <= 12: exponential 4 (its weight is at most 1 where the quotient is used), difference 1, sum 3, reciprocal 2, product 1, one spare
-#   a w <= 17: the smaller one 10, the other 5, product 1, one spare
+#   a w <= 17: the smaller one's 10 times (1 - 2 n) / (1 - n) <= 1, product and sum 2, spare
 # of inputs of any type: they are converted to fp32 first.
 KW, KC, KP = 10, 12, 17
 
