@@ -184,8 +184,9 @@ int mcrn_flat_clip_adam(float* p, float* g, float* m, float* v, long long n, flo
  * gate (B,T,N,G), cand (B,T,N,H), G divides H (gate j is shared by the channels j*H/G .. (j+1)*H/G - 1), mask (B,T,N) bytes
  * or NULL: any strides (in elements, >= 0) over B, T and N, the last dimension of gate and cand contiguous.  state (B,N,H)
  * fp32 or NULL (zeros).  out (B,T,N,H) of the inputs' type, last (B,N,H) fp32.  Arithmetic and states are fp32.
- * B, T, N may be 0.  T <= 2^30, at most 2^24 - 1 blocks a launch (a block for 256 vectors of 4 channels of a sequence, at least one a sequence); rows and nodes within a tile of at most 128 steps lie within 4 GB (strides of less than that).  `ws` belongs to
- * the call until its kernels have run; it needs no initial contents. */
+ * B, T, N may be 0.  T <= 2^30, at most 2^24 - 1 blocks a launch (one for 1024 channels of a sequence, at least one a sequence); rows and nodes
+ * within a tile of at most 128 steps lie within 4 GB (strides of less than that).  States that are not finite: a masked step keeps them as they
+ * are; one that moves them leaves infinities or NaN.  `ws` belongs to the call until its kernels have run; it needs no initial contents. */
 #define MCRN_T_F32 0
 #define MCRN_T_BF16 1
 #define MCRN_T_F16 2

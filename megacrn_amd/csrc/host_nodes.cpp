@@ -3,7 +3,7 @@
 //
 // Why C++: a node written in Python costs 175 us of host time for a forward and a backward pass (its backward runs on the autograd
 // engine's thread and waits for the interpreter lock), this one 45 - 75 (8 for the forward; the rest is the engine's hand-over between its
-// threads), where the kernels of a METR-LA training window take 60.  A serving step: 18 us before, 4.5 now.
+// threads), where the kernels of a METR-LA training window take 60.  A serving step: 18 us before, 4.8 now.
 // The library is not linked: `bind` takes the addresses of its entry points from the one that Python has loaded.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/jit/frontend/tracer.h>
