@@ -78,7 +78,7 @@ def traffic_profile(config_name, dtype, profiles_dir=None, build_id=None):
     """(table, source) - the committed PMC traffic table of this config and arithmetic (tools/pmc_traffic.sh): per kernel the
     FETCH_SIZE x 2 + WRITE_SIZE bytes per launch averaged over the dispatches of ONE steady-state train step (the window
     between the last two k_clip_adam dispatches of the run: no autotuner candidates, no warm-up), and `_step` = their sum.
-    The table of the NEWEST profiles/r<NN>/ that holds one is taken, and only if it was measured on THIS build of the library
+    The table in profiles/current/ is taken, else that of the NEWEST profiles/r<NN>/ that holds one, and only if it was measured on THIS build of the library
     (`_meta.build_id` == mcrn_build_id()): bytes of another build divided by this run's time would be a number about nothing.
     table is None when no table exists or the newest one is stale; source says which ({"file", "status", ...})."""
     profiles_dir = profiles_dir or PROFILES_DIR
@@ -86,8 +86,8 @@ def traffic_profile(config_name, dtype, profiles_dir=None, build_id=None):
     suffix = "" if dtype == DEFAULT_PREC[config_name] else f"_{dtype}"
     rounds = []
     for d in os.listdir(profiles_dir) if os.path.isdir(profiles_dir) else []:
-        if d[:1] == "r" and d[1:].isdigit() and os.path.exists(os.path.join(profiles_dir, d, f"traffic_{config_name}{suffix}.json")):
-            rounds.append((int(d[1:]), d))
+        if (d == "current" or d[:1] == "r" and d[1:].isdigit()) and os.path.exists(os.path.join(profiles_dir, d, f"traffic_{config_name}{suffix}.json")):
+            rounds.append((float("inf") if d == "current" else int(d[1:]), d))
     if not rounds:
         return None, {"status": "absent"}
     rd = max(rounds)[1]

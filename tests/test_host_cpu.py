@@ -85,6 +85,21 @@ def test_build_id_ties_measured_artefacts_to_the_library(tmp_path, monkeypatch):
     assert bench.tile_cache_current("syn8192", 32, "bf16") and bench.import_tile_cache("syn8192", 32, "bf16")
 
 
+def test_traffic_table_of_the_current_build_stands_apart(tmp_path):
+    """profiles/current/ holds the tables of the build at hand and goes before the dated ones, which stay what they were."""
+    import json
+    import bench
+    prof = tmp_path / "profiles"
+    for d, bid in (("r6", "a" * 16), ("r10", "b" * 16), ("current", "c" * 16)):
+        (prof / d).mkdir(parents=True)
+        json.dump({"_step": {"fabric_bytes": 1.0}, "_meta": {"build_id": bid}}, open(prof / d / "traffic_metrla.json", "w"))
+    table, src = bench.traffic_profile("metrla", "bf16x3", str(prof), "c" * 16)
+    assert table is not None and src["file"].endswith("current/traffic_metrla.json")
+    assert bench.traffic_profile("metrla", "bf16x3", str(prof), "b" * 16)[0] is None
+    (prof / "current" / "traffic_metrla.json").unlink()
+    assert bench.traffic_profile("metrla", "bf16x3", str(prof), "b" * 16)[0] is not None
+
+
 def test_flat_plane_sets_have_an_opt_out():
     """ADVICE (round 5): the per-cell gradient plane sets of the small graphs (ModelPlan::flat, up to 8 GB of workspace) can be switched
     off for smaller parts: MCRN_FLAT_SETS=0, read at plan time in a fresh process."""
