@@ -353,7 +353,7 @@ __global__ void glr_clear_kernel(unsigned* __restrict__ words, long long tickets
 // 4 transcendental ones (gate 8, tanh 11, map 8, the rest loads, scan and stores).  fp32 states ask for them: of a month's 254 us a tanh without its
 // polynomial saved 27, maps from 1 - a alone 11, an exponential without its rest 5.  Four waves a SIMD (128 registers) hide loads and hand-overs
 // without a second set of buffers, which would halve them.  Measured (MI355X, a large copy runs at 6.2 TB/s): a week of
-// 4 x 207 sensors, f32, 1.28 GB in 219 us = 5.8 TB/s; a month of 325 sensors, bf16, 1.12 GB in 244 us = 4.6 TB/s; a window of 64 x 12 x 207, f32, 122 MB
+// 4 x 207 sensors, f32, 1.28 GB in 219 us = 5.8 TB/s; a month of 325 sensors, bf16, 1.12 GB in 242 us = 4.6 TB/s; a window of 64 x 12 x 207, f32, 122 MB
 // in 24 us.
 // WALK: the block walks its chunk tile by tile, from the state that the maps of the chunks before it give (one chunk: from h0).
 // AGG: only the chunk's map is wanted (agg[chunk][b][A | X][N*H]).  CHAIN: the chunk is one tile, its state comes from the block before.
@@ -527,7 +527,7 @@ __device__ __forceinline__ float glr_lane_sum(float s, int L) {
 // Bound: bytes.  The states are not read but run again from the one before each K-th step (out for f32, kept apart for 16-bit types): 3 1/8 rows in
 // and 2 out instead of 4 and 2, and the 16-bit types' states come in fp32.  Two waves a SIMD: four values of 8 steps x 4 channels stay in
 // registers between the scan and the second run (a third wave would spill).  Measured: the week above 2.19 GB in 396 us = 5.5 TB/s, the
-// window 208 MB in 39 us = 5.3 TB/s.
+// window 208 MB in 35 us = 5.9 TB/s.
 // Walks the time axis from its end; `carry` is mu_{t+1} = a_{t+1} lam_{t+1}, what reaches step t from the steps behind it.
 template <class X, int V, int K, int CL, int GATES, int MODE>
 __global__ __launch_bounds__(GLR_THREADS, 2) void glr_bwd_kernel(GlrP p) {
