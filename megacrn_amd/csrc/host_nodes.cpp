@@ -200,6 +200,10 @@ std::pair<Tensor, Tensor> glr(const Tensor& gate0, const Tensor& cand0, const Op
     Tensor mask = check_inputs(gate0, cand0, h0, mask0.value_or(Tensor()), who, 3);
     if (cand0.numel() == 0) {                              // nothing to read, or no step to take
         const Tensor last = h0.defined() ? h0.clone() : at::zeros({cand0.size(0), cand0.size(2), cand0.size(3)}, cand0.options().dtype(at::kFloat));
+        if (at::GradMode::is_enabled() && (gate0.requires_grad() || cand0.requires_grad())) {      // a backward pass finds its way: gradients of no elements
+            const Tensor out = cand0 + gate0.sum(-1, true);
+            return {out, last + out.sum(1, false, at::kFloat)};
+        }
         return {at::empty(cand0.sizes(), cand0.options()), last};
     }
     const Tensor gate = rows(gate0, 3), cand = rows(cand0, 3);

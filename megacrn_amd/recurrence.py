@@ -51,7 +51,10 @@ class AGLRCell(nn.Module):
         self.gate_cand = AGCN(dim_in, 2 * dim_out, cheb_k)
 
     def _products(self, x, supports):
-        y = self.gate_cand(x, supports)
+        if x.shape[0] == 0:                       # no batch, or no step
+            y = x.new_empty(0, x.shape[1], 2 * self.hidden_dim)
+        else:
+            y = self.gate_cand(x, supports)
         return y[..., :self.hidden_dim], y[..., self.hidden_dim:]
 
     def forward(self, x, state, supports, mask=None):

@@ -439,6 +439,37 @@ def test_empty(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 0, 3, 8), (0, 5, 3, 8), (2, 5, 0, 8)])
+def test_backward_of_empty_sequences(shape, dt, state):
+    """No batch, no step or no node: a loss over the outputs still has a backward pass, with gradients of no elements."""
+    import megacrn_amd
+    B, T, N, H = shape
+    gate, cand = (torch.zeros(B, T, N, w, dtype=TORCH[dt], device="cuda", requires_grad=True) for w in (2, H))
+    st = torch.randn(B, N, H, device="cuda", requires_grad=True) if state else None
+    out, last = megacrn_amd.gated_linear_recurrence(gate, cand, st)
+    assert out.shape == shape and out.dtype == TORCH[dt] and last.dtype == torch.float32 and torch.equal(last, torch.zeros(B, N, H, device="cuda") if st is None else st)
+    for loss in (out.float().sum(), last.sum(), out.float().sum() + last.sum()):
+        grads = torch.autograd.grad(loss, [gate, cand], retain_graph=True)
+        assert grads[0].shape == gate.shape and grads[1].shape == cand.shape
+    if state:
+        assert torch.equal(torch.autograd.grad(last.sum(), st)[0], torch.ones_like(st))
+
+
+@pytest.mark.gpu
+def test_agl_cell_without_batch_or_steps():
+    import megacrn_amd
+    cell = megacrn_amd.AGLRCell(5, 3, 8, 3).cuda()
+    sup = [torch.eye(5, device="cuda")] * 2
+    for B, T in ((0, 4), (2, 0)):
+        st = torch.randn(B, 5, 8, device="cuda")
+        out, last = cell(torch.zeros(B, T, 5, 3, device="cuda"), st, sup)
+        assert out.shape == (B, T, 5, 8) and torch.equal(last, st)
+    assert cell.step(torch.zeros(0, 5, 3, device="cuda"), torch.zeros(0, 5, 8, device="cuda"), sup).shape == (0, 5, 8)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("G", [24, 3, 1])
 def test_steps_are_the_sequence(dt, G):
