@@ -279,8 +279,9 @@ void adamw_step(uintptr_t cfg_at, const std::vector<Tensor>& params, const std::
     auto count = [&](int by) {
         if (!cfg->on_device)
             for (size_t i = 0; i < n; ++i)
-                if (grads[i] && grads[i]->defined()) step[i] += by;
+                if (grads[i] && grads[i]->defined() && numel[i]) step[i] += by;      // as the device counts: a tensor without elements has no updates
     };
+    if (m.numel() == 0) return;                            // no tensor has any
     call("mcrn_adamw_step", [&] {
         count(1);
         const int rc = api.adamw_step(cfg, p.data(), g.data(), numel, reinterpret_cast<const double*>(lr), reinterpret_cast<const double*>(wd), step,
@@ -296,6 +297,7 @@ void adamw_step(uintptr_t cfg_at, const std::vector<Tensor>& params, const std::
 std::pair<Tensor, Tensor> adamw_unpack(const Tensor& m, const Tensor& ms, const Tensor& v, const Tensor& vs) {
     const at::DeviceGuard guard(m.device());
     const Tensor om = at::empty(m.sizes(), m.options().dtype(at::kFloat)), ov = at::empty(v.sizes(), v.options().dtype(at::kFloat));
+    if (m.numel() == 0) return {om, ov};
     auto bytes = [](const Tensor& t) { return (const unsigned char*)t.const_data_ptr(); };
     call("mcrn_adamw_unpack", [&] {
         return api.adamw_unpack(bytes(m), bytes(ms), bytes(v), bytes(vs), m.numel(), (float*)om.mutable_data_ptr(), (float*)ov.mutable_data_ptr(), stream_of(m));

@@ -457,6 +457,23 @@ def test_grad_attribute_views_and_errors():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_without_elements(bits, capturable):
+    """Alone they make a step that does nothing; beside others they have no updates, whoever counts."""
+    import megacrn_amd
+    e, p = torch.zeros(0, 4, device="cuda"), torch.ones(5, device="cuda")
+    opt = megacrn_amd.AdamW([e], state_bits=bits, max_grad_norm=1.0, capturable=capturable)
+    opt.step(grads=[torch.zeros_like(e)])
+    assert opt.steps() == [0] and all(t.numel() == 0 for t in opt.moments())
+    opt.load_state_dict(opt.state_dict())
+    opt = megacrn_amd.AdamW([e, p], state_bits=bits, max_grad_norm=1.0, capturable=capturable)
+    for _ in range(2):
+        opt.step(grads=[torch.zeros_like(e), torch.ones_like(p)])
+    assert opt.steps() == [0, 2] and (p < 1).all()
+
+
+@pytest.mark.gpu
 def test_rates_that_change_in_place_and_fixed_constants():
     """A rate held in a tensor is read at each step, whatever happened to it in place; betas and eps cannot be set without effect."""
     import megacrn_amd
