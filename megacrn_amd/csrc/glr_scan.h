@@ -147,7 +147,6 @@ __device__ __forceinline__ float glr_gate(float g) {
     return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
 }
 constexpr float GLR_HOLD = -1.f;
-__device__ __forceinline__ bool glr_open(float n) { return (int)__float_as_uint(n) >= 0; }
 // Open: x, closed: y - by the sign's mask and one bit-select (the empty statement keeps the compiler from comparing, twice, and selecting through VCC)
 __device__ __forceinline__ float glr_pick(float n, float x, float y) {
     int closed = (int)__float_as_uint(n) >> 31;
@@ -169,8 +168,8 @@ __device__ __forceinline__ float glr_tanh(float u) {
     return fabsf(u) < 0.375f ? fmaf(u * q, s, u) : far;
 }
 
-// c - h, what a step goes towards; where it goes nowhere (n = 0: a gate that is wholly open) an infinite state stays what it is
-__device__ __forceinline__ float glr_diff(float n, float c, float h) { return c - (n == 0.f && glr_open(n) ? 0.f : h); }
+// c - h, what a step goes towards; where it goes nowhere (n = +0: a gate that is wholly open) an infinite state stays what it is
+__device__ __forceinline__ float glr_diff(float n, float c, float h) { return c - (__float_as_uint(n) == 0u ? 0.f : h); }
 // a h + w c, as h + w (c - h) or as c - a (c - h)
 __device__ __forceinline__ float glr_next(float n, float c, float h, float diff) { return fmaf(n, diff, glr_pick(n, h, c)); }
 

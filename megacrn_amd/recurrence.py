@@ -30,7 +30,8 @@ def gated_linear_recurrence(gate, cand, state=None, mask=None, activation="tanh"
     has the inputs' type, `last` (B, N, H) is the float32 state behind the last step (T = 0: the state itself).
 
     Strided inputs (slices of one product, expanded masks) are read in place as long as the last dimension is contiguous.
-    Differentiable in gate, cand and state, once and in reverse mode (dual tensors and traces are refused).  A backward pass inside a graph capture wants leaves that no eager graph holds."""
+    Differentiable in gate, cand and state, once and in reverse mode (dual tensors and traces are refused).  A backward pass inside
+    a graph capture wants leaves that no eager graph holds."""
     return host.glr(gate, cand, state, mask, activation)
 
 
